@@ -387,6 +387,83 @@ int tnx_conv2d_forward(const tnx_conv2d_problem* problem, const tnx_config* conf
                        void* workspace, size_t workspace_bytes, int32_t* status_word,
                        void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Mixture of experts: routing, the experts' gated products, and the norms around a block.  None
+ * of these has a counterpart in the reference; they extend tnx_swiglu_mlp to layers with many
+ * expert MLPs of which each token uses a few.
+ * ------------------------------------------------------------------------------------------- */
+
+#define TNX_SCORE_SOFTMAX 0
+#define TNX_SCORE_SIGMOID 1
+
+/*
+ * Routing.  Per token: s = softmax(l) or sigmoid(l) over the experts; experts are chosen by
+ * c = s + bias.  Experts form `groups` groups of consecutive ones; only those of the `top_groups`
+ * groups whose two best c have the largest sum can be chosen.  ids = the top_k by c, best first,
+ * ties to the lowest index; weights = scale * s[ids], divided by the sum of s[ids] when
+ * `renormalize` is set (0 when that sum is 0).  Which experts are chosen is decided as in 64-bit
+ * arithmetic.  A NaN logit ranks below every other; ids are always distinct and in range.
+ */
+typedef struct tnx_route_problem {
+  int32_t tokens, experts; /* experts <= 512                                               */
+  int32_t top_k;           /* <= 32 and <= the experts of top_groups groups                */
+  int32_t groups;          /* divides experts, <= 32; 1 = no groups                        */
+  int32_t top_groups;      /* 1 .. groups                                                  */
+  int32_t scoring;         /* TNX_SCORE_*                                                  */
+  int32_t renormalize;
+  int32_t dtype;           /* of the logits and of their gradient                          */
+  float scale;
+  int32_t reserved0;
+  int64_t stride_logits;   /* elements between the logits of two tokens (inner stride 1)   */
+} tnx_route_problem;
+
+/* logits [tokens, experts]; bias fp32[experts] or NULL; weights fp32[tokens, top_k]; ids int32
+ * [tokens, top_k]. */
+int tnx_route_experts(const tnx_route_problem* problem, const void* logits, const float* bias, float* weights,
+                      int32_t* ids, void* stream);
+/* dlogits [tokens, experts] (contiguous) from dweights; ids as the forward call wrote them.  The
+ * bias only takes part in the choice and has no gradient. */
+int tnx_route_experts_backward(const tnx_route_problem* problem, const void* logits, const int32_t* ids,
+                               const float* dweights, void* dlogits, void* stream);
+
+/* Forms of the gate of tnx_gated_residual_norm. */
+#define TNX_GATE_NONE 0
+#define TNX_GATE_CHANNEL 1 /* [cols]                                      */
+#define TNX_GATE_TOKEN 2   /* one value per row, stride_gate elements apart */
+#define TNX_GATE_FULL 3    /* [rows, cols], row pitch stride_gate          */
+
+/*
+ * The seam between two blocks:
+ *   h = residual_scale * residual + gate * (y / rms(y)) * post_weight
+ *   n = (h / rms(h)) * pre_weight                 rms(v) = sqrt(mean(v^2) + eps) over a row
+ * y is the finished block's output, h the new residual stream, n the next block's input (computed
+ * from h before it is rounded).  h and n are contiguous; statistics and arithmetic are fp32.
+ */
+typedef struct tnx_norm_problem {
+  int32_t rows, cols;   /* cols <= 16384 */
+  int32_t dtype;        /* of y, residual, h, n and their gradients                   */
+  int32_t weight_dtype; /* of the weights, the gate and their gradients: dtype or TNX_F32 */
+  int32_t gate_form;    /* TNX_GATE_* */
+  float residual_scale, eps;
+  int32_t reserved0;
+  int64_t stride_y, stride_residual, stride_gate; /* row pitches in elements */
+} tnx_norm_problem;
+
+/* stats: fp32[rows, 2], the reciprocal norms of y and h for the backward call; NULL = not kept. */
+int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, const void* residual,
+                            const void* post_weight, const void* pre_weight, const void* gate, void* h, void* n,
+                            float* stats, void* stream);
+/* Bytes of workspace the backward call needs. */
+int64_t tnx_gated_residual_norm_workspace(const tnx_norm_problem* problem);
+/* Gradients of every input from those of h and n (row pitches stride_dh, stride_dn).  dy and
+ * dresidual [rows, cols], dpost and dpre [cols], dgate in the gate's form, all contiguous.
+ * Column sums are added in a fixed order. */
+int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void* dh, int64_t stride_dh,
+                                     const void* dn, int64_t stride_dn, const void* y, const void* residual,
+                                     const void* post_weight, const void* pre_weight, const void* gate,
+                                     const float* stats, void* dy, void* dresidual, void* dpost, void* dpre,
+                                     void* dgate, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,72 @@
+"""What the C entry points of routing and the norm refuse, without a device."""
+import ctypes
+
+import pytest
+
+from tritonix_b200 import _cabi
+
+lib = _cabi.lib
+PTR = 1 << 20  # never dereferenced: every call here is refused before a launch
+
+
+def route(**kw):
+    p = _cabi.RouteProblem(tokens=4, experts=64, top_k=4, groups=1, top_groups=1, scoring=0, renormalize=1,
+                           dtype=_cabi.F32, scale=1.0, stride_logits=64)
+    for key, value in kw.items():
+        setattr(p, key, value)
+    return p
+
+
+@pytest.mark.parametrize("bad", [dict(tokens=-1), dict(experts=0), dict(experts=513), dict(top_k=0), dict(top_k=33),
+                                 dict(experts=8, top_k=9), dict(groups=0), dict(groups=5), dict(groups=64, top_groups=4),
+                                 dict(groups=8, top_groups=0), dict(groups=8, top_groups=9),
+                                 dict(groups=32, top_groups=1), dict(scoring=2), dict(dtype=3), dict(stride_logits=-1)])
+def test_route_refuses(bad):
+    p = route(**bad)
+    assert lib.tnx_route_experts(ctypes.byref(p), PTR, None, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert lib.tnx_route_experts_backward(ctypes.byref(p), PTR, PTR, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert _cabi.last_error()
+
+
+def test_route_null_and_empty():
+    assert lib.tnx_route_experts(None, PTR, None, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert lib.tnx_route_experts(ctypes.byref(route()), None, None, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert lib.tnx_route_experts_backward(ctypes.byref(route()), PTR, None, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert lib.tnx_route_experts(ctypes.byref(route(tokens=0)), None, None, None, None, None) == _cabi.OK
+
+
+def norm(**kw):
+    p = _cabi.NormProblem(rows=4, cols=64, dtype=_cabi.BF16, weight_dtype=_cabi.BF16, gate_form=0,
+                          residual_scale=1.0, eps=1e-6, stride_y=64, stride_residual=64, stride_gate=64)
+    for key, value in kw.items():
+        setattr(p, key, value)
+    return p
+
+
+def forward(p, y=PTR, gate=PTR):
+    return lib.tnx_gated_residual_norm(ctypes.byref(p), y, PTR, PTR, PTR, gate, PTR, PTR, None, None)
+
+
+def backward(p, workspace=PTR, nbytes=1 << 30, stats=PTR, dgate=PTR):
+    return lib.tnx_gated_residual_norm_backward(ctypes.byref(p), PTR, 64, PTR, 64, PTR, PTR, PTR, PTR, PTR, stats, PTR,
+                                                PTR, PTR, PTR, dgate, workspace, nbytes, None)
+
+
+@pytest.mark.parametrize("bad", [dict(rows=-1), dict(cols=0), dict(cols=16385), dict(dtype=4), dict(weight_dtype=_cabi.F16),
+                                 dict(gate_form=4), dict(eps=0.0), dict(eps=float("nan")), dict(stride_y=-64)])
+def test_norm_refuses(bad):
+    assert forward(norm(**bad)) == _cabi.ERR_INVALID
+    assert backward(norm(**bad)) == _cabi.ERR_INVALID
+
+
+def test_norm_null_and_workspace():
+    assert forward(norm(), y=None) == _cabi.ERR_INVALID
+    assert forward(norm(gate_form=1), gate=None) == _cabi.ERR_INVALID
+    assert backward(norm(), stats=None) == _cabi.ERR_INVALID
+    assert backward(norm(gate_form=2), dgate=None) == _cabi.ERR_INVALID
+    need = lib.tnx_gated_residual_norm_workspace(ctypes.byref(norm()))
+    assert need == 4 * 2 * 64 * 4
+    assert lib.tnx_gated_residual_norm_workspace(ctypes.byref(norm(gate_form=1))) == 4 * 3 * 64 * 4
+    assert backward(norm(), nbytes=need - 1) == _cabi.ERR_INVALID
+    assert backward(norm(), workspace=PTR + 4) == _cabi.ERR_INVALID
+    assert forward(norm(rows=0), y=None) == _cabi.OK

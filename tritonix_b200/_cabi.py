@@ -101,6 +101,21 @@ class MlpExchange(ctypes.Structure):
                 ("signal_multicast", ctypes.c_void_p), ("signal_local", ctypes.c_void_p)]
 
 
+class RouteProblem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "experts", "top_k", "groups", "top_groups",
+                                              "scoring", "renormalize", "dtype")] + \
+        [("scale", ctypes.c_float), ("reserved0", ctypes.c_int32), ("stride_logits", ctypes.c_int64)]
+
+
+class NormProblem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "cols", "dtype", "weight_dtype", "gate_form")] + \
+        [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float), ("reserved0", ctypes.c_int32)] + \
+        [(n, ctypes.c_int64) for n in ("stride_y", "stride_residual", "stride_gate")]
+
+
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = range(4)
+
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
 WEIGHT_KCRS, WEIGHT_PACKED = 0, 1
 
@@ -108,7 +123,9 @@ EXPORTS = ("tnx_version", "tnx_last_error", "tnx_sm_count", "tnx_gemm_query", "t
            "tnx_glu", "tnx_read_status", "tnx_gemm_splitk_static", "tnx_selftest_bounded_wait",
            "tnx_conv2d_query", "tnx_conv2d_forward", "tnx_conv2d_packed_weight_bytes",
            "tnx_conv2d_pack_weights", "tnx_swiglu_mlp_query", "tnx_swiglu_mlp",
-           "tnx_swiglu_mlp_unit_order")
+           "tnx_swiglu_mlp_unit_order", "tnx_route_experts", "tnx_route_experts_backward",
+           "tnx_gated_residual_norm", "tnx_gated_residual_norm_workspace",
+           "tnx_gated_residual_norm_backward")
 STATIC_SCRATCH_BYTES = 16 * 1024 * 1024 + 65536
 
 
@@ -169,6 +186,18 @@ def _load() -> ctypes.CDLL:
                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                        ctypes.c_void_p, ctypes.c_void_p]
+    ptr = ctypes.c_void_p
+    for name, problem, args in (
+            ("tnx_route_experts", RouteProblem, [ptr] * 5),
+            ("tnx_route_experts_backward", RouteProblem, [ptr] * 5),
+            ("tnx_gated_residual_norm", NormProblem, [ptr] * 9),
+            ("tnx_gated_residual_norm_backward", NormProblem,
+             [ptr, ctypes.c_int64, ptr, ctypes.c_int64] + [ptr] * 12 + [ctypes.c_size_t, ptr])):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(problem)] + args
+    lib.tnx_gated_residual_norm_workspace.restype = ctypes.c_int64
+    lib.tnx_gated_residual_norm_workspace.argtypes = [ctypes.POINTER(NormProblem)]
     return lib
 
 
@@ -517,6 +546,33 @@ def launch_mlp(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, y: torch.Te
                                 status_word(x.device).data_ptr(), stream)
     raise_for(rc)
     return res
+
+
+# ---------------------------------------------------------------------------------------------
+# Mixture of experts, norms
+# ---------------------------------------------------------------------------------------------
+def call(device: torch.device, fn, *args) -> None:
+    """Calls an entry point whose last argument is the stream: on ``device``, with torch's current
+    stream of it.  The caller's current device is left as it was."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    previous = torch.cuda.current_device()
+    if idx != previous:
+        torch.cuda.set_device(idx)
+    try:
+        rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+    finally:
+        if idx != previous:
+            torch.cuda.set_device(previous)
+    if rc != OK:
+        raise_for(rc)
+
+
+def rows_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (2-D) with adjacent elements in its rows and a pitch the kernels can walk: itself
+    where that holds, a copy otherwise."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
 
 
 # ---------------------------------------------------------------------------------------------
