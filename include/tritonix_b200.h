@@ -464,6 +464,52 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
                                      const float* stats, void* dy, void* dresidual, void* dpost, void* dpre,
                                      void* dgate, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Experts' gated products:
+ *   y[t] = sum over s < top_k of  weights[t, s] * ((act(x[t].W1[e]) * (x[t].W2[e])) . W3[e])
+ * with e = ids[t, s]; a slot whose id is outside [0, experts) contributes nothing.  The same expert
+ * may stand in several slots of a token.  Sums are fp32; the hidden activation, times the
+ * routing weight, is rounded to the operands' type between the two products, the result once.
+ * Every sum has a fixed order.
+ */
+typedef struct tnx_moe_problem {
+  int32_t tokens, experts, top_k; /* experts <= 512                                              */
+  int32_t d_model, d_ff, n_out;   /* positive multiples of 8                                     */
+  int32_t dtype;                  /* TNX_F16 | TNX_BF16: x, w12, w3, y                           */
+  int32_t activation;             /* TNX_EPI_GLU_*                                               */
+  int32_t wide_ids;               /* ids are int64 instead of int32                              */
+  int32_t train;                  /* keep what tnx_moe_swiglu_backward needs in `saved`          */
+  int64_t stride_x;               /* row pitches in elements, multiples of 8                     */
+  int64_t stride_w12e, stride_w12k; /* w12: [experts][d_model][2 d_ff], W1/W2 column-interleaved */
+  int64_t stride_w3e, stride_w3k;   /* w3:  [experts][d_ff][n_out]                               */
+  int64_t stride_y;
+} tnx_moe_problem;
+
+typedef struct tnx_moe_resources {
+  int32_t tile_rows; /* rows per row tile: an expert's rows are padded to it */
+  int32_t max_tiles; /* row tiles at most                                    */
+  int64_t workspace_bytes;          /* scratch of one forward call                  */
+  int64_t saved_bytes;              /* what a training forward call keeps           */
+  int64_t backward_workspace_bytes; /* scratch of one backward call                 */
+} tnx_moe_resources;
+
+int tnx_moe_query(const tnx_moe_problem* problem, tnx_moe_resources* out);
+
+/* ids [tokens, top_k] and weights fp32[tokens, top_k] contiguous.  workspace and saved (NULL unless
+ * `train`) are 256-byte aligned; their content before the call does not matter, and calls that
+ * share a workspace must be ordered on one stream. */
+int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w12, const void* w3, const void* ids,
+                   const float* weights, void* y, void* saved, void* workspace, size_t workspace_bytes,
+                   int32_t* status_word, void* stream);
+
+/* Gradients of a training forward call whose operands are unchanged.  dx [tokens, d_model], dw12 and
+ * dw3 shaped like the weights, dweights fp32[tokens, top_k], all contiguous; NULL skips one.  The
+ * gradient of a weight matrix without rows is zero.  `saved` is only read. */
+int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int64_t stride_dy, const void* x,
+                            const void* w12, const void* w3, const void* saved, void* dx, void* dw12, void* dw3,
+                            float* dweights, void* workspace, size_t workspace_bytes, int32_t* status_word,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

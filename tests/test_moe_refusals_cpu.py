@@ -70,3 +70,62 @@ def test_norm_null_and_workspace():
     assert backward(norm(), nbytes=need - 1) == _cabi.ERR_INVALID
     assert backward(norm(), workspace=PTR + 4) == _cabi.ERR_INVALID
     assert forward(norm(rows=0), y=None) == _cabi.OK
+
+
+def moe(**kw):
+    p = _cabi.MoeProblem(tokens=10, experts=4, top_k=2, d_model=64, d_ff=32, n_out=48, dtype=_cabi.BF16,
+                         activation=_cabi.EPI_GLU_SILU, wide_ids=0, train=0, stride_x=64, stride_w12e=64 * 64,
+                         stride_w12k=64, stride_w3e=32 * 48, stride_w3k=48, stride_y=48)
+    for key, value in kw.items():
+        setattr(p, key, value)
+    return p
+
+
+def query(p):
+    res = _cabi.MoeResources()
+    return lib.tnx_moe_query(ctypes.byref(p), ctypes.byref(res)), res
+
+
+@pytest.mark.parametrize("bad", [dict(tokens=-1), dict(experts=0), dict(experts=513), dict(top_k=0), dict(d_model=60),
+                                 dict(d_ff=0), dict(n_out=4), dict(dtype=_cabi.F32), dict(activation=0),
+                                 dict(activation=4), dict(tokens=1 << 28, top_k=2), dict(stride_x=56), dict(stride_x=68),
+                                 dict(stride_w12k=56), dict(stride_w12e=64 * 64 - 8), dict(stride_w3e=0),
+                                 dict(stride_w12k=0), dict(stride_y=40), dict(d_model=1 << 21, stride_x=1 << 21),
+                                 dict(tokens=1 << 27, n_out=1 << 20, stride_y=1 << 20, stride_w3k=1 << 20,
+                                      stride_w3e=1 << 25)])
+def test_moe_refuses(bad):
+    p = moe(**bad)
+    assert query(p)[0] == _cabi.ERR_INVALID and _cabi.last_error()
+    assert lib.tnx_moe_swiglu(ctypes.byref(p), PTR, PTR, PTR, PTR, PTR, PTR, None, PTR, 1 << 40, None,
+                              None) == _cabi.ERR_INVALID
+
+
+def test_moe_resources_and_workspace():
+    rc, res = query(moe())
+    # 20 pairs on 4 experts: a tile of 128 rows for each expert, and none left over
+    assert rc == _cabi.OK and (res.tile_rows, res.max_tiles) == (128, 4)
+    part = 4 * 128 * 48 * 4
+    assert res.workspace_bytes >= part + 4 * 128 * 32 * 2
+    rc, train = query(moe(train=1))
+    assert rc == _cabi.OK and train.workspace_bytes == part and train.saved_bytes >= 4 * 128 * 32 * 10
+    assert query(moe(tokens=4000))[1].tile_rows == 256
+
+    def forward(p, nbytes, workspace=PTR, saved=None, x=PTR):
+        return lib.tnx_moe_swiglu(ctypes.byref(p), x, PTR, PTR, PTR, PTR, PTR, saved, workspace, nbytes, None, None)
+
+    assert forward(moe(), res.workspace_bytes - 1) == _cabi.ERR_INVALID
+    assert forward(moe(), res.workspace_bytes, workspace=PTR + 16) == _cabi.ERR_INVALID
+    assert forward(moe(), res.workspace_bytes, x=None) == _cabi.ERR_INVALID
+    assert forward(moe(), res.workspace_bytes, x=PTR + 2) == _cabi.ERR_INVALID
+    assert forward(moe(train=1), 1 << 30) == _cabi.ERR_INVALID                     # nothing to save into
+    assert forward(moe(tokens=0), 0, workspace=None, x=None) == _cabi.OK
+
+    def gradients(p, nbytes, dy=PTR, stride=48, workspace=PTR, saved=PTR):
+        return lib.tnx_moe_swiglu_backward(ctypes.byref(p), dy, stride, PTR, PTR, PTR, saved, PTR, PTR, PTR, PTR,
+                                           workspace, nbytes, None, None)
+
+    need = train.backward_workspace_bytes
+    for kw in (dict(nbytes=need - 1), dict(nbytes=need, workspace=PTR + 128), dict(nbytes=need, saved=PTR + 128),
+               dict(nbytes=need, saved=None), dict(nbytes=need, dy=None), dict(nbytes=need, stride=44),
+               dict(nbytes=need, stride=40), dict(nbytes=need, dy=PTR + 8)):
+        assert gradients(moe(train=1), **kw) == _cabi.ERR_INVALID

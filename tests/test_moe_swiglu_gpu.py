@@ -1,0 +1,257 @@
+"""Experts' gated products and their gradients against the 64-bit oracle."""
+import pytest
+import torch
+
+import tritonix_b200 as tnx
+from oracle import moe as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+f16, bf16, f32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def make(t, n, k, d, f, n_out, dtype, seed=0, ids=None):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    if ids is None:
+        ids = r(t, n).topk(k, dim=1).indices.to(torch.int32)
+    return {"x": r(t, d).to(dtype), "w12": (r(n, d, 2 * f) * d ** -0.5).to(dtype),
+            "w3": (r(n, f, n_out) * f ** -0.5).to(dtype), "weights": torch.softmax(r(t, k), 1), "ids": ids,
+            "dy": r(t, n_out).to(dtype)}
+
+
+def operands(case, grad=False):
+    return [case[name].to(DEV).requires_grad_(grad and name != "ids") for name in ("x", "w12", "w3", "ids", "weights")]
+
+
+def close(out, ref, roundings, name):
+    """Norm of the difference: `roundings` independent ones to the operands' type between the inputs
+    and the result, each of at most half a step relative to a value (together at most their sum),
+    and fp32 sums of a few thousand terms.  Per element: the same against the result's size, with
+    room for the largest of many."""
+    out, half = out.detach().cpu().double(), torch.finfo(out.dtype).eps / 2 if out.dtype != f32 else 0.0
+    assert out.shape == ref.shape and torch.isfinite(out).all(), name
+    norm = ref.norm()
+    bound = roundings + 2e-6
+    assert (out - ref).norm() <= bound * norm + 1e-30, f"{name}: {(out - ref).norm() / norm:.2e} > {bound:.2e}"
+    if norm > 0:
+        rms = ref.square().mean().sqrt()
+        worst = ((out - ref).abs() / (ref.abs() + rms)).max()
+        assert worst <= 8 * bound + half, f"{name}: an element is {worst:.2e} off"
+
+
+def check(case, activation="silu", train=True):
+    half = torch.finfo(case["x"].dtype).eps / 2
+    cpu = [case[n] for n in ("x", "w12", "w3", "ids", "weights")]
+    args = operands(case)
+    y = tnx.moe_swiglu(*args, activation=activation)
+    tnx.check_status(y.device)
+    want = O.experts_oracle(*cpu, activation, case["dy"] if train else None)
+    # rounded twice: the hidden activation and the result
+    close(y, want[0] if train else want, 2 * half, "y")
+    if not train:
+        return
+    leaves = operands(case, True)
+    y2 = tnx.moe_swiglu(*leaves, activation=activation)
+    assert y2.dtype == y.dtype
+    close(y2, want[0], 2 * half, "y (training)")
+    x, w12, w3, _, weights = leaves
+    grads = torch.autograd.grad(y2, [x, w12, w3, weights], case["dy"].to(DEV))
+    tnx.check_status(y.device)
+    # the gradient of the gate/up products is rounded, and the result; dw3 meets the hidden
+    # activation's rounding instead; the routing weights' gradient is fp32 throughout
+    # (exp and the division in the gate: 2^-21 each)
+    for grad, ref, name in zip(grads, want[1:], ("dx", "dw12", "dw3", "dweights")):
+        close(grad, ref, 2 * half if name != "dweights" else 2.0 ** -20, name)
+    return grads
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16])
+@pytest.mark.parametrize("t,n,k,d,f,n_out", [(1, 4, 2, 64, 64, 64), (1, 1, 1, 8, 8, 8), (5, 8, 2, 72, 40, 24),
+                                             (37, 3, 3, 200, 136, 264), (130, 16, 4, 256, 128, 256),
+                                             (300, 4, 1, 328, 200, 520), (33, 60, 6, 136, 264, 128)])
+def test_single_cta_tiles(t, n, k, d, f, n_out, dtype):
+    check(make(t, n, k, d, f, n_out, dtype, seed=t + d))
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16])
+@pytest.mark.parametrize("t,n,k,d,f,n_out", [(800, 2, 1, 136, 200, 264), (1000, 4, 2, 256, 128, 256),
+                                             (700, 1, 1, 64, 320, 72)])
+def test_cta_pairs(t, n, k, d, f, n_out, dtype):
+    check(make(t, n, k, d, f, n_out, dtype, seed=t + d))
+
+
+@pytest.mark.parametrize("activation", ["silu", "sigmoid", "none"])
+def test_activations(activation):
+    check(make(50, 4, 2, 128, 96, 64, bf16), activation)
+
+
+def test_many_pairs_use_the_chunked_plan():
+    check(make(3001, 24, 3, 64, 40, 48, bf16, seed=9))
+    check(make(2100, 7, 4, 32, 24, 40, f16, seed=4))
+
+
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+def test_ids_out_of_range_and_repeated(wide):
+    t, n, k = 90, 6, 3
+    ids = torch.randint(0, n, (t, k), generator=torch.Generator().manual_seed(1))
+    ids[::4, 0] = -1
+    ids[1::5, 1] = n
+    ids[7] = -1                      # a token no expert takes
+    ids[8] = 2                       # the same expert three times
+    ids[9] = 2 ** 31 - 1
+    if wide == torch.int64:
+        ids[10] = 2 ** 32            # would be expert 0 in 32 bits
+        ids[11] = -2 ** 40
+    case = make(t, n, k, 96, 64, 72, bf16, ids=ids.to(wide))
+    grads = check(case)
+    assert torch.equal(grads[0][7].cpu(), torch.zeros(96, dtype=bf16))
+    assert not grads[3].cpu()[(case["ids"] < 0) | (case["ids"] >= n)].any()
+    none = make(5, n, k, 96, 64, 72, bf16, ids=torch.full((5, k), -1, dtype=wide))
+    x, w12, w3, i, w = operands(none, True)
+    y = tnx.moe_swiglu(x, w12, w3, i, w)
+    assert torch.equal(y, torch.zeros_like(y))
+    for g in torch.autograd.grad(y, [x, w12, w3, w], none["dy"].to(DEV)):
+        assert torch.equal(g, torch.zeros_like(g))
+
+
+def test_one_expert_takes_all_and_others_get_zero_gradients():
+    ids = torch.zeros(400, 1, dtype=torch.int32) + 3
+    grads = check(make(400, 5, 1, 72, 64, 136, bf16, ids=ids))
+    for e in (0, 1, 2, 4):
+        assert not grads[1][e].any() and not grads[2][e].any()
+
+
+def test_no_tokens():
+    case = make(0, 4, 2, 64, 64, 64, bf16, ids=torch.empty(0, 2, dtype=torch.int32))
+    x, w12, w3, ids, w = operands(case, True)
+    y = tnx.moe_swiglu(x, w12, w3, ids, w)
+    assert y.shape == (0, 64)
+    dx, dw12, dw3, dw = torch.autograd.grad(y, [x, w12, w3, w], case["dy"].to(DEV))
+    assert dx.shape == (0, 64) and dw.shape == (0, 2) and not dw12.any() and not dw3.any()
+
+
+def test_nan_and_inf_rows_stay_their_own():
+    case = make(60, 4, 2, 64, 64, 64, bf16)
+    clean = tnx.moe_swiglu(*operands(case))
+    case["x"][13] = float("nan")
+    case["x"][21] = float("inf")
+    dirty = tnx.moe_swiglu(*operands(case))
+    keep = [i for i in range(60) if i not in (13, 21)]
+    assert torch.equal(clean[keep], dirty[keep])
+    assert torch.isnan(dirty[13]).all() and not torch.isfinite(dirty[21]).any()
+
+
+def test_strided_operands():
+    case = make(40, 4, 2, 64, 64, 72, bf16)
+    x, w12, w3, ids, w = operands(case)
+    want = tnx.moe_swiglu(x, w12, w3, ids, w)
+    pad = lambda t, n: torch.nn.functional.pad(t, (0, n))[..., :t.shape[-1]]  # noqa: E731
+    wide = lambda t: torch.stack((t, torch.full_like(t, float("nan"))), 1)[:, 0]  # noqa: E731
+    # padded rows, matrices apart, columns stored first, an odd pitch, transposed ids
+    for args in ((pad(x, 8), pad(w12, 16), pad(w3, 8), ids, w), (x, wide(w12), wide(w3), ids, w),
+                 (x.t().contiguous().t(), w12.mT.contiguous().mT, w3, ids.t().contiguous().t(), w),
+                 (pad(x, 3), pad(w12, 1), w3, ids, w.t().contiguous().t())):
+        assert torch.equal(tnx.moe_swiglu(*args), want)
+    shared = tnx.moe_swiglu(x, w12[:1].expand(4, -1, -1), w3[:1].expand(4, -1, -1), ids, w)
+    assert torch.equal(shared, tnx.moe_swiglu(x, w12[:1].repeat(4, 1, 1), w3[:1].repeat(4, 1, 1), ids, w))
+
+
+def test_gradients_of_some_operands_only_and_runs_are_bit_identical():
+    case = make(260, 8, 2, 128, 72, 136, bf16)
+    want = check(case)
+    dy = case["dy"].to(DEV)
+    for i, name in enumerate(("x", "w12", "w3", "weights")):
+        args = operands(case)
+        leaf = args[i if i < 3 else 4].requires_grad_(True)
+        (grad,) = torch.autograd.grad(tnx.moe_swiglu(*args), leaf, dy)
+        assert torch.equal(grad, want[i]), name
+    # a broadcast gradient
+    x, *rest = operands(case)
+    x.requires_grad_(True)
+    (a,) = torch.autograd.grad(tnx.moe_swiglu(x, *rest).sum(), x)
+    (b,) = torch.autograd.grad(tnx.moe_swiglu(x, *rest), x, torch.ones_like(dy))
+    assert torch.equal(a, b)
+
+
+def test_weights_gradient_against_differences():
+    case = make(6, 3, 2, 32, 24, 16, f16)
+    *args, w = operands(case)
+    w.requires_grad_(True)
+    (grad,) = torch.autograd.grad(tnx.moe_swiglu(*args, w), w, case["dy"].to(DEV))
+    cpu = [case[n] for n in ("x", "w12", "w3", "ids")]
+    for t in range(6):
+        for s in range(2):
+            delta = torch.zeros(6, 2, dtype=torch.float64)
+            delta[t, s] = 0.5   # the output is linear in the weights: any step will do
+            up = O.experts_oracle(*cpu, case["weights"].double() + delta)
+            down = O.experts_oracle(*cpu, case["weights"].double() - delta)
+            diff = ((up - down) * case["dy"].double()).sum().item()
+            assert abs(grad[t, s].item() - diff) <= 1e-5 * (1 + abs(diff))
+
+
+def test_other_stream_and_captured_graphs_do_not_share_scratch():
+    a, b = make(70, 8, 2, 128, 64, 64, bf16, seed=1), make(70, 8, 2, 128, 64, 64, bf16, seed=2)
+    want = [tnx.moe_swiglu(*operands(c)) for c in (a, b)]
+    args = [operands(c) for c in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(10):
+        for s, arg in zip(streams, args):
+            with torch.cuda.stream(s):
+                outs.append(tnx.moe_swiglu(*arg))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
+    graphs, held = [], []
+    for arg in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(tnx.moe_swiglu(*arg))
+        graphs.append(g)
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(h, w) for h, w in zip(held, want))
+        for h in held:
+            h.zero_()
+    # the routing of a replayed graph is the one in its buffers now
+    args[0][3].copy_(args[1][3])
+    graphs[0].replay()
+    assert torch.equal(held[0], tnx.moe_swiglu(*args[0]))
+
+
+def test_captured_backward():
+    case = make(200, 8, 2, 128, 64, 72, bf16)
+    want = check(case)
+    leaves = operands(case, True)
+    dy = case["dy"].to(DEV)
+    inputs = [leaves[i] for i in (0, 1, 2, 4)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(tnx.moe_swiglu(*leaves), inputs, dy)
+    for g in grads:
+        g.zero_()
+    graph.replay()
+    assert all(torch.equal(g, w) for g, w in zip(grads, want))
+
+
+def test_refusals():
+    x, w12, w3, ids, w = operands(make(4, 4, 2, 64, 64, 64, bf16))
+    for bad, match in (((x.float(), w12, w3, ids, w), "float16"), ((x, w12.half(), w3, ids, w), "float16"),
+                       ((x[0], w12, w3, ids, w), "expects"), ((x[:, :32], w12, w3, ids, w), "fit"),
+                       ((x, w12[:3], w3, ids, w), "fit"), ((x, w12, w3[:, :32], ids, w), "fit"),
+                       ((x, w12, w3, ids[:3], w), "ids"), ((x, w12, w3, ids.float(), w), "ids"),
+                       ((x, w12, w3, ids[:, :0], w[:, :0]), "ids"), ((x, w12, w3, ids, w[:, :1]), "weights"),
+                       ((x, w12, w3, ids, w.double()), "weights"), ((x, w12, w3[:, :, :60], ids, w), "multiples of 8"),
+                       ((x[:, :60], w12[:, :60], w3, ids, w), "multiples of 8")):
+        with pytest.raises(ValueError, match=match):
+            tnx.moe_swiglu(*bad)
+    with pytest.raises(ValueError, match="activation"):
+        tnx.moe_swiglu(x, w12, w3, ids, w, activation="relu")
+    with pytest.raises(ValueError, match="512"):
+        tnx.moe_swiglu(x, w12[:1].expand(513, -1, -1), w3[:1].expand(513, -1, -1), ids, w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tnx.moe_swiglu(x.cpu(), w12, w3, ids, w)

@@ -14,7 +14,7 @@ from tritonix_b200.dispatcher import DynamicDispatcher, dynamic_dispatch
 from tritonix_b200.ops import (conv2d_forward, conv2d_forward_kernel, cuda_matmul,
                                gated_residual_norm, gemm_splitk_kernel, glu, glu_kernel,
                                interleave_weights, matmul, matmul_kernel, matmul_splitk,
-                               route_experts, swiglu, swiglu_kernel, swiglu_mlp,
+                               moe_swiglu, route_experts, swiglu, swiglu_kernel, swiglu_mlp,
                                torch_conv2d_forward, triton_matmul)
 from tritonix_b200.host_io import HostRowPipeline, matmul_from_host
 from tritonix_b200.testing import do_bench
@@ -30,7 +30,7 @@ __all__ = ["matmul", "matmul_splitk", "cuda_matmul", "triton_matmul", "matmul_ke
            "CoordinateMonotonicFunction", "DynamicDispatcher", "dynamic_dispatch",
            "OutOfResources", "DeviceStatusError", "check_status", "do_bench", "install_as_tritonix",
            "HostRowPipeline", "matmul_from_host", "conv2d_forward", "conv2d_forward_kernel",
-           "torch_conv2d_forward", "route_experts", "gated_residual_norm"]
+           "torch_conv2d_forward", "route_experts", "moe_swiglu", "gated_residual_norm"]
 
 
 def install_as_tritonix() -> None:

@@ -113,6 +113,18 @@ class NormProblem(ctypes.Structure):
         [(n, ctypes.c_int64) for n in ("stride_y", "stride_residual", "stride_gate")]
 
 
+class MoeProblem(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "experts", "top_k", "d_model", "d_ff", "n_out", "dtype",
+                                              "activation", "wide_ids", "train")] + \
+        [(n, ctypes.c_int64) for n in ("stride_x", "stride_w12e", "stride_w12k", "stride_w3e", "stride_w3k",
+                                       "stride_y")]
+
+
+class MoeResources(ctypes.Structure):
+    _fields_ = [("tile_rows", ctypes.c_int32), ("max_tiles", ctypes.c_int32)] + \
+        [(n, ctypes.c_int64) for n in ("workspace_bytes", "saved_bytes", "backward_workspace_bytes")]
+
+
 SCORINGS = {"softmax": 0, "sigmoid": 1}
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = range(4)
 
@@ -125,7 +137,8 @@ EXPORTS = ("tnx_version", "tnx_last_error", "tnx_sm_count", "tnx_gemm_query", "t
            "tnx_conv2d_pack_weights", "tnx_swiglu_mlp_query", "tnx_swiglu_mlp",
            "tnx_swiglu_mlp_unit_order", "tnx_route_experts", "tnx_route_experts_backward",
            "tnx_gated_residual_norm", "tnx_gated_residual_norm_workspace",
-           "tnx_gated_residual_norm_backward")
+           "tnx_gated_residual_norm_backward", "tnx_moe_query", "tnx_moe_swiglu",
+           "tnx_moe_swiglu_backward")
 STATIC_SCRATCH_BYTES = 16 * 1024 * 1024 + 65536
 
 
@@ -192,10 +205,15 @@ def _load() -> ctypes.CDLL:
             ("tnx_route_experts_backward", RouteProblem, [ptr] * 5),
             ("tnx_gated_residual_norm", NormProblem, [ptr] * 9),
             ("tnx_gated_residual_norm_backward", NormProblem,
-             [ptr, ctypes.c_int64, ptr, ctypes.c_int64] + [ptr] * 12 + [ctypes.c_size_t, ptr])):
+             [ptr, ctypes.c_int64, ptr, ctypes.c_int64] + [ptr] * 12 + [ctypes.c_size_t, ptr]),
+            ("tnx_moe_swiglu", MoeProblem, [ptr] * 8 + [ctypes.c_size_t, ptr, ptr]),
+            ("tnx_moe_swiglu_backward", MoeProblem,
+             [ptr, ctypes.c_int64] + [ptr] * 9 + [ctypes.c_size_t, ptr, ptr])):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(problem)] + args
+    lib.tnx_moe_query.restype = ctypes.c_int
+    lib.tnx_moe_query.argtypes = [ctypes.POINTER(MoeProblem), ctypes.POINTER(MoeResources)]
     lib.tnx_gated_residual_norm_workspace.restype = ctypes.c_int64
     lib.tnx_gated_residual_norm_workspace.argtypes = [ctypes.POINTER(NormProblem)]
     return lib

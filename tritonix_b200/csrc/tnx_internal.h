@@ -31,6 +31,9 @@ int umma_launch(const tnx_problem& p, const tnx_config& cfg, const tnx_resources
 // maps are cached).  is_operand selects the L2 promotion used for loads.
 int make_tmap_2d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows,
                  int64_t pitch_elems, int box_cols, int box_rows, bool is_operand);
+// 3-D (column, row, matrix) over `depth` row-major matrices of 16-bit elements, boxes of one matrix.
+int make_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows, int64_t depth,
+                 int64_t row_pitch, int64_t matrix_pitch, int box_cols, int box_rows, bool is_operand);
 int sm_count();                             // SMs of the current device (148 when none is visible)
 unsigned long long bounded_wait_limit_ns(); // wall-clock limit of every device-side wait
 

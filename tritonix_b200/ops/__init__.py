@@ -6,11 +6,11 @@ from tritonix_b200.ops.swiglu import (glu, glu_kernel, interleave_weights, swigl
                                       swiglu_mlp)
 from tritonix_b200.ops.conv2d import (conv2d_forward, conv2d_forward_kernel,
                                       torch_conv2d_forward)
-from tritonix_b200.ops.moe import route_experts
+from tritonix_b200.ops.moe import moe_swiglu, route_experts
 from tritonix_b200.ops.norm import gated_residual_norm
 from tritonix_b200.ops import _torch_ops  # noqa: F401  (registers torch.ops.tritonix.*)
 
 __all__ = ["matmul", "matmul_splitk", "cuda_matmul", "triton_matmul", "matmul_kernel",
            "gemm_splitk_kernel", "glu_kernel", "swiglu_kernel", "glu", "swiglu", "swiglu_mlp",
            "interleave_weights", "conv2d_forward", "conv2d_forward_kernel", "torch_conv2d_forward",
-           "route_experts", "gated_residual_norm"]
+           "route_experts", "moe_swiglu", "gated_residual_norm"]

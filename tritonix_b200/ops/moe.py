@@ -1,7 +1,8 @@
 """Mixture-of-experts layers: routing tokens to experts and the experts' gated products.
 
-``route_experts`` turns router logits into the experts each token uses and their weights, with a
-gradient for the logits.  The reference has no counterpart.
+``route_experts`` turns router logits into the experts each token uses and their weights;
+``moe_swiglu`` is ``swiglu_mlp`` with many expert MLPs of which each token uses a few.  Both have
+their gradients.  The reference has no counterpart.
 """
 from __future__ import annotations
 
@@ -83,3 +84,136 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     if torch.is_grad_enabled() and logits.requires_grad:
         return _RouteExperts.apply(logits, bias, args)
     return _route(logits, bias, args)
+
+
+# ------------------------------------------------------------------------------ experts' products
+
+def _pitched(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the copy engine can address it: adjacent elements in rows, 16-byte aligned base and
+    pitches, no overlapping rows or matrices; a contiguous copy of anything else."""
+    shape, stride = t.shape, t.stride()
+    fine = stride[-1] == 1 and t.data_ptr() % 16 == 0
+    extent = shape[-1]
+    for size, step in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if size > 1:
+            fine = fine and step % 8 == 0 and step >= extent
+        extent = size * (step if size > 1 else extent)
+    return t if fine else t.clone(memory_format=torch.contiguous_format)
+
+
+def _pitches(t: torch.Tensor) -> list:
+    """Strides of all dimensions but the last, from the first on; those of dimensions of one element
+    (torch may give any) as if it were contiguous."""
+    out, extent = [], t.shape[-1]
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        step = step if size > 1 else extent
+        out.append(step)
+        extent = step * size
+    return out[::-1]
+
+
+_moe_plans: dict = {}
+
+
+def _moe_plan(x, w12, w3, ids, activation, train):
+    """(problem, resources) of a call signature, validated once."""
+    key = (x.shape, w12.shape, w3.shape[2], ids.shape, x.dtype, ids.dtype, activation, train, x.stride(),
+           w12.stride(), w3.stride())
+    plan = _moe_plans.get(key)
+    if plan is None:
+        tokens, d_model = x.shape
+        experts, d_ff, n_out = w3.shape
+        (sx,), (s12e, s12k), (s3e, s3k) = _pitches(x), _pitches(w12), _pitches(w3)
+        problem = _cabi.MoeProblem(tokens, experts, ids.shape[1], d_model, d_ff, n_out, _cabi.DTYPES[x.dtype],
+                                   activation, int(ids.dtype == torch.int64), int(train), sx, s12e, s12k, s3e, s3k,
+                                   n_out)
+        res = _cabi.MoeResources()
+        _cabi.raise_for(_cabi.lib.tnx_moe_query(ctypes.byref(problem), ctypes.byref(res)))
+        if len(_moe_plans) > 4096:
+            _moe_plans.clear()
+        plan = _moe_plans[key] = (problem, res)
+    return plan
+
+
+def _moe_forward(x, w12, w3, ids, weights, activation, train):
+    problem, res = _moe_plan(x, w12, w3, ids, activation, train)
+    device = x.device
+    y = torch.empty((x.shape[0], w3.shape[2]), device=device, dtype=x.dtype)
+    # (scratch of the call's own: calls on different streams or in different graphs never share it)
+    workspace = torch.empty(res.workspace_bytes, device=device, dtype=torch.uint8)
+    saved = torch.empty(res.saved_bytes, device=device, dtype=torch.uint8) if train else None
+    _cabi.call(device, _cabi.lib.tnx_moe_swiglu, ctypes.byref(problem), x.data_ptr(), w12.data_ptr(), w3.data_ptr(),
+               ids.data_ptr(), weights.data_ptr(), y.data_ptr(), saved.data_ptr() if train else None,
+               workspace.data_ptr(), workspace.numel(), _cabi.status_word(device).data_ptr())
+    return y, saved
+
+
+class _MoeSwiglu(torch.autograd.Function):
+    """Keeps the operands, the pairs' order, the hidden activation (16 bits) and the gate/up products
+    (fp32): 10 bytes per pair and hidden column."""
+
+    @staticmethod
+    def forward(ctx, x, w12, w3, weights, ids, activation):
+        y, saved = _moe_forward(x, w12, w3, ids, weights, activation, True)
+        ctx.save_for_backward(x, w12, w3, saved)
+        ctx.ids_like, ctx.activation = torch.empty(ids.shape, dtype=ids.dtype, device="meta"), activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w12, w3, saved = ctx.saved_tensors
+        problem, res = _moe_plan(x, w12, w3, ctx.ids_like, ctx.activation, True)
+        dy = _pitched(dy)
+        (stride_dy,) = _pitches(dy)
+        wants = ctx.needs_input_grad
+        new = lambda shape, dtype: torch.empty(shape, device=x.device, dtype=dtype)  # noqa: E731
+        dx = new(x.shape, x.dtype) if wants[0] else None
+        dw12 = new(w12.shape, x.dtype) if wants[1] else None
+        dw3 = new(w3.shape, x.dtype) if wants[2] else None
+        dweights = new(ctx.ids_like.shape, torch.float32) if wants[3] else None
+        workspace = new(res.backward_workspace_bytes, torch.uint8)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        _cabi.call(x.device, _cabi.lib.tnx_moe_swiglu_backward, ctypes.byref(problem), dy.data_ptr(), stride_dy,
+                   x.data_ptr(), w12.data_ptr(), w3.data_ptr(), saved.data_ptr(), ptr(dx), ptr(dw12), ptr(dw3),
+                   ptr(dweights), workspace.data_ptr(), workspace.numel(), _cabi.status_word(x.device).data_ptr())
+        return dx, dw12, dw3, dweights, None, None
+
+
+def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+               activation: str = "silu") -> torch.Tensor:
+    """The experts' MLPs of every token, weighted and added:
+
+        y[t] = sum over slots s of  weights[t, s] * ((act(x[t] W1[e]) * (x[t] W2[e])) W3[e]),  e = ids[t, s]
+
+    ``x`` [tokens, D]; ``w12`` [experts, D, 2F], each expert's W1 and W2 column-interleaved
+    (``interleave_weights``); ``w3`` [experts, F, N]: all fp16 or all bf16, with D, F and N multiples
+    of 8 and at most 512 experts.  ``ids`` [tokens, top_k] int32 or int64 and ``weights`` fp32, as
+    ``route_experts`` returns them; a slot whose id is not an expert (-1, say) contributes nothing,
+    and an expert may stand in several slots of a token.  ``activation``: "silu", "sigmoid" or
+    "none" (``swiglu`` and ``glu`` take the same).
+
+    Gradients flow to ``x``, ``w12``, ``w3`` and ``weights``.  The routing stays on the device: no
+    call waits for it.  Results do not depend on timing (every sum has a fixed order)."""
+    _cabi.require_cuda(x, w12, w3, ids, weights)
+    if x.dtype not in (torch.float16, torch.bfloat16) or w12.dtype != x.dtype or w3.dtype != x.dtype:
+        raise ValueError(f"x, w12 and w3 must all be float16 or all bfloat16, got {x.dtype}, {w12.dtype}, {w3.dtype}")
+    if x.dim() != 2 or w12.dim() != 3 or w3.dim() != 3:
+        raise ValueError("moe_swiglu expects x (tokens, D), w12 (experts, D, 2F) and w3 (experts, F, N)")
+    if w12.shape[0] != w3.shape[0] or w12.shape[1] != x.shape[1] or w12.shape[2] != 2 * w3.shape[1]:
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w12 {tuple(w12.shape)}, w3 {tuple(w3.shape)}")
+    if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape[1] < 1 or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be int32 or int64 (tokens, top_k), got {tuple(ids.shape)} {ids.dtype}")
+    if weights.shape != ids.shape or weights.dtype != torch.float32:
+        raise ValueError(f"weights must be float32 {tuple(ids.shape)}, got {tuple(weights.shape)} {weights.dtype}")
+    if any(t.device != x.device for t in (w12, w3, ids, weights)):
+        raise ValueError("all operands must live on the same device")
+    act = _cabi.ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {sorted(_cabi.ACTIVATIONS)}, got {activation!r}")
+    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w12, w3, weights))
+    x, w12, w3 = _pitched(x), _pitched(w12), _pitched(w3)
+    ids, weights = ids.contiguous(), weights.contiguous()
+    if needs_grad:
+        return _MoeSwiglu.apply(x, w12, w3, weights, ids, act)
+    return _moe_forward(x, w12, w3, ids, weights, act, False)[0]
