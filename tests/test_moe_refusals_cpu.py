@@ -107,7 +107,7 @@ def test_moe_resources_and_workspace():
     part = 4 * 128 * 48 * 4
     assert res.workspace_bytes >= part + 4 * 128 * 32 * 2
     rc, train = query(moe(train=1))
-    assert rc == _cabi.OK and train.workspace_bytes == part and train.saved_bytes >= 4 * 128 * 32 * 10
+    assert rc == _cabi.OK and train.workspace_bytes >= part and train.saved_bytes >= 4 * 128 * 32 * 10
     assert query(moe(tokens=4000))[1].tile_rows == 256
 
     def forward(p, nbytes, workspace=PTR, saved=None, x=PTR):

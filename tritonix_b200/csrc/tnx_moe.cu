@@ -5,14 +5,18 @@
 //  * A (token, slot) pair is a row of a grouped problem.  plan_* sorts the pairs by expert (stable:
 //    rows of an expert keep the pairs' order, so every sum has a fixed order) and pads each expert
 //    to whole row tiles.  Nothing about the routing is needed on the host.
-//  * moe_gemm_kernel runs the five products on the TMA -> shared memory -> tcgen05 -> TMEM pipeline
-//    of the library's GEMM.  Rows are picked by the copy engine itself (tile::gather4, one lane per
-//    four rows): x and dy are never copied into expert order.
-//        kGateUp  H = w * act(x W1) * (x W2)          rows gathered, weights N-major
+//  * moe_gemm_kernel runs the products on the TMA -> shared memory -> tcgen05 -> TMEM pipeline of
+//    the library's GEMM, with X and dY the rows of x and dy in expert order:
+//        kGateUp  H = w * act(X W1) * (X W2)          weights N-major
 //        kDown    O = H W3                            fp32, one row per pair
-//        kDHidden dH = dy W3^T, then dGU and dw       rows gathered, weights K-major
+//        kDHidden dH = dY W3^T, then dGU and dw       weights K-major
 //        kDX      O = dGU W12^T                       fp32, one row per pair
-//        kDW12, kDW3   x^T dGU and H^T dy per expert  K = the expert's rows
+//        kDW12, kDW3   X^T dGU and H^T dY per expert  K = the expert's rows
+//    permute_kernel copies rows into expert order.  With few rows per expert the copy engine picks
+//    them itself instead (kGateUpGather, tile::gather4, one lane per four rows): a gather of four
+//    128-byte row pieces was measured to take about as long as a whole box of rows (40-75 cycles),
+//    so 128 rows by gathers cost 2.3 times the tensor cores' time (8192 tokens, 64 experts
+//    2048/1024: gate/up product 1287 us gathered), while a few rows cost nothing and save a launch.
 //    The routing weight is applied to the hidden activation before it is rounded: the rows of O
 //    only need adding, and H is the very operand dW3 needs, so no value on the way is rounded
 //    twice.
@@ -52,14 +56,14 @@ constexpr int kAbortProducer = 0x301;
 constexpr int kAbortMma = 0x302;
 constexpr int kAbortEpilogue = 0x303;
 
-enum Mode { kGateUp, kDown, kDHidden, kDX, kDW12, kDW3 };
+enum Mode { kGateUp, kGateUpGather, kDown, kDHidden, kDX, kDW12, kDW3 };
 
 // What a mode's operands look like.
 template <int MODE>
 struct Traits {
   static constexpr bool wgrad = MODE == kDW12 || MODE == kDW3;
-  static constexpr bool gather_a = MODE == kGateUp || MODE == kDHidden || MODE == kDW12;
-  static constexpr bool gather_b = MODE == kDW3;
+  static constexpr bool gather_a = MODE == kGateUpGather;
+  static constexpr bool gate_up = MODE == kGateUp || MODE == kGateUpGather;
   static constexpr bool b_kmajor = MODE == kDHidden || MODE == kDX;
 };
 // Accumulator columns per tile.  (dHidden streams gate/up through shared memory as well; a
@@ -89,7 +93,7 @@ struct GemmParams {
   int tiles_m;     // wgrad: row tiles of the weight
   int m;           // wgrad: rows of the weight
   int activation;
-  int save_gu;     // kGateUp: also store the fp32 products
+  int save_gu;     // gate/up: also store the fp32 products
   float* part;     // kDown, kDX: O, [max_rows, cols]
   float* dw_part;  // kDHidden: [max_rows, tiles_n]
   int stages;
@@ -126,23 +130,32 @@ struct PlanParams {
   int* chunk_counts;  // [chunks][experts] (large problems)
 };
 
-// One warp walks its chunk of pairs 32 at a time.  Pass 1 counts experts in counts[]; pass 2 hands
-// out rows from counts[], which then holds the chunk's first row of every expert.
-template <typename C>
-__device__ __forceinline__ void count_chunk(const PlanParams& p, int first, int last, int lane, C* counts) {
-  for (int base = first; base < last; base += 32) {
-    const int i = base + lane;
-    const int e = i < last ? pair_expert(p.ids, p.wide, p.experts, i) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) counts[e] = static_cast<C>(counts[e] + __popc(same));
-    __syncwarp();
+// One warp walks its chunk of pairs, 32 at a time, with the ids of eight such steps in flight.
+// Pass 1 counts experts in counts[]; pass 2 hands out rows from next[], which holds the chunk's
+// first row of every expert.
+constexpr int kAhead = 8;
+template <typename Step>
+__device__ __forceinline__ void walk_chunk(const PlanParams& p, int first, int last, int lane, Step step) {
+  for (int base = first; base < last; base += 32 * kAhead) {
+    int e[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = base + a * 32 + lane;
+      e[a] = i < last ? pair_expert(p.ids, p.wide, p.experts, i) : -1;
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      if (base + a * 32 < last) step(base + a * 32 + lane, e[a], __match_any_sync(0xffffffffu, e[a]));
   }
 }
+__device__ __forceinline__ void count_chunk(const PlanParams& p, int first, int last, int lane, int* counts) {
+  walk_chunk(p, first, last, lane, [&](int, int e, unsigned same) {
+    if (e >= 0 && lane == __ffs(same) - 1) counts[e] += __popc(same);
+    __syncwarp();
+  });
+}
 __device__ __forceinline__ void place_chunk(const PlanParams& p, int first, int last, int lane, int* next) {
-  for (int base = first; base < last; base += 32) {
-    const int i = base + lane;
-    const int e = i < last ? pair_expert(p.ids, p.wide, p.experts, i) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
+  walk_chunk(p, first, last, lane, [&](int i, int e, unsigned same) {
     int row = -1;
     if (e >= 0) row = next[e] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
@@ -153,7 +166,7 @@ __device__ __forceinline__ void place_chunk(const PlanParams& p, int first, int 
       p.plan.row_token[row] = i / p.top_k;
       p.plan.row_weight[row] = p.weights[i];
     }
-  }
+  });
 }
 
 // Given total[e] in shared memory: first row of every expert (in start[]), row tiles and their
@@ -224,7 +237,7 @@ __global__ void __launch_bounds__(kSmallWarps * 32) plan_small_kernel(const Plan
 
 // More pairs: count per chunk, scan over chunks and experts, place.
 constexpr int kChunkWarps = 4;
-constexpr int kChunkPairs = 1024;
+constexpr int kChunkPairs = 32 * kAhead;
 __global__ void __launch_bounds__(kChunkWarps * 32) plan_count_kernel(const PlanParams p) {
   __shared__ int counts[kChunkWarps][kMaxExperts];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -238,29 +251,42 @@ __global__ void __launch_bounds__(kChunkWarps * 32) plan_count_kernel(const Plan
   count_chunk(p, first, last, lane, counts[warp]);
   for (int e = lane; e < p.experts; e += 32) p.chunk_counts[static_cast<long long>(chunk) * p.experts + e] = counts[warp][e];
 }
+// Threads (expert, strand): a strand owns a run of chunks, its threads read neighbouring experts.
 __global__ void __launch_bounds__(1024) plan_scan_kernel(const PlanParams p) {
-  __shared__ int total[kMaxExperts], start[kMaxExperts];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int total[kMaxExperts], start[kMaxExperts], strand_sum[1024];
   dependency_wait();
   dependency_release();
-  for (int e = warp; e < p.experts; e += 32) {
-    int carry = 0;
-    for (int base = 0; base < p.chunks; base += 32) {
-      const int c = base + lane;
-      int* at = p.chunk_counts + static_cast<long long>(c) * p.experts + e;
-      const int v = c < p.chunks ? *at : 0;
-      int sum = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
-      }
-      if (c < p.chunks) *at = carry + sum - v;
-      carry += __shfl_sync(0xffffffffu, sum, 31);
+  const int strands = 1024 / p.experts;
+  const int strand = threadIdx.x / p.experts, e = threadIdx.x - strand * p.experts;
+  const int run = (p.chunks + strands - 1) / strands;
+  const int c0 = min(strand * run, p.chunks), c1 = strand < strands ? min(c0 + run, p.chunks) : c0;
+  int sum = 0;
+#pragma unroll 8
+  for (int c = c0; c < c1; ++c) sum += p.chunk_counts[static_cast<long long>(c) * p.experts + e];
+  strand_sum[threadIdx.x] = sum;
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.experts; x += blockDim.x) {
+    int before = 0;
+    for (int t = 0; t < strands; ++t) {
+      const int v = strand_sum[t * p.experts + x];
+      strand_sum[t * p.experts + x] = before;
+      before += v;
     }
-    if (lane == 0) total[e] = carry;
+    total[x] = before;
   }
   __syncthreads();
+  int before = strand_sum[threadIdx.x];
+  for (int c = c0; c < c1; c += 8) {
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = c + i < c1 ? p.chunk_counts[static_cast<long long>(c + i) * p.experts + e] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c + i < c1) p.chunk_counts[static_cast<long long>(c + i) * p.experts + e] = before;
+      before += v[i];
+    }
+  }
   lay_out(p, total, start);
 }
 __global__ void __launch_bounds__(kChunkWarps * 32) plan_place_kernel(const PlanParams p) {
@@ -464,16 +490,11 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const uint32_t stage_tx =
           static_cast<uint32_t>(CTA_GROUP * ((T::gather_a ? 512 : T::wgrad ? 8192 : 4096) * a_lanes + b_stage_bytes));
       int rows[4] = {0, 0, 0, 0};
-      if (T::gather_a && !T::wgrad) {
+      if (T::gather_a) {
         // rows past the expert's last are copies of that one: addressable, and dropped later
         const int last = un.row0 + un.valid - 1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) rows[i] = p.plan.row_token[min(row0 + 4 * lane + i, last)];
-      }
-      const int k_last = un.k_row0 + un.k_rows - 1;
-      if (T::wgrad && un.num_kb > 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rows[i] = p.plan.row_token[min(un.k_row0 + 4 * (lane & 15) + i, k_last)];
       }
       for (int kb = 0; kb < un.num_kb; ++kb) {
         const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns);
@@ -491,29 +512,8 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (T::wgrad) {
           // K = pair rows; both operands lie in memory as (pair row, column), 64-column atoms
           const int k_row = un.k_row0 + k0;
-          const int atom = lane >> 4, quad = lane & 15;
-          if (T::gather_a) {
-            // (an atom wholly past the matrix feeds rows that are never stored: any column will do)
-            const int x = row0 + atom * 64;
-            tma_gather4<CTA_GROUP>(a_dst + atom * 8192 + quad * 512, &tmap_a, x < p.m ? x : 0, rows, bar);
-          } else if (lane < 2) {
-            load_2d<CTA_GROUP>(a_dst + lane * 8192, &tmap_a, row0 + lane * 64, k_row, bar);
-          }
-          if (T::gather_b) {
-#pragma unroll
-            for (int half = 0; half < LOAD_N / 128; ++half) {
-              const int na = half * 2 + atom;
-              const int x = b_col0 + na * 64;
-              tma_gather4<CTA_GROUP>(b_dst + na * 8192 + quad * 512, &tmap_b, x < p.cols ? x : 0, rows, bar);
-            }
-          } else if (lane < LOAD_N / 64) {
-            load_2d<CTA_GROUP>(b_dst + lane * 8192, &tmap_b, b_col0 + lane * 64, k_row, bar);
-          }
-          if (kb + 1 < un.num_kb) {  // the next block's rows, while this one's copies are in flight
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              rows[i] = p.plan.row_token[min(k_row + kTileK + 4 * quad + i, k_last)];
-          }
+          if (lane < 2) load_2d<CTA_GROUP>(a_dst + lane * 8192, &tmap_a, row0 + lane * 64, k_row, bar);
+          if (lane < LOAD_N / 64) load_2d<CTA_GROUP>(b_dst + lane * 8192, &tmap_b, b_col0 + lane * 64, k_row, bar);
         } else {
           if (T::gather_a) {
             if (lane < a_lanes) tma_gather4<CTA_GROUP>(a_dst + lane * 512, &tmap_a, k0, rows, bar);
@@ -659,7 +659,7 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         fetch_gu(0, gu_chunks);
         if (gu_total > 1) fetch_gu(1, gu_chunks + 1);
       }
-      const float weight = !T::wgrad && live && (MODE == kGateUp || MODE == kDHidden)
+      const float weight = !T::wgrad && live && (T::gate_up || MODE == kDHidden)
                                ? p.plan.row_weight[row0 + row_in_tile] : 0.f;
 
       const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc]), acc_phase, abort_flag, p.timeout_ns);
@@ -671,7 +671,7 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const uint32_t t_acc = tmem_base + lane_sel + acc * TILE_N;
       uint32_t r[32];
 
-      if (MODE == kGateUp) {
+      if (T::gate_up) {
         if (p.save_gu) {
           for (int col = 0; col < TILE_N; col += 32) {
             if (un.col0 + col >= p.cols) break;
@@ -859,7 +859,34 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   }
 }
 
-// --------------------------------------------------------------------------------- row joins
+// ----------------------------------------------------------------------- rows in and out of order
+
+// out[pos[t, s]] = in[t] for every slot: a 16-byte piece of a token is read once and stored top_k
+// times.  The blocks from `copy_blocks` on (where there are any) clear an expert's rows from its
+// last to the next multiple of 64 each, which products over K = rows read.
+__global__ void __launch_bounds__(256) permute_kernel(const Plan plan, const uint4* in, long long ld_in, uint4* out,
+                                                      int tokens, int top_k, int vectors, int copy_blocks) {
+  dependency_wait();
+  dependency_release();
+  if (static_cast<int>(blockIdx.x) >= copy_blocks) {
+    const int e = blockIdx.x - copy_blocks;
+    const int count = plan.count[e];
+    const long long first = static_cast<long long>(plan.start[e] + count) * vectors;
+    const int clear = ((count + kTileK - 1) / kTileK * kTileK - count) * vectors;
+    for (int i = threadIdx.x; i < clear; i += 256) out[first + i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const long long total = static_cast<long long>(tokens) * vectors;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += copy_blocks * 256ll) {
+    const int t = static_cast<int>(i / vectors);
+    const int c = static_cast<int>(i - static_cast<long long>(t) * vectors);
+    const uint4 v = in[t * ld_in + c];
+    for (int s = 0; s < top_k; ++s) {
+      const int row = plan.pos[static_cast<long long>(t) * top_k + s];
+      if (row >= 0) out[static_cast<long long>(row) * vectors + c] = v;
+    }
+  }
+}
 
 // out[t] = sum over slots of part[pos[t, s]], in slot order; slots without an expert add nothing.
 template <typename T>
@@ -912,8 +939,9 @@ struct Layout {
   int chunk, chunks;
   // forward: everything in `saved` when training (and the rest in the workspace)
   int64_t off_tiles, off_count, off_start, off_tile_expert, off_row_token, off_row_weight, off_pos, plan_bytes;
-  int64_t hidden_bytes, gu_bytes, part_bytes, chunk_bytes;
-  int64_t dgu_bytes, dx_bytes, dw_bytes;
+  bool gather;         // the copy engine picks the rows of x
+  int64_t hidden_bytes, gu_bytes, part_bytes, chunk_bytes, x_bytes;
+  int64_t dgu_bytes, dx_bytes, dw_bytes, dy_bytes;
 };
 
 int moe_check(const tnx_moe_problem* p) {
@@ -990,6 +1018,10 @@ Layout lay_out_problem(const tnx_moe_problem& p) {
   l.off_row_weight = take(4 * l.max_rows);
   l.off_pos = take(4ll * l.pairs);
   l.plan_bytes = at;
+  // (a training step needs the rows in order for the weights' gradients anyway)
+  l.gather = !p.train && l.pairs / p.experts <= 32;
+  l.x_bytes = l.gather ? 0 : align256(l.max_rows * p.d_model * 2);
+  l.dy_bytes = align256(l.max_rows * p.n_out * 2);
   l.hidden_bytes = align256(l.max_rows * p.d_ff * 2);
   l.gu_bytes = align256(l.max_rows * p.d_ff * 8);
   l.part_bytes = align256(l.max_rows * p.n_out * 4);
@@ -1116,6 +1148,18 @@ int run_plan(const tnx_moe_problem& p, const Layout& l, const Plan& plan, const 
   return rc;
 }
 
+// Rows of `in` [tokens, cols] in expert order.
+int run_permute(const tnx_moe_problem& p, const Plan& plan, const void* in, int64_t ld_in, void* out, int cols,
+                bool clear, cudaStream_t stream) {
+  const int vectors = cols / 8;
+  const int64_t blocks = (static_cast<int64_t>(p.tokens) * vectors + 255) / 256;
+  const int most = 16 * sm_count();
+  const int grid = blocks < most ? static_cast<int>(blocks) : most;
+  return launch("rows in expert order", permute_kernel, grid + (clear ? p.experts : 0), 256, 0, 1, stream, plan,
+                static_cast<const uint4*>(in), static_cast<long long>(ld_in / 8), static_cast<uint4*>(out), p.tokens,
+                p.top_k, vectors, grid);
+}
+
 int run_combine(int dtype, const float* part, const int* pos, void* out, int64_t ld_out, int tokens, int top_k,
                 int cols, cudaStream_t stream) {
   const int64_t blocks = (static_cast<int64_t>(tokens) * (cols / 8) + 255) / 256;
@@ -1160,8 +1204,8 @@ int tnx_moe_query(const tnx_moe_problem* problem, tnx_moe_resources* out) {
   out->max_tiles = l.max_tiles;
   const int64_t keep = l.plan_bytes + l.hidden_bytes;
   out->saved_bytes = keep + l.gu_bytes;
-  out->workspace_bytes = l.part_bytes + l.chunk_bytes + (problem->train ? 0 : keep);
-  out->backward_workspace_bytes = l.dgu_bytes + l.dx_bytes + l.dw_bytes;
+  out->workspace_bytes = l.part_bytes + l.chunk_bytes + l.x_bytes + (problem->train ? 0 : keep);
+  out->backward_workspace_bytes = l.dgu_bytes + l.dx_bytes + l.dw_bytes + l.x_bytes + l.dy_bytes;
   return TNX_OK;
 }
 
@@ -1194,12 +1238,14 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   char* ws = static_cast<char*>(workspace);
   float* part = reinterpret_cast<float*>(ws);
   void* chunk_counts = ws + l.part_bytes;
-  char* keep = p.train ? static_cast<char*>(saved) : ws + l.part_bytes + l.chunk_bytes;
+  void* xp = ws + l.part_bytes + l.chunk_bytes;
+  char* keep = p.train ? static_cast<char*>(saved) : ws + l.part_bytes + l.chunk_bytes + l.x_bytes;
   const Plan plan = plan_at(l, keep);
   void* hidden = keep + l.plan_bytes;
   void* gu = p.train ? keep + l.plan_bytes + l.hidden_bytes : nullptr;
 
   rc = run_plan(p, l, plan, ids, weights, chunk_counts, s);
+  if (rc == TNX_OK && !l.gather) rc = run_permute(p, plan, x, p.stride_x, xp, p.d_model, false, s);
   if (rc != TNX_OK) return rc;
 
   // H = w * act(x W1) * (x W2)
@@ -1209,7 +1255,8 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   g.tiles_n = cdiv(g.cols, 256);
   g.save_gu = p.train;
   CUtensorMap ta, tb, tc, tgu;
-  rc = make_tmap_2d(&ta, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true);
+  rc = l.gather ? make_tmap_2d(&ta, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true)
+                : make_tmap_2d(&ta, xp, p.dtype, p.d_model, l.max_rows, p.d_model, 64, 32, true);
   if (rc == TNX_OK)
     rc = make_tmap_3d(&tb, w12, p.dtype, 2ll * p.d_ff, p.d_model, p.experts, p.stride_w12k, p.stride_w12e, 64, kTileK, true);
   if (rc == TNX_OK) rc = make_tmap_2d(&tc, hidden, p.dtype, p.d_ff, l.max_rows, p.d_ff, 64, kRows, false);
@@ -1217,7 +1264,9 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   if (rc == TNX_OK && p.train)
     rc = make_tmap_2d(&tgu, gu, TNX_F32, 2ll * p.d_ff, l.max_rows, 2ll * p.d_ff, 32, kRows, false);
   if (rc != TNX_OK) return rc;
-  rc = launch_gemm<kGateUp>(l, p.dtype, ta, tb, tc, tgu, g, static_cast<int64_t>(l.max_tiles) * g.tiles_n, s);
+  const int64_t units = static_cast<int64_t>(l.max_tiles) * g.tiles_n;
+  rc = l.gather ? launch_gemm<kGateUpGather>(l, p.dtype, ta, tb, tc, tgu, g, units, s)
+                : launch_gemm<kGateUp>(l, p.dtype, ta, tb, tc, tgu, g, units, s);
   if (rc != TNX_OK) return rc;
 
   // O = H W3
@@ -1276,18 +1325,24 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
   void* dgu = ws;
   float* dx_part = reinterpret_cast<float*>(ws + l.dgu_bytes);
   float* dw_part = reinterpret_cast<float*>(ws + l.dgu_bytes + l.dx_bytes);
+  void* xp = ws + l.dgu_bytes + l.dx_bytes + l.dw_bytes;
+  void* dyp = ws + l.dgu_bytes + l.dx_bytes + l.dw_bytes + l.x_bytes;
   const int64_t two_f = 2ll * p.d_ff;
+  const bool hidden_grad = dx != nullptr || dw12 != nullptr || dweights != nullptr;
+  if (hidden_grad || dw3 != nullptr) rc = run_permute(p, plan, dy, stride_dy, dyp, p.n_out, true, s);
+  if (rc == TNX_OK && dw12 != nullptr) rc = run_permute(p, plan, x, p.stride_x, xp, p.d_model, true, s);
+  if (rc != TNX_OK) return rc;
 
   // dH = dy W3^T; dGU and the routing weights' gradient from it
   GemmParams g = gemm_params(p, plan, status_word);
   CUtensorMap ta, tb, tc, tgu;
-  if (dx != nullptr || dw12 != nullptr || dweights != nullptr) {
+  if (hidden_grad) {
     const int n = tile_n(kDHidden, l.cta_group);
     g.num_kb = cdiv(p.n_out, kTileK);
     g.cols = p.d_ff;
     g.tiles_n = cdiv(g.cols, n);
     g.dw_part = dw_part;
-    rc = make_tmap_2d(&ta, dy, p.dtype, p.n_out, p.tokens, stride_dy, 64, 1, true);
+    rc = make_tmap_2d(&ta, dyp, p.dtype, p.n_out, l.max_rows, p.n_out, 64, 32, true);
     if (rc == TNX_OK)
       rc = make_tmap_3d(&tb, w3, p.dtype, p.n_out, p.d_ff, p.experts, p.stride_w3k, p.stride_w3e, 64,
                         n / l.cta_group, true);
@@ -1323,7 +1378,7 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
     g.tiles_m = cdiv(p.d_model, l.tile_rows);
     g.cols = static_cast<int>(two_f);
     g.tiles_n = cdiv(g.cols, 256);
-    rc = make_tmap_2d(&ta, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true);
+    rc = make_tmap_2d(&ta, xp, p.dtype, p.d_model, l.max_rows, p.d_model, 64, kTileK, true);
     if (rc == TNX_OK) rc = make_tmap_2d(&tb, dgu, p.dtype, two_f, l.max_rows, two_f, 64, kTileK, true);
     if (rc == TNX_OK)
       rc = make_tmap_3d(&tc, dw12, p.dtype, two_f, p.d_model, p.experts, two_f, two_f * p.d_model, 64, kRows, false);
@@ -1337,7 +1392,7 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
     g.cols = p.n_out;
     g.tiles_n = cdiv(g.cols, 256);
     rc = make_tmap_2d(&ta, hidden, p.dtype, p.d_ff, l.max_rows, p.d_ff, 64, kTileK, true);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tb, dy, p.dtype, p.n_out, p.tokens, stride_dy, 64, 1, true);
+    if (rc == TNX_OK) rc = make_tmap_2d(&tb, dyp, p.dtype, p.n_out, l.max_rows, p.n_out, 64, kTileK, true);
     if (rc == TNX_OK)
       rc = make_tmap_3d(&tc, dw3, p.dtype, p.n_out, p.d_ff, p.experts, p.n_out, static_cast<int64_t>(p.n_out) * p.d_ff,
                         64, kRows, false);

@@ -32,6 +32,7 @@ class _RouteExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, args):
         weights, ids = _route(logits, bias, args)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids)
         ctx.args = args
         ctx.mark_non_differentiable(ids)
@@ -40,6 +41,8 @@ class _RouteExperts(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dweights, _):
+        if dweights is None:
+            return None, None, None
         logits, ids = ctx.saved_tensors
         problem = _route_problem(logits, *ctx.args)
         dweights = dweights.contiguous()
