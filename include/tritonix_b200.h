@@ -486,7 +486,7 @@ typedef struct tnx_moe_problem {
 } tnx_moe_problem;
 
 typedef struct tnx_moe_resources {
-  int32_t tile_rows; /* rows per row tile: an expert's rows are padded to it */
+  int32_t tile_rows; /* rows of an expert that share one pass over its weights */
   int32_t max_tiles; /* row tiles at most                                    */
   int64_t workspace_bytes;          /* scratch of one forward call                  */
   int64_t saved_bytes;              /* what a training forward call keeps           */

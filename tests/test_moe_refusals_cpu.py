@@ -102,13 +102,14 @@ def test_moe_refuses(bad):
 
 def test_moe_resources_and_workspace():
     rc, res = query(moe())
-    # 20 pairs on 4 experts: a tile of 128 rows for each expert, and none left over
-    assert rc == _cabi.OK and (res.tile_rows, res.max_tiles) == (128, 4)
-    part = 4 * 128 * 48 * 4
-    assert res.workspace_bytes >= part + 4 * 128 * 32 * 2
+    # 20 pairs on 4 experts: a tile for each expert, rows padded to multiples of 16
+    assert rc == _cabi.OK and (res.tile_rows, res.max_tiles) == (256, 4)
+    rows = 20 + 4 * 15
+    part = rows * 48 * 4
+    assert res.workspace_bytes >= part + rows * 32 * 2
     rc, train = query(moe(train=1))
-    assert rc == _cabi.OK and train.workspace_bytes >= part and train.saved_bytes >= 4 * 128 * 32 * 10
-    assert query(moe(tokens=4000))[1].tile_rows == 256
+    assert rc == _cabi.OK and train.workspace_bytes >= part and train.saved_bytes >= rows * 32 * 10
+    assert query(moe(tokens=4000))[1].max_tiles == 4 + (8000 - 4) // 256
 
     def forward(p, nbytes, workspace=PTR, saved=None, x=PTR):
         return lib.tnx_moe_swiglu(ctypes.byref(p), x, PTR, PTR, PTR, PTR, PTR, saved, workspace, nbytes, None, None)

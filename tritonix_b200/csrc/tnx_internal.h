@@ -34,6 +34,10 @@ int make_tmap_2d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int
 // 3-D (column, row, matrix) over `depth` row-major matrices of 16-bit elements, boxes of one matrix.
 int make_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows, int64_t depth,
                  int64_t row_pitch, int64_t matrix_pitch, int box_cols, int box_rows, bool is_operand);
+// The same matrices as `cols / 64` panels of 64 columns (cols a multiple of 64): (column in panel,
+// row, panel, matrix), boxes of box_rows rows of two neighbouring panels.
+int make_tmap_panels(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows, int64_t depth,
+                     int64_t row_pitch, int64_t matrix_pitch, int box_rows);
 int sm_count();                             // SMs of the current device (148 when none is visible)
 unsigned long long bounded_wait_limit_ns(); // wall-clock limit of every device-side wait
 

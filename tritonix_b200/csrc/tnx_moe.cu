@@ -3,24 +3,30 @@
 // with W12 = W1/W2 column-interleaved per expert, and its backward pass.
 //
 //  * A (token, slot) pair is a row of a grouped problem.  plan_* sorts the pairs by expert (stable:
-//    rows of an expert keep the pairs' order, so every sum has a fixed order) and pads each expert
-//    to whole row tiles.  Nothing about the routing is needed on the host.
-//  * moe_gemm_kernel runs the products on the TMA -> shared memory -> tcgen05 -> TMEM pipeline of
-//    the library's GEMM, with X and dY the rows of x and dy in expert order:
-//        kGateUp  H = w * act(X W1) * (X W2)          weights N-major
+//    rows of an expert keep the pairs' order, so every sum has a fixed order).  Nothing about the
+//    routing is needed on the host.
+//  * moe_rows_kernel multiplies rows by their expert's weights on CTA pairs (TMA -> shared memory ->
+//    tcgen05 -> TMEM, the pipeline of the library's GEMM), with the WEIGHTS as the 256-row M
+//    operand and the rows as N:  out^T = W^T rows^T.  N is a field of each instruction, so a tile
+//    costs what its rows need, to a multiple of 32, instead of what 256 rows would (with rows as M
+//    an expert's last tile is half empty on average: 12 % of the work at 64 experts and 65536
+//    pairs, and under the power cap that is 12 % of the time), and all the rows of an expert with
+//    up to 256 of them share one pass over its weights.  In the epilogue a lane then is a column
+//    of the output and a register a row: every store is a coalesced row piece, straight from
+//    registers, and unused rows cost nothing.
+//        kGateUp  H = w * act(X W1) * (X W2)          X: the rows of x in expert order
 //        kDown    O = H W3                            fp32, one row per pair
-//        kDHidden dH = dY W3^T, then dGU and dw       weights K-major
+//        kDHidden dH = dY W3^T, then dGU and dw       dY: the rows of dy in expert order
 //        kDX      O = dGU W12^T                       fp32, one row per pair
-//        kDW12, kDW3   X^T dGU and H^T dY per expert  K = the expert's rows
 //    permute_kernel copies rows into expert order.  With few rows per expert the copy engine picks
 //    them itself instead (kGateUpGather, tile::gather4, one lane per four rows): a gather of four
 //    128-byte row pieces was measured to take about as long as a whole box of rows (40-75 cycles),
-//    so 128 rows by gathers cost 2.3 times the tensor cores' time (8192 tokens, 64 experts
-//    2048/1024: gate/up product 1287 us gathered), while a few rows cost nothing and save a launch.
-//    The routing weight is applied to the hidden activation before it is rounded: the rows of O
+//    so many rows are better copied once (8192 tokens, 64 experts 2048/1024: gate/up product
+//    1287 us gathered, 420 us copied), while a few rows cost nothing and save a launch.
+//  * moe_wgrad_kernel computes X^T dGU and H^T dY per expert, K = the expert's rows.
+//  * The routing weight is applied to the hidden activation before it is rounded: the rows of O
 //    only need adding, and H is the very operand dW3 needs, so no value on the way is rounded
-//    twice.
-//  * combine_kernel adds a token's rows of O in slot order (fp32) and rounds once.
+//    twice.  combine_kernel adds a token's rows of O in slot order (fp32) and rounds once.
 //  * The gate/up products are kept in fp32 for the backward pass: rounding them to 16 bits would
 //    add two more roundings to every gradient.
 #include <cuda.h>
@@ -29,8 +35,8 @@
 #include <cuda_runtime.h>
 
 #include <mutex>
+#include <type_traits>
 #include <utility>
-#include <vector>
 
 #include "tnx_elem.cuh"
 #include "tnx_internal.h"
@@ -41,13 +47,17 @@ namespace tnx {
 namespace {
 
 constexpr int kMaxExperts = 512;
-constexpr int kRows = 128;       // rows per CTA (TMEM lanes)
+constexpr int kRows = 128;       // rows of the M operand per CTA (TMEM lanes); a pair has 256
+constexpr int kTileN = 256;      // columns of the N operand per pair at most
+constexpr int kPad = 16;         // an expert's rows are padded to this: one MMA's K
 constexpr int kTileK = 64;       // K elements per ring slot: one 128-byte swizzle row
-constexpr int kThreads = 192;    // producer warp, MMA warp, four epilogue warps
-constexpr int kEpiThreads = 128;
-constexpr int kEpiBarrier = 1;
+constexpr int kThreads = 192;      // producer warp, MMA warp, four epilogue warps
+constexpr int kRowsEpilogue = 16;  // epilogue warps of the rows' kernel: four per quarter of the TMEM lanes
+constexpr int kRowsThreads = 64 + 32 * kRowsEpilogue;
 constexpr int kAtomBytes = 128;
-constexpr int kBoxBytes = kRows * kAtomBytes;  // a 128-row box of 128-byte rows
+constexpr int kStageBytes = 2 * kRows * kTileK * 2;  // 128 rows of each operand
+constexpr int kBoxBytes = 32 * kAtomBytes;           // an epilogue warp's box: 32 rows of 128 bytes
+constexpr int kBoxes = 2;                            // staging boxes per epilogue warp
 constexpr int kMaxStages = 8;
 constexpr int kCtrlBytes = 512;
 constexpr int kAlignSlack = 1024;
@@ -56,46 +66,44 @@ constexpr int kAbortProducer = 0x301;
 constexpr int kAbortMma = 0x302;
 constexpr int kAbortEpilogue = 0x303;
 
-enum Mode { kGateUp, kGateUpGather, kDown, kDHidden, kDX, kDW12, kDW3 };
-
-// What a mode's operands look like.
-template <int MODE>
-struct Traits {
-  static constexpr bool wgrad = MODE == kDW12 || MODE == kDW3;
-  static constexpr bool gather_a = MODE == kGateUpGather;
-  static constexpr bool gate_up = MODE == kGateUp || MODE == kGateUpGather;
-  static constexpr bool b_kmajor = MODE == kDHidden || MODE == kDX;
-};
-// Accumulator columns per tile.  (dHidden streams gate/up through shared memory as well; a
-// single CTA then has room for 128 columns only.)
-constexpr int tile_n(int mode, int cta_group) { return mode == kDHidden && cta_group == 1 ? 128 : 256; }
-constexpr int staging_boxes(int mode) { return mode == kDHidden ? 6 : 2; }
+enum Mode { kGateUp, kGateUpGather, kDown, kDHidden, kDX };
 
 // Where the pairs went (device memory, written by the plan kernels).
 struct Plan {
   int* tiles;        // [1] row tiles in use
   int* count;        // [experts] rows of an expert
-  int* start;        // [experts] its first (padded) row
-  int* tile_expert;  // [max_tiles]
+  int* start;        // [experts] its first row (a multiple of kPad)
+  int4* tile;        // [max_tiles] expert, first row, rows in use, rows up to the padding
   int* row_token;    // [max_rows] token of a row (rows in use only)
   float* row_weight; // [max_rows]
   int* pos;          // [pairs] row of a pair, -1 where its id is no expert
 };
 
-struct GemmParams {
+struct RowsParams {
+  Plan plan;
+  int num_kb, splits, kb_per_split;  // K blocks; slices of K, each with its own copy of O
+  int cols;         // columns of the weight operand: 2 d_ff, n_out, d_ff or d_model
+  int tiles_n;      // tiles of 256 of them
+  int panels;       // the weights' map takes two 64-column panels at a time
+  int band;         // row tiles per band of the tile order
+  int activation;
+  int train;        // gate/up: keep the fp32 products, write padding rows as zeros
+  long long max_rows;
+  void* out;        // H, dGU (16 bit) or O (fp32, [splits][max_rows][cols])
+  float* gu;        // [max_rows][2 d_ff]: written by gate/up, read by kDHidden
+  float* dw_part;   // kDHidden: [max_rows][dw_parts], one sum per 32 columns
+  int dw_parts;
+  int stages;
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+struct WgradParams {
   Plan plan;
   int experts;
-  int tile_rows;   // rows per row tile (kRows * CTA_GROUP)
-  int num_kb;      // K blocks (not wgrad)
-  int cols;        // output columns in accumulator columns
-  int tiles_n;     // column tiles
-  int band;        // row tiles per band of the tile order
-  int tiles_m;     // wgrad: row tiles of the weight
-  int m;           // wgrad: rows of the weight
-  int activation;
-  int save_gu;     // gate/up: also store the fp32 products
-  float* part;     // kDown, kDX: O, [max_rows, cols]
-  float* dw_part;  // kDHidden: [max_rows, tiles_n]
+  int m, n;              // rows and columns of a weight's gradient
+  int tiles_m, tiles_n;  // 256 x 256 tiles
+  int panels_a, panels_b;  // whether the operands' maps take two 64-column panels at a time
   int stages;
   int* status;
   unsigned long long timeout_ns;
@@ -106,7 +114,6 @@ struct Ctrl {
   uint64_t empty[kMaxStages];
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
-  uint64_t gu_full[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -124,7 +131,7 @@ struct PlanParams {
   Plan plan;
   const void* ids;
   const float* weights;
-  int wide, experts, top_k, pairs, tile_rows;
+  int wide, experts, top_k, pairs;
   int chunk;          // pairs per warp, a multiple of 32
   int chunks;
   int* chunk_counts;  // [chunks][experts] (large problems)
@@ -169,32 +176,46 @@ __device__ __forceinline__ void place_chunk(const PlanParams& p, int first, int 
   });
 }
 
-// Given total[e] in shared memory: first row of every expert (in start[]), row tiles and their
-// experts.  All threads of the block take part.
-__device__ __forceinline__ void lay_out(const PlanParams& p, const int* total, int* start) {
+// Given total[e] in shared memory: first row of every expert (in start[]) and the row tiles.  An
+// expert's rows are cut into as few tiles of at most kTileN rows as possible, of equal size up to
+// a multiple of 32.  All threads of the block take part; tile0[] is scratch.
+__device__ __forceinline__ void lay_out(const PlanParams& p, const int* total, int* start, int* tile0) {
   const int tid = threadIdx.x;
   if (tid < 32) {
-    int carry = 0;
+    int rows_before = 0, tiles_before = 0;
     for (int base = 0; base < p.experts; base += 32) {
       const int e = base + tid;
-      const int tiles = e < p.experts ? (total[e] + p.tile_rows - 1) / p.tile_rows : 0;
-      int sum = tiles;
+      const int count = e < p.experts ? total[e] : 0;
+      const int rows = (count + kPad - 1) / kPad * kPad, tiles = (count + kTileN - 1) / kTileN;
+      int row_sum = rows, tile_sum = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (tid >= o) sum += v;
+        const int r = __shfl_up_sync(0xffffffffu, row_sum, o), t = __shfl_up_sync(0xffffffffu, tile_sum, o);
+        if (tid >= o) {
+          row_sum += r;
+          tile_sum += t;
+        }
       }
-      if (e < p.experts) start[e] = (carry + sum - tiles) * p.tile_rows;
-      carry += __shfl_sync(0xffffffffu, sum, 31);
+      if (e < p.experts) {
+        start[e] = rows_before + row_sum - rows;
+        tile0[e] = tiles_before + tile_sum - tiles;
+      }
+      rows_before += __shfl_sync(0xffffffffu, row_sum, 31);
+      tiles_before += __shfl_sync(0xffffffffu, tile_sum, 31);
     }
-    if (tid == 0) *p.plan.tiles = carry;
+    if (tid == 0) *p.plan.tiles = tiles_before;
   }
   __syncthreads();
   for (int e = tid; e < p.experts; e += blockDim.x) {
-    p.plan.count[e] = total[e];
+    const int count = total[e];
+    p.plan.count[e] = count;
     p.plan.start[e] = start[e];
-    const int t0 = start[e] / p.tile_rows, tiles = (total[e] + p.tile_rows - 1) / p.tile_rows;
-    for (int i = 0; i < tiles; ++i) p.plan.tile_expert[t0 + i] = e;
+    const int tiles = (count + kTileN - 1) / kTileN;
+    const int size = tiles > 0 ? ((count + tiles - 1) / tiles + 31) / 32 * 32 : 0;
+    for (int i = 0; i < tiles; ++i) {
+      const int used = min(size, count - i * size);
+      p.plan.tile[tile0[e] + i] = make_int4(e, start[e] + i * size, used, (used + kPad - 1) / kPad * kPad);
+    }
   }
 }
 
@@ -205,6 +226,7 @@ struct SmallPlanSmem {
   int next[kSmallWarps][kMaxExperts];
   int total[kMaxExperts];
   int start[kMaxExperts];
+  int tile0[kMaxExperts];
 };
 __global__ void __launch_bounds__(kSmallWarps * 32) plan_small_kernel(const PlanParams p) {
   extern __shared__ uint8_t plan_smem[];
@@ -228,7 +250,7 @@ __global__ void __launch_bounds__(kSmallWarps * 32) plan_small_kernel(const Plan
     s.total[e] = run;
   }
   __syncthreads();
-  lay_out(p, s.total, s.start);
+  lay_out(p, s.total, s.start, s.tile0);
   __syncthreads();
   for (int e = lane; e < p.experts; e += 32) s.next[warp][e] += s.start[e];
   __syncwarp();
@@ -253,7 +275,7 @@ __global__ void __launch_bounds__(kChunkWarps * 32) plan_count_kernel(const Plan
 }
 // Threads (expert, strand): a strand owns a run of chunks, its threads read neighbouring experts.
 __global__ void __launch_bounds__(1024) plan_scan_kernel(const PlanParams p) {
-  __shared__ int total[kMaxExperts], start[kMaxExperts], strand_sum[1024];
+  __shared__ int total[kMaxExperts], start[kMaxExperts], tile0[kMaxExperts], strand_sum[1024];
   dependency_wait();
   dependency_release();
   const int strands = 1024 / p.experts;
@@ -287,7 +309,7 @@ __global__ void __launch_bounds__(1024) plan_scan_kernel(const PlanParams p) {
       before += v[i];
     }
   }
-  lay_out(p, total, start);
+  lay_out(p, total, start, tile0);
 }
 __global__ void __launch_bounds__(kChunkWarps * 32) plan_place_kernel(const PlanParams p) {
   __shared__ int next[kChunkWarps][kMaxExperts];
@@ -309,7 +331,7 @@ __global__ void __launch_bounds__(kChunkWarps * 32) plan_place_kernel(const Plan
 __device__ __forceinline__ float2 gate_act(float g, int activation) {
   if (activation == TNX_EPI_GLU_LINEAR) return make_float2(g, 1.f);
   const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-  if (activation == TNX_EPI_GLU_SILU) return make_float2(g * s, s * (1.f + g * (1.f - s)));
+  if (activation == TNX_EPI_GLU_SILU) return make_float2(g * s, s + g * s * (1.f - s));
   return make_float2(s, s * (1.f - s));
 }
 
@@ -326,519 +348,45 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+// Four rows of 64 elements each, picked by row number, for a CTA pair (see ptx::tma_load_2d_pair).
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const void* tmap, int x, const int (&rows)[4],
+                                                 uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3]),
+      "r"(leader_bar)
+      : "memory");
 }
 
-// Four rows of 64 elements each, picked by row number.
-template <int CTA_GROUP>
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int x, const int (&rows)[4], uint32_t bar) {
-  if (CTA_GROUP == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3]), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3]), "r"(bar)
-        : "memory");
-}
-template <int CTA_GROUP>
-__device__ __forceinline__ void load_2d(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
-  if (CTA_GROUP == 1)
-    ptx::tma_load_2d(dst, tmap, x, y, bar);
-  else
-    ptx::tma_load_2d_pair(dst, tmap, x, y, bar);
-}
-template <int CTA_GROUP>
-__device__ __forceinline__ void load_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
-  if (CTA_GROUP == 1)
-    ptx::tma_load_3d(dst, tmap, x, y, z, bar);
-  else
-    ptx::tma_load_3d_pair(dst, tmap, x, y, z, bar);
-}
-
-// One output tile: which expert, where its rows start, how much K there is.
-struct Unit {
-  int expert;
-  int row0;    // first row: padded pair row, or (wgrad) row of the weight
-  int valid;   // rows in use from row0 on (may exceed the tile); wgrad: unused
-  int col0;    // first accumulator column
-  int tile_col;
-  int num_kb;
-  int k_row0;  // wgrad: first padded pair row of the expert
-  int k_rows;  // wgrad: its rows
-};
-
-template <int MODE, int TILE_N>
-__device__ __forceinline__ Unit decode_unit(const GemmParams& p, int u, int num_tiles) {
-  Unit r;
-  if (Traits<MODE>::wgrad) {
-    // an expert's tiles one after another, column tile by column tile
-    const int per = p.tiles_m * p.tiles_n;
-    r.expert = u / per;
-    const int rem = u - r.expert * per;
-    r.tile_col = rem / p.tiles_m;
-    r.row0 = (rem - r.tile_col * p.tiles_m) * p.tile_rows;
-    r.k_row0 = p.plan.start[r.expert];
-    r.k_rows = p.plan.count[r.expert];
-    r.num_kb = (r.k_rows + kTileK - 1) / kTileK;
-    r.valid = p.m - r.row0;
-  } else {
-    // bands of `band` row tiles, column tile by column tile inside a band: the CTAs at work share
-    // the weight tiles of few experts and the rows of one band through L2
-    const int full = p.band * p.tiles_n;
-    const int b = u / full;
-    const int rem = u - b * full;
-    const int rows = min(p.band, num_tiles - b * p.band);
-    r.tile_col = rem / rows;
-    const int t = b * p.band + (rem - r.tile_col * rows);
-    r.expert = p.plan.tile_expert[t];
-    r.row0 = t * p.tile_rows;
-    r.valid = p.plan.start[r.expert] + p.plan.count[r.expert] - r.row0;
-    r.num_kb = p.num_kb;
-    r.k_row0 = r.k_rows = 0;
-  }
-  r.col0 = r.tile_col * TILE_N;
-  return r;
-}
-
-template <int MODE, int CTA_GROUP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
-moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_gu,
-                const GemmParams p) {
-  using T = Traits<MODE>;
-  constexpr int TILE_N = tile_n(MODE, CTA_GROUP);
-  constexpr int LOAD_N = TILE_N / CTA_GROUP;  // B columns this CTA loads
-  constexpr int a_stage_bytes = kRows * kTileK * 2;
-  constexpr int b_stage_bytes = LOAD_N * kTileK * 2;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
-  const uint32_t base_addr = (raw_addr + 1023u) & ~1023u;
-  const uint32_t smem_a = base_addr;
-  const uint32_t smem_b = smem_a + p.stages * a_stage_bytes;
-  const uint32_t smem_out = smem_b + p.stages * b_stage_bytes;
-  const uint32_t smem_gu = smem_out + 2 * kBoxBytes;  // kDHidden: two sets of two boxes
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem_raw + (smem_out - raw_addr) + staging_boxes(MODE) * kBoxBytes);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  const uint32_t cta_rank = CTA_GROUP == 2 ? ptx::cluster_ctarank() : 0;
-  const bool leader = cta_rank == 0;
-  const int cluster_id = blockIdx.x / CTA_GROUP;
-  const int num_clusters = gridDim.x / CTA_GROUP;
-  volatile int* abort_flag = &ctrl->abort;
-
+// What both kernels share: barriers, the pair's rendezvous, 512 columns of TMEM (two accumulators
+// of 256), and their release.  Returns the TMEM base address.
+__device__ __forceinline__ uint32_t set_up_pair(Ctrl* ctrl, int stages, int epilogue_warps, int warp) {
   if (threadIdx.x == 0) {
-    ptx::prefetch_tensormap(&tmap_a);
-    ptx::prefetch_tensormap(&tmap_b);
-    for (int s = 0; s < p.stages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       ptx::mbar_init(ptx::smem_u32(&ctrl->full[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&ctrl->empty[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(ptx::smem_u32(&ctrl->tmem_full[a]), 1);
-      ptx::mbar_init(ptx::smem_u32(&ctrl->tmem_empty[a]), 4 * CTA_GROUP);  // one arrive per epilogue warp
-      ptx::mbar_init(ptx::smem_u32(&ctrl->gu_full[a]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctrl->tmem_empty[a]), 2 * epilogue_warps);  // one arrive each
     }
     ctrl->abort = 0;
     ptx::fence_mbar_init();
   }
   __syncwarp();
-  if (CTA_GROUP == 2) {  // the peer's barriers must exist before anything signals them
-    ptx::cluster_arrive();
-    ptx::cluster_wait();
-  }
+  ptx::cluster_arrive();  // the peer's barriers must exist before anything signals them
+  ptx::cluster_wait();
   if (warp == 1) {
-    ptx::tmem_alloc<CTA_GROUP>(ptx::smem_u32(&ctrl->tmem_base), 2 * TILE_N);
-    ptx::tmem_relinquish<CTA_GROUP>();
+    ptx::tmem_alloc<2>(ptx::smem_u32(&ctrl->tmem_base), 2 * kTileN);
+    ptx::tmem_relinquish<2>();
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
-  const uint32_t tmem_base = ctrl->tmem_base;
-  // Everything above touches no global memory and may run under the tail of the kernel before.
-  dependency_wait();
-  dependency_release();
-  const int num_tiles = T::wgrad ? 0 : *p.plan.tiles;
-  const int total_units = T::wgrad ? p.experts * p.tiles_m * p.tiles_n : num_tiles * p.tiles_n;
-
-  if (warp == 0) {
-    // ===== TMA producer: every lane issues its share of a stage's copies =====
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
-      const Unit un = decode_unit<MODE, TILE_N>(p, u, num_tiles);
-      const int row0 = un.row0 + static_cast<int>(cta_rank) * kRows;
-      const int b_col0 = un.col0 + static_cast<int>(cta_rank) * LOAD_N;
-      // Lanes that copy rows of A.  A tile of one CTA with few rows in use fetches only those (the
-      // MMA reads the slot's old contents in the other rows, which feed accumulator rows that are
-      // never stored); a pair always fetches all.
-      int a_lanes = T::gather_a ? 32 : T::wgrad ? 2 : 4;
-      if (CTA_GROUP == 1 && !T::wgrad && un.valid < kRows)
-        a_lanes = T::gather_a ? (un.valid + 3) / 4 : (un.valid + 31) / 32;
-      const uint32_t stage_tx =
-          static_cast<uint32_t>(CTA_GROUP * ((T::gather_a ? 512 : T::wgrad ? 8192 : 4096) * a_lanes + b_stage_bytes));
-      int rows[4] = {0, 0, 0, 0};
-      if (T::gather_a) {
-        // rows past the expert's last are copies of that one: addressable, and dropped later
-        const int last = un.row0 + un.valid - 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rows[i] = p.plan.row_token[min(row0 + 4 * lane + i, last)];
-      }
-      for (int kb = 0; kb < un.num_kb; ++kb) {
-        const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->empty[stage]), phase ^ 1u, abort_flag, p.timeout_ns);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
-        }
-        uint32_t bar = ptx::smem_u32(&ctrl->full[stage]);
-        if (leader && lane == 0) ptx::mbar_arrive_expect_tx(bar, stage_tx);
-        if (CTA_GROUP == 2) bar = ptx::mapa(bar, 0);  // both CTAs' copies complete on the leader's barrier
-        __syncwarp();
-        const uint32_t a_dst = smem_a + stage * a_stage_bytes;
-        const uint32_t b_dst = smem_b + stage * b_stage_bytes;
-        const int k0 = kb * kTileK;
-        if (T::wgrad) {
-          // K = pair rows; both operands lie in memory as (pair row, column), 64-column atoms
-          const int k_row = un.k_row0 + k0;
-          if (lane < 2) load_2d<CTA_GROUP>(a_dst + lane * 8192, &tmap_a, row0 + lane * 64, k_row, bar);
-          if (lane < LOAD_N / 64) load_2d<CTA_GROUP>(b_dst + lane * 8192, &tmap_b, b_col0 + lane * 64, k_row, bar);
-        } else {
-          if (T::gather_a) {
-            if (lane < a_lanes) tma_gather4<CTA_GROUP>(a_dst + lane * 512, &tmap_a, k0, rows, bar);
-          } else if (lane < a_lanes) {
-            load_2d<CTA_GROUP>(a_dst + lane * 4096, &tmap_a, k0, row0 + lane * 32, bar);
-          }
-          if (T::b_kmajor) {
-            if (lane == 0) load_3d<CTA_GROUP>(b_dst, &tmap_b, k0, b_col0, un.expert, bar);
-          } else if (lane < LOAD_N / 64) {
-            load_3d<CTA_GROUP>(b_dst + lane * 8192, &tmap_b, b_col0 + lane * 64, k0, un.expert, bar);
-          }
-        }
-        __syncwarp();
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortProducer);
-  } else if (warp == 1) {
-    // ===== MMA issuer (leader CTA) =====
-    if (leader && lane == 0) {
-      const uint32_t fmt = BF16 ? 1u : 0u;
-      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((T::wgrad ? 1u : 0u) << 15) |
-                             ((T::b_kmajor ? 0u : 1u) << 16) | (static_cast<uint32_t>(TILE_N >> 3) << 17) |
-                             (static_cast<uint32_t>((kRows * CTA_GROUP) >> 4) << 24);
-      // K-major operands: rows of 128 bytes, 16 elements of K = 32 bytes further.  MN-major ones:
-      // 64-wide atoms of 64 K rows x 128 bytes, 8192 bytes apart, 16 elements of K = 16 rows.
-      const uint64_t a_desc = T::wgrad ? ptx::make_smem_desc(0, 8192, 1024) : ptx::make_smem_desc(0, 0, 1024);
-      const uint64_t b_desc = T::b_kmajor ? ptx::make_smem_desc(0, 0, 1024) : ptx::make_smem_desc(0, 8192, 1024);
-      constexpr uint32_t a_step16 = (T::wgrad ? 2048u : 32u) >> 4;
-      constexpr uint32_t b_step16 = (T::b_kmajor ? 32u : 2048u) >> 4;
-      int stage = 0;
-      uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
-      bool ok = true;
-      for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
-        const int num_kb = T::wgrad ? decode_unit<MODE, TILE_N>(p, u, num_tiles).num_kb : p.num_kb;
-        if (num_kb == 0) continue;  // an expert without rows: the epilogue writes zeros by itself
-        if (!ptx::mbar_wait<CTA_GROUP == 2>(ptx::smem_u32(&ctrl->tmem_empty[acc]), acc_phase ^ 1u, abort_flag,
-                                            p.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + acc * TILE_N;
-        uint32_t accumulate = 0;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&ctrl->full[stage]), phase, abort_flag, p.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          ptx::tc_fence_after_sync();
-          const uint32_t a16 = (smem_a + stage * a_stage_bytes) >> 4;
-          const uint32_t b16 = (smem_b + stage * b_stage_bytes) >> 4;
-#pragma unroll
-          for (int k16 = 0; k16 < kTileK / 16; ++k16) {
-            ptx::umma_f16<CTA_GROUP>(d_tmem, a_desc | ((a16 + k16 * a_step16) & 0x3fffu),
-                                     b_desc | ((b16 + k16 * b_step16) & 0x3fffu), idesc, accumulate);
-            accumulate = 1;
-          }
-          if (CTA_GROUP == 1)
-            ptx::umma_commit(ptx::smem_u32(&ctrl->empty[stage]));
-          else
-            ptx::umma_commit_pair(ptx::smem_u32(&ctrl->empty[stage]), 0x3);
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (!ok) break;
-        if (CTA_GROUP == 1)
-          ptx::umma_commit(ptx::smem_u32(&ctrl->tmem_full[acc]));
-        else
-          ptx::umma_commit_pair(ptx::smem_u32(&ctrl->tmem_full[acc]), 0x3);
-        if (++acc == 2) {
-          acc = 0;
-          acc_phase ^= 1u;
-        }
-      }
-      if (!ok && p.status != nullptr) atomicCAS(p.status, 0, kAbortMma);
-    }
-  } else {
-    // ===== epilogue: warp w owns TMEM lanes 32 (w mod 4) ..., a thread owns a row =====
-    const int quarter = warp & 3;
-    const int row_in_tile = quarter * 32 + lane;
-    const int epi_tid = threadIdx.x - 64;
-    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t stage_row = static_cast<uint32_t>(row_in_tile) * kAtomBytes;
-    const uint32_t sw = static_cast<uint32_t>(row_in_tile & 7);
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    uint32_t stores = 0, gu_chunks = 0;
-    bool ok = true;
-    // Staging: begin() hands out a box that no store reads any more, end() sends it off.
-    auto begin = [&]() -> uint32_t {
-      if (epi_tid == 0) ptx::tma_store_wait_read<1>();
-      ptx::named_barrier_sync(kEpiBarrier, kEpiThreads);
-      return smem_out + (stores & 1u) * kBoxBytes;
-    };
-    auto end = [&]() {
-      ptx::fence_proxy_async_smem();
-      ptx::named_barrier_sync(kEpiBarrier, kEpiThreads);
-      ++stores;
-    };
-    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
-      const Unit un = decode_unit<MODE, TILE_N>(p, u, num_tiles);
-      const int row0 = un.row0 + static_cast<int>(cta_rank) * kRows;
-      const int rows_here = un.valid - static_cast<int>(cta_rank) * kRows;  // rows of this CTA in use (<= 0: none)
-      const bool live = row_in_tile < rows_here;
-
-      if (T::wgrad && un.num_kb == 0) {
-        // no rows: the gradient is zero
-        for (int col = 0; col < TILE_N; col += 64) {
-          if (un.col0 + col >= p.cols) break;
-          const uint32_t buf = begin();
-#pragma unroll
-          for (uint32_t piece = 0; piece < 8; ++piece) st_shared_v4(buf + stage_row + piece * 16, 0, 0, 0, 0);
-          end();
-          if (epi_tid == 0 && row0 < p.m) {
-            ptx::tma_store_3d(&tmap_c, un.col0 + col, row0, un.expert, buf);
-            ptx::tma_store_commit();
-          }
-        }
-        continue;
-      }
-
-      // kDHidden: this tile's gate/up products come in chunks of 32 hidden columns (two boxes of
-      // 32 fp32 columns), two chunks ahead.
-      const int gu_total = MODE == kDHidden ? (min(TILE_N, p.cols - un.col0) + 31) / 32 : 0;
-      auto fetch_gu = [&](int chunk, uint32_t ordinal) {
-        const uint32_t set = ordinal & 1u;
-        const uint32_t bar = ptx::smem_u32(&ctrl->gu_full[set]);
-        const uint32_t dst = smem_gu + set * (2 * kBoxBytes);
-        const int x = 2 * (un.col0 + chunk * 32);
-        ptx::mbar_arrive_expect_tx(bar, 2 * kBoxBytes);
-        ptx::tma_load_2d(dst, &tmap_gu, x, row0, bar);
-        ptx::tma_load_2d(dst + kBoxBytes, &tmap_gu, x + 32, row0, bar);
-      };
-      if (MODE == kDHidden && epi_tid == 0) {
-        fetch_gu(0, gu_chunks);
-        if (gu_total > 1) fetch_gu(1, gu_chunks + 1);
-      }
-      const float weight = !T::wgrad && live && (T::gate_up || MODE == kDHidden)
-                               ? p.plan.row_weight[row0 + row_in_tile] : 0.f;
-
-      const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc]), acc_phase, abort_flag, p.timeout_ns);
-      if (!ptx::named_barrier_all(kEpiBarrier, kEpiThreads, got)) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after_sync();
-      const uint32_t t_acc = tmem_base + lane_sel + acc * TILE_N;
-      uint32_t r[32];
-
-      if (T::gate_up) {
-        if (p.save_gu) {
-          for (int col = 0; col < TILE_N; col += 32) {
-            if (un.col0 + col >= p.cols) break;
-            const uint32_t buf = begin();
-            ptx::tmem_ld_32x32(t_acc + col, r);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (uint32_t piece = 0; piece < 8; ++piece)
-              st_shared_v4(buf + stage_row + (piece ^ sw) * 16, r[piece * 4], r[piece * 4 + 1], r[piece * 4 + 2],
-                           r[piece * 4 + 3]);
-            end();
-            if (epi_tid == 0) {
-              ptx::tma_store_2d(&tmap_gu, un.col0 + col, row0, buf);
-              ptx::tma_store_commit();
-            }
-          }
-        }
-        for (int col = 0; col < TILE_N; col += 128) {
-          if (un.col0 + col >= p.cols) break;
-          const uint32_t buf = begin();
-#pragma unroll
-          for (int sub = 0; sub < 4; ++sub) {
-            ptx::tmem_ld_32x32(t_acc + col + sub * 32, r);
-            ptx::tmem_ld_wait();
-            uint32_t o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float z0 = weight * gate_act(__uint_as_float(r[4 * j]), p.activation).x * __uint_as_float(r[4 * j + 1]);
-              const float z1 = weight * gate_act(__uint_as_float(r[4 * j + 2]), p.activation).x * __uint_as_float(r[4 * j + 3]);
-              o[j] = live ? pack2<BF16>(z0, z1) : 0u;
-            }
-#pragma unroll
-            for (uint32_t piece = 0; piece < 2; ++piece)
-              st_shared_v4(buf + stage_row + ((sub * 2 + piece) ^ sw) * 16, o[piece * 4], o[piece * 4 + 1],
-                           o[piece * 4 + 2], o[piece * 4 + 3]);
-          }
-          end();
-          if (epi_tid == 0) {
-            ptx::tma_store_2d(&tmap_c, (un.col0 + col) / 2, row0, buf);
-            ptx::tma_store_commit();
-          }
-        }
-      } else if (MODE == kDown || MODE == kDX) {
-        if (rows_here <= 32) {
-          // few rows: straight from registers, so that unused rows cost no bytes
-          if (quarter == 0) {
-            float* dst = p.part + static_cast<long long>(row0 + row_in_tile) * p.cols + un.col0;
-            for (int col = 0; col < TILE_N; col += 32) {
-              if (un.col0 + col >= p.cols) break;
-              ptx::tmem_ld_32x32(t_acc + col, r);
-              ptx::tmem_ld_wait();
-              if (live) {
-#pragma unroll
-                for (int piece = 0; piece < 8; ++piece)
-                  if (un.col0 + col + piece * 4 < p.cols)
-                    *reinterpret_cast<float4*>(dst + col + piece * 4) =
-                        make_float4(__uint_as_float(r[piece * 4]), __uint_as_float(r[piece * 4 + 1]),
-                                    __uint_as_float(r[piece * 4 + 2]), __uint_as_float(r[piece * 4 + 3]));
-              }
-            }
-          }
-        } else {
-          for (int col = 0; col < TILE_N; col += 32) {
-            if (un.col0 + col >= p.cols) break;
-            const uint32_t buf = begin();
-            ptx::tmem_ld_32x32(t_acc + col, r);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (uint32_t piece = 0; piece < 8; ++piece)
-              st_shared_v4(buf + stage_row + (piece ^ sw) * 16, r[piece * 4], r[piece * 4 + 1], r[piece * 4 + 2],
-                           r[piece * 4 + 3]);
-            end();
-            if (epi_tid == 0) {
-              ptx::tma_store_2d(&tmap_c, un.col0 + col, row0, buf);
-              ptx::tma_store_commit();
-            }
-          }
-        }
-      } else if (MODE == kDHidden) {
-        float dw = 0.f;
-        for (int chunk = 0; chunk < gu_total; ++chunk, ++gu_chunks) {
-          const uint32_t set = gu_chunks & 1u;
-          const bool here =
-              ptx::mbar_wait(ptx::smem_u32(&ctrl->gu_full[set]), (gu_chunks >> 1) & 1u, abort_flag, p.timeout_ns);
-          if (epi_tid == 0) ptx::tma_store_wait_read<1>();
-          if (!ptx::named_barrier_all(kEpiBarrier, kEpiThreads, here)) {
-            ok = false;
-            break;
-          }
-          const uint32_t buf = smem_out + (stores & 1u) * kBoxBytes;
-          const uint32_t gu = smem_gu + set * (2 * kBoxBytes) + stage_row;
-          ptx::tmem_ld_32x32(t_acc + chunk * 32, r);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (uint32_t half = 0; half < 2; ++half) {
-#pragma unroll
-            for (uint32_t piece = 0; piece < 4; ++piece) {
-              // four hidden columns: eight products, eight gradients, 16 bytes of output
-              uint32_t o[4];
-#pragma unroll
-              for (uint32_t q = 0; q < 2; ++q) {
-                const float4 v = ld_shared_v4(gu + half * kBoxBytes + ((piece * 2 + q) ^ sw) * 16);
-                const int j = half * 16 + piece * 4 + q * 2;
-                const float d0 = __uint_as_float(r[j]), d1 = __uint_as_float(r[j + 1]);
-                const float2 a0 = gate_act(v.x, p.activation), a1 = gate_act(v.z, p.activation);
-                // (columns past the last are zero in both operands)
-                dw += d0 * (a0.x * v.y) + d1 * (a1.x * v.w);
-                o[q * 2] = live ? pack2<BF16>(weight * d0 * v.y * a0.y, weight * d0 * a0.x) : 0u;
-                o[q * 2 + 1] = live ? pack2<BF16>(weight * d1 * v.w * a1.y, weight * d1 * a1.x) : 0u;
-              }
-              st_shared_v4(buf + stage_row + ((half * 4 + piece) ^ sw) * 16, o[0], o[1], o[2], o[3]);
-            }
-          }
-          end();
-          if (epi_tid == 0) {
-            ptx::tma_store_2d(&tmap_c, 2 * (un.col0 + chunk * 32), row0, buf);
-            ptx::tma_store_commit();
-            // (the barrier in end() says that everyone has read this chunk)
-            if (chunk + 2 < gu_total) fetch_gu(chunk + 2, gu_chunks + 2);
-          }
-        }
-        if (!ok) break;
-        if (live) p.dw_part[static_cast<long long>(row0 + row_in_tile) * p.tiles_n + un.tile_col] = dw;
-      } else {
-        for (int col = 0; col < TILE_N; col += 64) {
-          if (un.col0 + col >= p.cols) break;
-          const uint32_t buf = begin();
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            ptx::tmem_ld_32x32(t_acc + col + sub * 32, r);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (uint32_t piece = 0; piece < 4; ++piece)
-              st_shared_v4(buf + stage_row + ((sub * 4 + piece) ^ sw) * 16,
-                           pack2<BF16>(__uint_as_float(r[piece * 8]), __uint_as_float(r[piece * 8 + 1])),
-                           pack2<BF16>(__uint_as_float(r[piece * 8 + 2]), __uint_as_float(r[piece * 8 + 3])),
-                           pack2<BF16>(__uint_as_float(r[piece * 8 + 4]), __uint_as_float(r[piece * 8 + 5])),
-                           pack2<BF16>(__uint_as_float(r[piece * 8 + 6]), __uint_as_float(r[piece * 8 + 7])));
-          }
-          end();
-          // (the second CTA of a pair may lie past the last row altogether)
-          if (epi_tid == 0 && row0 < p.m) {
-            ptx::tma_store_3d(&tmap_c, un.col0 + col, row0, un.expert, buf);
-            ptx::tma_store_commit();
-          }
-        }
-      }
-      // All loads of this accumulator are complete: hand the TMEM buffer back.
-      ptx::tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        const uint32_t te = ptx::smem_u32(&ctrl->tmem_empty[acc]);
-        if (leader)
-          ptx::mbar_arrive(te);
-        else
-          ptx::mbar_arrive_cluster(ptx::mapa(te, 0));
-      }
-      if (++acc == 2) {
-        acc = 0;
-        acc_phase ^= 1u;
-      }
-    }
-    if (epi_tid == 0) ptx::tma_store_wait_all<0>();
-    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortEpilogue);
-  }
-
-  // ------------------------------------------------------------------ teardown
+  return ctrl->tmem_base;
+}
+__device__ __forceinline__ void tear_down_pair(Ctrl* ctrl, uint32_t tmem_base, int warp) {
   ptx::tc_fence_before_sync();
   __syncthreads();
   if (ctrl->abort != 0) {
@@ -848,22 +396,563 @@ moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     while (ptx::globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
   }
   __syncwarp();
-  if (CTA_GROUP == 2) {
-    ptx::cluster_arrive();
-    ptx::cluster_wait();
-  }
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
   if (warp == 1) {
     __syncwarp();
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc<CTA_GROUP>(tmem_base, 2 * TILE_N);
+    ptx::tmem_dealloc<2>(tmem_base, 2 * kTileN);
   }
+}
+// An epilogue warp has read all it needs of accumulator `acc`.
+__device__ __forceinline__ void release_accumulator(Ctrl* ctrl, int acc, bool leader, int lane) {
+  ptx::tc_fence_before_sync();
+  __syncwarp();
+  if (lane == 0) {
+    const uint32_t te = ptx::smem_u32(&ctrl->tmem_empty[acc]);
+    if (leader)
+      ptx::mbar_arrive(te);
+    else
+      ptx::mbar_arrive_cluster(ptx::mapa(te, 0));
+  }
+}
+// Ring position / accumulator that advances with its phase bit.
+struct Cursor {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++at == size) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// One tile: a row tile of an expert and 256 columns of its weights (and a slice of K).
+struct Unit {
+  int expert, row0, used, padded;  // as in Plan::tile
+  int n;                           // `used` up to a multiple of 32: N of the product
+  int col0;
+  int slice, kb0, num_kb;
+};
+template <int MODE>
+__device__ __forceinline__ Unit decode_unit(const RowsParams& p, int u, int num_tiles) {
+  Unit r;
+  r.slice = 0;
+  if (MODE == kDown || MODE == kDX) {
+    r.slice = u % p.splits;
+    u /= p.splits;
+  }
+  // bands of `band` row tiles, column tile by column tile inside a band: the pairs at work share the
+  // weight tiles of few experts and the rows of one band through L2
+  const int full = p.band * p.tiles_n;
+  const int b = u / full;
+  const int rem = u - b * full;
+  const int rows = min(p.band, num_tiles - b * p.band);
+  const int col = rem / rows;
+  const int4 tile = p.plan.tile[b * p.band + (rem - col * rows)];
+  r.expert = tile.x;
+  r.row0 = tile.y;
+  r.used = tile.z;
+  r.padded = tile.w;
+  r.n = (tile.z + 31) / 32 * 32;
+  r.col0 = col * (2 * kRows);
+  r.kb0 = r.slice * p.kb_per_split;
+  r.num_kb = min(p.kb_per_split, p.num_kb - r.kb0);
+  return r;
+}
+
+// Sum over the lanes of v[t] for every t, left in lane t.  31 exchanges: each halves the values a
+// lane still carries.
+__device__ __forceinline__ float transposed_sum(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = upper ? v[i] : v[i + o];
+      const float got = __shfl_xor_sync(0xffffffffu, give, o);
+      v[i] = (upper ? v[i + o] : v[i]) + got;
+    }
+  }
+  return v[0];
+}
+
+// What an epilogue warp reads from memory for 32 rows, before it needs it.
+template <int MODE>
+struct Prefetched {
+  float weight = 0.f;  // routing weight of row j0 + lane, 0 for padding
+  __device__ __forceinline__ void fetch(const RowsParams& p, const Unit& un, int j0, int) {
+    if (MODE == kGateUp || MODE == kGateUpGather)
+      weight = j0 + static_cast<int>(threadIdx.x & 31) < un.used ? p.plan.row_weight[un.row0 + j0 + (threadIdx.x & 31)] : 0.f;
+  }
+};
+template <>
+struct Prefetched<kDHidden> {
+  static constexpr int kBatch = 8;
+  float weight = 0.f;
+  float2 gu[kBatch];  // gate/up products of the first rows; write_rows fetches the others
+  // Rows and columns that do not exist are read at the tile's first and not used: no branches.
+  __device__ __forceinline__ static void batch(const RowsParams& p, const Unit& un, int j0, int col, float2 (&to)[kBatch]) {
+    const float2* src =
+        reinterpret_cast<const float2*>(p.gu) + static_cast<long long>(un.row0) * p.cols + (col < p.cols ? col : 0);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      to[j] = __ldcs(src + static_cast<long long>(j0 + j < un.used ? j0 + j : 0) * p.cols);
+  }
+  __device__ __forceinline__ void fetch(const RowsParams& p, const Unit& un, int j0, int col) {
+    const int j = j0 + static_cast<int>(threadIdx.x & 31);
+    weight = j < un.used ? p.plan.row_weight[un.row0 + j] : 0.f;
+    batch(p, un, j0, col, gu);
+  }
+};
+
+// Output of 32 rows (from row j0 of the tile) x 32 columns (a lane each), r[j] = product of row j0 + j.
+// WHOLE: all rows are in use and all columns exist.
+template <int MODE, bool BF16, bool WHOLE>
+__device__ __forceinline__ void write_rows(const RowsParams& p, const Unit& un, int j0, int rows, int warp_col, int lane,
+                                           uint32_t (&r)[32], Prefetched<MODE>& pre) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const long long row = un.row0 + j0;
+  const int col = warp_col + lane;
+  const bool inside = WHOLE || col < p.cols;
+  const int used = un.used - j0, write = rows - j0;  // of these 32
+  if (MODE == kDown || MODE == kDX) {
+    float* dst = static_cast<float*>(p.out) + (un.slice * p.max_rows + row) * p.cols + col;
+#pragma unroll
+    for (int j = 0; j < 32; ++j, dst += p.cols)
+      if (WHOLE || (inside && j < write)) *dst = __uint_as_float(r[j]);
+  } else if (MODE == kGateUp || MODE == kGateUpGather) {
+    if (p.train) {
+      float* dst = p.gu + row * p.cols + col;
+#pragma unroll
+      for (int j = 0; j < 32; ++j, dst += p.cols)
+        if (WHOLE || (inside && j < used)) *dst = __uint_as_float(r[j]);
+    }
+    // Even lanes hold gates, odd lanes their up columns.  For four rows at a time: lanes of a pair
+    // exchange so that each has both products of one of two rows, then lanes two apart so that each
+    // has two neighbouring hidden columns of one row: 4 bytes to store.
+    const bool odd = (lane & 1) != 0, second = (lane & 2) != 0;
+    const int d_ff = p.cols >> 1, hidden_col = (warp_col >> 1) + (lane >> 2) * 2;
+    T* dst = static_cast<T*>(p.out) + (row + (lane & 1) + (lane & 2)) * d_ff + hidden_col;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4, dst += 4 * d_ff) {
+      if (!WHOLE && j >= write) break;
+      float z[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int ja = j + 2 * h;
+        const float x = __uint_as_float(__shfl_xor_sync(0xffffffffu, odd ? r[ja] : r[ja + 1], 1));
+        const float g = odd ? x : __uint_as_float(r[ja]);
+        const float up = odd ? __uint_as_float(r[ja + 1]) : x;
+        const float w = __shfl_sync(0xffffffffu, pre.weight, ja + (lane & 1));
+        z[h] = w * up * gate_act(g, p.activation).x;
+        if (!WHOLE && ja + (lane & 1) >= used) z[h] = 0.f;
+      }
+      const float y = __shfl_xor_sync(0xffffffffu, second ? z[0] : z[1], 2);
+      const uint32_t pair = second ? pack2<BF16>(y, z[1]) : pack2<BF16>(z[0], y);
+      if (WHOLE || (hidden_col < d_ff && j + (lane & 3) < write)) *reinterpret_cast<uint32_t*>(dst) = pair;
+    }
+  } else {
+    // dG = w dH up act'(gate), dUp = w dH act(gate); dw = sum over hidden columns of dH H
+    constexpr int kBatch = Prefetched<kDHidden>::kBatch;
+    auto& first = reinterpret_cast<Prefetched<kDHidden>&>(pre);
+    uint32_t* dst = static_cast<uint32_t*>(p.out) + row * p.cols + col;
+    float2 other[kBatch];
+    float dw[32];
+#pragma unroll
+    for (int b = 0; b < 32; b += 2 * kBatch) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        auto& now = h == 0 ? first.gu : other;
+        if (b + h * kBatch + kBatch < 32)
+          Prefetched<kDHidden>::batch(p, un, j0 + b + (h + 1) * kBatch, col, h == 0 ? other : first.gu);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i, dst += p.cols) {
+          const int j = b + h * kBatch + i;
+          const float d = __uint_as_float(r[j]);
+          const float2 a = gate_act(now[i].x, p.activation);
+          const float wd = __shfl_sync(0xffffffffu, first.weight, j) * d;
+          dw[j] = WHOLE || (inside && j < used) ? d * (a.x * now[i].y) : 0.f;
+          const uint32_t pair = pack2<BF16>(wd * now[i].y * a.y, wd * a.x);
+          if (WHOLE || (inside && j < write)) *dst = WHOLE || j < used ? pair : 0u;
+        }
+      }
+    }
+    const float sum = transposed_sum(dw, lane);
+    if (WHOLE || lane < used) p.dw_part[(row + lane) * p.dw_parts + (warp_col >> 5)] = sum;
+  }
+}
+
+// out^T[256 columns, n rows] = W^T rows^T for one expert's rows; see the top of the file.
+// tmap_w: the weights.  kGateUp, kDown: K runs down their rows, M along them: 64 x 64 boxes, two at
+// a time where the columns are whole panels of 64 (p.panels); kDHidden, kDX: M down, K along: 64 x
+// 128 boxes.  tmap_r128, tmap_r64, tmap_r16: the rows, 64 elements by that many (kGateUpGather:
+// tmap_r16 is x itself, one row high).  A stage is kept to two or three copies: the copy engine
+// takes some 50 to 75 cycles for each whatever its size, against 512 for the stage's products.
+template <int MODE, bool BF16>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_r128,
+                const __grid_constant__ CUtensorMap tmap_r64, const __grid_constant__ CUtensorMap tmap_r16,
+                const RowsParams p) {
+  constexpr bool gate_up = MODE == kGateUp || MODE == kGateUpGather;
+  constexpr bool gather = MODE == kGateUpGather;
+  constexpr bool w_kmajor = MODE == kDHidden || MODE == kDX;
+  constexpr int operand_bytes = kRows * kTileK * 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  const uint32_t smem_w = (raw_addr + 1023u) & ~1023u;
+  const uint32_t smem_r = smem_w + p.stages * operand_bytes;
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem_raw + (smem_r + p.stages * operand_bytes - raw_addr));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const bool leader = rank == 0;
+  const int cluster_id = blockIdx.x >> 1;
+  const int num_clusters = gridDim.x >> 1;
+  volatile int* abort_flag = &ctrl->abort;
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tmap_w);
+    ptx::prefetch_tensormap(&tmap_r128);
+    ptx::prefetch_tensormap(&tmap_r64);
+    ptx::prefetch_tensormap(&tmap_r16);
+  }
+  const uint32_t tmem_base = set_up_pair(ctrl, p.stages, kRowsEpilogue, warp);
+  // Everything above touches no global memory and may run under the tail of the kernel before.
+  dependency_wait();
+  dependency_release();
+  const int num_tiles = *p.plan.tiles;
+  const int total_units = num_tiles * p.tiles_n * p.splits;
+
+  if (warp == 0) {
+    // ===== TMA producer: every lane issues its share of a stage's copies =====
+    Cursor ring;
+    bool ok = true;
+    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+      const Unit un = decode_unit<MODE>(p, u, num_tiles);
+      const int half = un.n >> 1;  // rows each CTA fetches
+      const int row0 = un.row0 + rank * half;
+      const int w_col = un.col0 + rank * kRows;
+      // one box of 128 or 64 rows, read a little past the tile's last row, or up to two of 16
+      const int box = gather ? half : half > 64 ? 128 : half > 32 ? 64 : half;
+      const uint32_t stage_tx = 2u * static_cast<uint32_t>(operand_bytes + box * kAtomBytes);
+      int rows[4] = {0, 0, 0, 0};
+      if (gather) {
+        // rows past the last are copies of that one: addressable, and never stored
+        const int last = un.row0 + un.used - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rows[i] = p.plan.row_token[min(row0 + 4 * lane + i, last)];
+      }
+      for (int kb = 0; kb < un.num_kb; ++kb) {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->empty[ring.at]), ring.phase ^ 1u, abort_flag, p.timeout_ns);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full_bar = ptx::smem_u32(&ctrl->full[ring.at]);
+        if (leader && lane == 0) ptx::mbar_arrive_expect_tx(full_bar, stage_tx);
+        const uint32_t bar = ptx::mapa(full_bar, 0);  // both CTAs' copies complete on the leader's barrier
+        __syncwarp();
+        const uint32_t w_dst = smem_w + ring.at * operand_bytes;
+        const uint32_t r_dst = smem_r + ring.at * operand_bytes;
+        const int k0 = (un.kb0 + kb) * kTileK;
+        if (w_kmajor) {
+          if (lane == 31) ptx::tma_load_3d_pair(w_dst, &tmap_w, k0, w_col, un.expert, bar);
+        } else if (p.panels) {
+          if (lane == 31) ptx::tma_load_4d_pair(w_dst, &tmap_w, 0, k0, w_col >> 6, un.expert, bar);
+        } else if (lane >= 30) {
+          ptx::tma_load_3d_pair(w_dst + (lane - 30) * 8192, &tmap_w, w_col + (lane - 30) * 64, k0, un.expert, bar);
+        }
+        if (gather) {
+          if (4 * lane < half) tma_gather4_pair(r_dst + lane * 512, &tmap_r16, k0, rows, bar);
+        } else if (box >= 64) {
+          if (lane == 0) ptx::tma_load_2d_pair(r_dst, box == 64 ? &tmap_r64 : &tmap_r128, k0, row0, bar);
+        } else if (16 * lane < box) {
+          ptx::tma_load_2d_pair(r_dst + lane * 2048, &tmap_r16, k0, row0 + lane * 16, bar);
+        }
+        __syncwarp();
+        ring.next(p.stages);
+      }
+    }
+    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortProducer);
+  } else if (warp == 1) {
+    // ===== MMA issuer (leader CTA) =====
+    if (leader && lane == 0) {
+      const uint32_t fmt = BF16 ? 1u : 0u;
+      // fp32 accumulate, M = 256 weight columns, N = the tile's rows (K-major)
+      const uint32_t idesc_base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_kmajor ? 0u : 1u) << 15) |
+                                  (static_cast<uint32_t>((kRows * 2) >> 4) << 24);
+      // K-major operands: rows of 128 bytes, 16 elements of K = 32 bytes further.  An M-major one:
+      // 64-wide atoms of 64 K rows x 128 bytes, 8192 bytes apart, 16 elements of K = 16 rows.
+      const uint64_t w_desc = w_kmajor ? ptx::make_smem_desc(0, 0, 1024) : ptx::make_smem_desc(0, 8192, 1024);
+      const uint64_t r_desc = ptx::make_smem_desc(0, 0, 1024);
+      constexpr uint32_t w_step16 = (w_kmajor ? 32u : 2048u) >> 4;
+      Cursor ring, acc;
+      bool ok = true;
+      for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+        const Unit un = decode_unit<MODE>(p, u, num_tiles);
+        const uint32_t idesc = idesc_base | (static_cast<uint32_t>(un.n >> 3) << 17);
+        if (!ptx::mbar_wait<true>(ptx::smem_u32(&ctrl->tmem_empty[acc.at]), acc.phase ^ 1u, abort_flag, p.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc.at * kTileN;
+        uint32_t accumulate = 0;
+        for (int kb = 0; kb < un.num_kb; ++kb) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&ctrl->full[ring.at]), ring.phase, abort_flag, p.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after_sync();
+          const uint32_t w16 = (smem_w + ring.at * operand_bytes) >> 4;
+          const uint32_t r16 = (smem_r + ring.at * operand_bytes) >> 4;
+#pragma unroll
+          for (int k16 = 0; k16 < kTileK / 16; ++k16) {
+            ptx::umma_f16<2>(d_tmem, w_desc | ((w16 + k16 * w_step16) & 0x3fffu), r_desc | ((r16 + k16 * 2u) & 0x3fffu),
+                             idesc, accumulate);
+            accumulate = 1;
+          }
+          ptx::umma_commit_pair(ptx::smem_u32(&ctrl->empty[ring.at]), 0x3);
+          ring.next(p.stages);
+        }
+        if (!ok) break;
+        ptx::umma_commit_pair(ptx::smem_u32(&ctrl->tmem_full[acc.at]), 0x3);
+        acc.next(2);
+      }
+      if (!ok && p.status != nullptr) atomicCAS(p.status, 0, kAbortMma);
+    }
+  } else {
+    // ===== epilogue: warp w owns TMEM lanes 32 (w mod 4) ..., i.e. 32 columns of the output; a
+    // register is a row.  Four warps share the columns and take every fourth 32 rows.  A warp's
+    // arithmetic is one dependent chain after another (about 7 cycles per instruction were
+    // measured), so it takes this many warps to stay ahead of the products: with four (eight)
+    // the gate/up product of 8192 tokens, 64 experts 2048/1024 took 523 (449) us. =====
+    const int quarter = warp & 3;
+    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
+    const int first_row = ((warp - 2) >> 2) * 32;
+    constexpr int kStep = 8 * kRowsEpilogue;  // rows from one of a warp's chunks to its next
+    Cursor acc;
+    bool ok = true;
+    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+      const Unit un = decode_unit<MODE>(p, u, num_tiles);
+      const int warp_col = un.col0 + rank * kRows + quarter * 32;
+      // rows to write: those in use, and in a training step the zeros that pad an expert
+      const int rows = (gate_up || MODE == kDHidden) && p.train ? un.padded : un.used;
+      const int mine = warp_col < p.cols ? rows : 0;  // (warp-uniform)
+      Prefetched<MODE> pre;
+      if (first_row < mine) pre.fetch(p, un, first_row, warp_col + lane);
+
+      const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc.at]), acc.phase, abort_flag, p.timeout_ns);
+      if (!__all_sync(0xffffffffu, got)) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      const uint32_t t_acc = tmem_base + lane_sel + acc.at * kTileN;
+      for (int j0 = first_row; j0 < mine; j0 += kStep) {
+        uint32_t r[32];
+        ptx::tmem_ld_32x32(t_acc + j0, r);
+        ptx::tmem_ld_wait(r);
+        const bool whole = j0 + 32 <= un.used && warp_col + 32 <= p.cols;
+        if (whole)
+          write_rows<MODE, BF16, true>(p, un, j0, rows, warp_col, lane, r, pre);
+        else
+          write_rows<MODE, BF16, false>(p, un, j0, rows, warp_col, lane, r, pre);
+        if (j0 + kStep < mine) pre.fetch(p, un, j0 + kStep, warp_col + lane);
+      }
+      release_accumulator(ctrl, acc.at, leader, lane);
+      acc.next(2);
+    }
+    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortEpilogue);
+  }
+  tear_down_pair(ctrl, tmem_base, warp);
+}
+
+// out[e] (m x n) = A[rows of e]^T B[rows of e]: tmap_a and tmap_b are 64 x 64 boxes over matrices of
+// rows in expert order, tmap_c 64 x 32 boxes over the gradients.  An expert's last K block ends at
+// the padding (zeros in both operands): one to four MMAs of 16 rows.
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+moe_wgrad_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_c, const WgradParams p) {
+  constexpr int operand_bytes = kRows * kTileK * 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  const uint32_t smem_a = (raw_addr + 1023u) & ~1023u;
+  const uint32_t smem_b = smem_a + p.stages * operand_bytes;
+  const uint32_t smem_out = smem_b + p.stages * operand_bytes;
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem_raw + (smem_out + 4 * kBoxes * kBoxBytes - raw_addr));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const bool leader = rank == 0;
+  const int cluster_id = blockIdx.x >> 1;
+  const int num_clusters = gridDim.x >> 1;
+  volatile int* abort_flag = &ctrl->abort;
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tmap_a);
+    ptx::prefetch_tensormap(&tmap_b);
+    ptx::prefetch_tensormap(&tmap_c);
+  }
+  const uint32_t tmem_base = set_up_pair(ctrl, p.stages, 4, warp);
+  dependency_wait();
+  dependency_release();
+  const int per_expert = p.tiles_m * p.tiles_n;
+  const int total_units = p.experts * per_expert;
+
+  if (warp == 0) {
+    Cursor ring;
+    bool ok = true;
+    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+      const int e = u / per_expert, rem = u - e * per_expert, tn = rem / p.tiles_m;
+      const int m0 = (rem - tn * p.tiles_m) * (2 * kRows) + rank * kRows;
+      const int n0 = tn * kTileN + rank * kRows;
+      const int k_row0 = p.plan.start[e], num_kb = (p.plan.count[e] + kTileK - 1) / kTileK;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->empty[ring.at]), ring.phase ^ 1u, abort_flag, p.timeout_ns);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full_bar = ptx::smem_u32(&ctrl->full[ring.at]);
+        if (leader && lane == 0) ptx::mbar_arrive_expect_tx(full_bar, 4u * operand_bytes);
+        const uint32_t bar = ptx::mapa(full_bar, 0);
+        __syncwarp();
+        const int k = k_row0 + kb * kTileK;
+        const uint32_t a_dst = smem_a + ring.at * operand_bytes, b_dst = smem_b + ring.at * operand_bytes;
+        if (p.panels_a) {
+          if (lane == 0) ptx::tma_load_4d_pair(a_dst, &tmap_a, 0, k, m0 >> 6, 0, bar);
+        } else if (lane < 2) {
+          ptx::tma_load_2d_pair(a_dst + lane * 8192, &tmap_a, m0 + lane * 64, k, bar);
+        }
+        if (p.panels_b) {
+          if (lane == 2) ptx::tma_load_4d_pair(b_dst, &tmap_b, 0, k, n0 >> 6, 0, bar);
+        } else if (lane == 2 || lane == 3) {
+          ptx::tma_load_2d_pair(b_dst + (lane - 2) * 8192, &tmap_b, n0 + (lane - 2) * 64, k, bar);
+        }
+        __syncwarp();
+        ring.next(p.stages);
+      }
+    }
+    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortProducer);
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      const uint32_t fmt = BF16 ? 1u : 0u;
+      // fp32 accumulate, both operands MN-major, 256 x 256
+      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
+                             (static_cast<uint32_t>(kTileN >> 3) << 17) | (static_cast<uint32_t>((kRows * 2) >> 4) << 24);
+      const uint64_t desc = ptx::make_smem_desc(0, 8192, 1024);
+      Cursor ring, acc;
+      bool ok = true;
+      for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+        const int count = p.plan.count[u / per_expert];
+        const int num_kb = (count + kTileK - 1) / kTileK;
+        if (num_kb == 0) continue;  // an expert without rows: the epilogue writes zeros by itself
+        if (!ptx::mbar_wait<true>(ptx::smem_u32(&ctrl->tmem_empty[acc.at]), acc.phase ^ 1u, abort_flag, p.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc.at * kTileN;
+        uint32_t accumulate = 0;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&ctrl->full[ring.at]), ring.phase, abort_flag, p.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after_sync();
+          const uint32_t a16 = (smem_a + ring.at * operand_bytes) >> 4;
+          const uint32_t b16 = (smem_b + ring.at * operand_bytes) >> 4;
+          const int steps = min(kTileK / 16, (count - kb * kTileK + 15) / 16);
+#pragma unroll
+          for (int k16 = 0; k16 < kTileK / 16; ++k16) {
+            if (k16 < steps)
+              ptx::umma_f16<2>(d_tmem, desc | ((a16 + k16 * 128u) & 0x3fffu), desc | ((b16 + k16 * 128u) & 0x3fffu),
+                               idesc, accumulate);
+            accumulate = 1;
+          }
+          ptx::umma_commit_pair(ptx::smem_u32(&ctrl->empty[ring.at]), 0x3);
+          ring.next(p.stages);
+        }
+        if (!ok) break;
+        ptx::umma_commit_pair(ptx::smem_u32(&ctrl->tmem_full[acc.at]), 0x3);
+        acc.next(2);
+      }
+      if (!ok && p.status != nullptr) atomicCAS(p.status, 0, kAbortMma);
+    }
+  } else {
+    // a thread owns a row of the tile, a warp stages boxes of 32 rows x 64 columns and stores them
+    const int quarter = warp & 3;
+    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t my_smem = smem_out + quarter * (kBoxes * kBoxBytes);
+    const uint32_t stage_row = static_cast<uint32_t>(lane) * kAtomBytes;
+    const uint32_t sw = static_cast<uint32_t>(lane & 7);
+    Cursor acc;
+    uint32_t stores = 0;
+    bool ok = true;
+    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+      const int e = u / per_expert, rem = u - e * per_expert, tn = rem / p.tiles_m;
+      const int row0 = (rem - tn * p.tiles_m) * (2 * kRows) + rank * kRows + quarter * 32;
+      const int n0 = tn * kTileN;
+      const bool empty = p.plan.count[e] == 0;
+      if (!empty) {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc.at]), acc.phase, abort_flag, p.timeout_ns);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after_sync();
+      }
+      const uint32_t t_acc = tmem_base + lane_sel + acc.at * kTileN;
+      for (int c = 0; c < kTileN && row0 < p.m && n0 + c < p.n; c += 64) {
+        // a box that no store reads any more
+        if (lane == 0) ptx::tma_store_wait_read<kBoxes - 1>();
+        __syncwarp();
+        const uint32_t buf = my_smem + (stores++ % kBoxes) * kBoxBytes;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          uint32_t r[32];
+          if (!empty) {
+            ptx::tmem_ld_32x32(t_acc + c + sub * 32, r);
+            ptx::tmem_ld_wait(r);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          }
+#pragma unroll
+          for (uint32_t piece = 0; piece < 4; ++piece)
+            st_shared_v4(buf + stage_row + ((sub * 4 + piece) ^ sw) * 16,
+                         pack2<BF16>(__uint_as_float(r[piece * 8]), __uint_as_float(r[piece * 8 + 1])),
+                         pack2<BF16>(__uint_as_float(r[piece * 8 + 2]), __uint_as_float(r[piece * 8 + 3])),
+                         pack2<BF16>(__uint_as_float(r[piece * 8 + 4]), __uint_as_float(r[piece * 8 + 5])),
+                         pack2<BF16>(__uint_as_float(r[piece * 8 + 6]), __uint_as_float(r[piece * 8 + 7])));
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::tma_store_3d(&tmap_c, n0 + c, row0, e, buf);
+          ptx::tma_store_commit();
+        }
+      }
+      if (!empty) {
+        release_accumulator(ctrl, acc.at, leader, lane);
+        acc.next(2);
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait_all<0>();
+    if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortEpilogue);
+  }
+  tear_down_pair(ctrl, tmem_base, warp);
 }
 
 // ----------------------------------------------------------------------- rows in and out of order
 
 // out[pos[t, s]] = in[t] for every slot: a 16-byte piece of a token is read once and stored top_k
-// times.  The blocks from `copy_blocks` on (where there are any) clear an expert's rows from its
-// last to the next multiple of 64 each, which products over K = rows read.
+// times.  The blocks from `copy_blocks` on (where there are any) clear an expert's padding rows each,
+// which products over K = rows read.
 __global__ void __launch_bounds__(256) permute_kernel(const Plan plan, const uint4* in, long long ld_in, uint4* out,
                                                       int tokens, int top_k, int vectors, int copy_blocks) {
   dependency_wait();
@@ -872,7 +961,7 @@ __global__ void __launch_bounds__(256) permute_kernel(const Plan plan, const uin
     const int e = blockIdx.x - copy_blocks;
     const int count = plan.count[e];
     const long long first = static_cast<long long>(plan.start[e] + count) * vectors;
-    const int clear = ((count + kTileK - 1) / kTileK * kTileK - count) * vectors;
+    const int clear = ((count + kPad - 1) / kPad * kPad - count) * vectors;
     for (int i = threadIdx.x; i < clear; i += 256) out[first + i] = make_uint4(0, 0, 0, 0);
     return;
   }
@@ -888,10 +977,12 @@ __global__ void __launch_bounds__(256) permute_kernel(const Plan plan, const uin
   }
 }
 
-// out[t] = sum over slots of part[pos[t, s]], in slot order; slots without an expert add nothing.
+// out[t] = sum over slots and slices of part[slice][pos[t, s]], in order; slots without an expert
+// add nothing.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const float* part, const int* pos, T* out, long long ld_out,
-                                                      int tokens, int top_k, int cols) {
+                                                      int tokens, int top_k, int cols, int splits,
+                                                      long long slice) {
   dependency_wait();
   dependency_release();
   const int vectors = cols >> 3;
@@ -904,18 +995,20 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, const i
     for (int s = 0; s < top_k; ++s) {
       const int row = pos[static_cast<long long>(t) * top_k + s];
       if (row < 0) continue;
-      float v[8];
-      elem::load<float, 8>(part + static_cast<long long>(row) * cols + c, v);
+      for (int q = 0; q < splits; ++q) {
+        float v[8];
+        elem::load<float, 8>(part + q * slice + static_cast<long long>(row) * cols + c, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        for (int j = 0; j < 8; ++j) sum[j] += v[j];
+      }
     }
     elem::store<T, 8>(out + t * ld_out + c, sum);
   }
 }
 
-// dweights[pair] = sum over column tiles of the pair's row, in order.
+// dweights[pair] = sum over the parts of the pair's row, in order.
 __global__ void __launch_bounds__(256) weight_grad_kernel(const float* dw_part, const int* pos, float* dweights,
-                                                          int pairs, int tiles_n) {
+                                                          int pairs, int parts) {
   dependency_wait();
   dependency_release();
   const int i = blockIdx.x * 256 + threadIdx.x;
@@ -923,7 +1016,7 @@ __global__ void __launch_bounds__(256) weight_grad_kernel(const float* dw_part, 
   const int row = pos[i];
   float sum = 0.f;
   if (row >= 0)
-    for (int c = 0; c < tiles_n; ++c) sum += dw_part[static_cast<long long>(row) * tiles_n + c];
+    for (int c = 0; c < parts; ++c) sum += dw_part[static_cast<long long>(row) * parts + c];
   dweights[i] = sum;
 }
 
@@ -934,12 +1027,14 @@ inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Sizes and offsets of one problem.
 struct Layout {
-  int cta_group, tile_rows, pairs, max_tiles;
+  int pairs, max_tiles;
   int64_t max_rows;
   int chunk, chunks;
-  // forward: everything in `saved` when training (and the rest in the workspace)
-  int64_t off_tiles, off_count, off_start, off_tile_expert, off_row_token, off_row_weight, off_pos, plan_bytes;
-  bool gather;         // the copy engine picks the rows of x
+  bool gather;                 // the copy engine picks the rows of x
+  int down_splits, dx_splits;  // slices of K of the two products with fp32 rows
+  int dw_parts;
+  // The plan, the hidden activation and the gate/up products: in `saved` when training.
+  int64_t off_tiles, off_count, off_start, off_tile, off_row_token, off_row_weight, off_pos, plan_bytes;
   int64_t hidden_bytes, gu_bytes, part_bytes, chunk_bytes, x_bytes;
   int64_t dgu_bytes, dx_bytes, dw_bytes, dy_bytes;
 };
@@ -976,26 +1071,44 @@ int moe_check(const tnx_moe_problem* p) {
     set_error("pitches of rows and of experts must cover them and be multiples of 8 elements (16 bytes)");
     return TNX_ERR_INVALID;
   }
-  // (tile numbers are 32-bit; the smallest tiles are 128 rows x 128 columns)
-  const int64_t row_tiles = static_cast<int64_t>(p->tokens) * p->top_k / kRows + p->experts;
-  const int64_t widest = p->d_model > 2 * p->d_ff ? p->d_model : 2 * p->d_ff;
-  const int64_t weight_tiles = static_cast<int64_t>(p->experts) * (widest / 128 + 1);
-  if ((row_tiles > weight_tiles ? row_tiles : weight_tiles) * ((widest > p->n_out ? widest : p->n_out) / 128 + 1) >
-      (1 << 30)) {
+  // (tile numbers are 32-bit, with up to eight slices of K per tile)
+  const int64_t row_tiles = static_cast<int64_t>(p->tokens) * p->top_k / kTileN + p->experts;
+  int64_t widest = p->d_model > 2 * p->d_ff ? p->d_model : 2 * p->d_ff;
+  if (widest < p->n_out) widest = p->n_out;
+  const int64_t col_tiles = widest / 256 + 1, weight_tiles = p->experts * col_tiles;
+  if ((row_tiles > weight_tiles ? row_tiles : weight_tiles) * col_tiles > (1 << 27)) {
     set_error("problem has too many tiles");
     return TNX_ERR_INVALID;
   }
   return TNX_OK;
 }
 
+// Slices of K for a product with `cols` output columns over num_kb K blocks: the number that takes
+// the least time when a K block costs 0.3 us, a tile 2 us of its own, and each slice writes and
+// reads its copy of the rows at 6 TB/s.  With few tiles this fills the last wave (8 experts of
+// 4096/14336, 500 tokens: 128 tiles for 74 pairs of SMs).
+int pick_splits(const Layout& l, int cols, int num_kb) {
+  const int clusters = sm_count() / 2;
+  const double units = static_cast<double>(l.max_tiles) * cdiv(cols, 2 * kRows);
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 8 && num_kb / s >= 4; s *= 2) {
+    const int waves = static_cast<int>((units * s + clusters - 1) / clusters);
+    const double us = waves * (0.3 * cdiv(num_kb, s) + 2.0) + s * (8.0 * l.pairs * cols / 6.0e6);
+    if (s == 1 || us < 0.95 * least) {
+      best = s;
+      least = us;
+    }
+  }
+  return best;
+}
+
 Layout lay_out_problem(const tnx_moe_problem& p) {
   Layout l = {};
   l.pairs = p.tokens * p.top_k;
-  // Pairs of CTAs (256-row tiles) halve the weight traffic per row but pad an expert to 256 rows.
-  l.cta_group = l.pairs / p.experts >= 384 ? 2 : 1;
-  l.tile_rows = kRows * l.cta_group;
-  l.max_tiles = l.pairs / l.tile_rows + (l.pairs < p.experts ? l.pairs : p.experts);
-  l.max_rows = static_cast<int64_t>(l.max_tiles) * l.tile_rows;
+  const int hit = l.pairs < p.experts ? l.pairs : p.experts;  // experts with rows at most
+  l.max_tiles = (l.pairs - hit) / kTileN + hit;
+  l.max_rows = (static_cast<int64_t>(l.pairs) + static_cast<int64_t>(hit) * (kPad - 1)) / kPad * kPad;
   if (l.pairs <= kSmallPairs) {
     l.chunk = cdiv(cdiv(l.pairs, kSmallWarps), 32) * 32;
     l.chunks = kSmallWarps;
@@ -1013,21 +1126,24 @@ Layout lay_out_problem(const tnx_moe_problem& p) {
   l.off_tiles = take(4);
   l.off_count = take(4ll * p.experts);
   l.off_start = take(4ll * p.experts);
-  l.off_tile_expert = take(4ll * l.max_tiles);
+  l.off_tile = take(16ll * l.max_tiles);
   l.off_row_token = take(4 * l.max_rows);
   l.off_row_weight = take(4 * l.max_rows);
   l.off_pos = take(4ll * l.pairs);
   l.plan_bytes = at;
   // (a training step needs the rows in order for the weights' gradients anyway)
   l.gather = !p.train && l.pairs / p.experts <= 32;
+  l.down_splits = pick_splits(l, p.n_out, cdiv(p.d_ff, kTileK));
+  l.dx_splits = pick_splits(l, p.d_model, cdiv(2 * p.d_ff, kTileK));
+  l.dw_parts = cdiv(p.d_ff, 32);
   l.x_bytes = l.gather ? 0 : align256(l.max_rows * p.d_model * 2);
   l.dy_bytes = align256(l.max_rows * p.n_out * 2);
   l.hidden_bytes = align256(l.max_rows * p.d_ff * 2);
   l.gu_bytes = align256(l.max_rows * p.d_ff * 8);
-  l.part_bytes = align256(l.max_rows * p.n_out * 4);
+  l.part_bytes = align256(l.down_splits * l.max_rows * p.n_out * 4);
   l.dgu_bytes = align256(l.max_rows * p.d_ff * 4);
-  l.dx_bytes = align256(l.max_rows * p.d_model * 4);
-  l.dw_bytes = align256(l.max_rows * cdiv(p.d_ff, tile_n(kDHidden, l.cta_group)) * 4);
+  l.dx_bytes = align256(l.dx_splits * l.max_rows * p.d_model * 4);
+  l.dw_bytes = align256(l.max_rows * l.dw_parts * 4);
   return l;
 }
 
@@ -1037,7 +1153,7 @@ Plan plan_at(const Layout& l, void* base) {
   q.tiles = reinterpret_cast<int*>(b + l.off_tiles);
   q.count = reinterpret_cast<int*>(b + l.off_count);
   q.start = reinterpret_cast<int*>(b + l.off_start);
-  q.tile_expert = reinterpret_cast<int*>(b + l.off_tile_expert);
+  q.tile = reinterpret_cast<int4*>(b + l.off_tile);
   q.row_token = reinterpret_cast<int*>(b + l.off_row_token);
   q.row_weight = reinterpret_cast<float*>(b + l.off_row_weight);
   q.pos = reinterpret_cast<int*>(b + l.off_pos);
@@ -1094,31 +1210,74 @@ int launch(const char* what, void (*fn)(KArgs...), int grid, int block, int smem
   return e == cudaSuccess ? TNX_OK : cuda_failed(what, e);
 }
 
-template <int MODE, int CTA_GROUP>
-int launch_gemm(int dtype, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const CUtensorMap& gu,
-                GemmParams p, int64_t units, cudaStream_t stream) {
-  constexpr int n = tile_n(MODE, CTA_GROUP);
-  constexpr int stage_bytes = (kRows + n / CTA_GROUP) * kTileK * 2;
-  constexpr int fixed = staging_boxes(MODE) * kBoxBytes + kCtrlBytes + kAlignSlack;
-  constexpr int fit = (kMaxDynamicSmem - fixed) / stage_bytes;
-  constexpr int stages = fit > kMaxStages ? kMaxStages : fit;
-  static_assert(stages >= 3, "too little shared memory for the ring");
-  p.stages = stages;
-  p.tile_rows = kRows * CTA_GROUP;
-  auto fn = dtype == TNX_BF16 ? moe_gemm_kernel<MODE, CTA_GROUP, true> : moe_gemm_kernel<MODE, CTA_GROUP, false>;
-  const int smem = stages * stage_bytes + fixed;
+// One pair of CTAs per pair of SMs, or per unit where there are fewer.
+template <typename Fn, typename Params, typename... Maps>
+int launch_pairs(Fn fn, int threads, Params p, int staging_bytes, int64_t units, cudaStream_t stream,
+                 const Maps&... maps) {
+  const int fixed = staging_bytes + kCtrlBytes + kAlignSlack;
+  const int fit = (kMaxDynamicSmem - fixed) / kStageBytes;
+  p.stages = fit > kMaxStages ? kMaxStages : fit;
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kMaxDynamicSmem);
   if (e != cudaSuccess) return cuda_failed("experts' products: shared memory", e);
-  const int most = sm_count() / CTA_GROUP;
+  const int most = sm_count() / 2;
   const int clusters = units < most ? static_cast<int>(units) : most;
-  if (clusters < 1) return TNX_OK;
-  return launch("experts' products", fn, clusters * CTA_GROUP, kThreads, smem, CTA_GROUP, stream, a, b, c, gu, p);
+  return launch("experts' products", fn, clusters * 2, threads, p.stages * kStageBytes + fixed, 2, stream, maps..., p);
+}
+// Tensor maps over rows in expert order, as moe_rows_kernel reads them.
+struct RowsMaps {
+  CUtensorMap r128, r64, r16;
+};
+int rows_maps(RowsMaps* m, const void* rows, int dtype, int cols, int64_t max_rows) {
+  int rc = make_tmap_2d(&m->r128, rows, dtype, cols, max_rows, cols, 64, 128, true);
+  if (rc == TNX_OK) rc = make_tmap_2d(&m->r64, rows, dtype, cols, max_rows, cols, 64, 64, true);
+  if (rc == TNX_OK) rc = make_tmap_2d(&m->r16, rows, dtype, cols, max_rows, cols, 64, 16, true);
+  return rc;
+}
+// A map over the weights [experts][rows][cols] with K down their rows.
+int weights_map(CUtensorMap* w, RowsParams* g, const tnx_moe_problem& p, const void* ptr, int cols, int rows,
+                int64_t row_pitch, int64_t expert_pitch) {
+  g->panels = cols % 64 == 0;
+  return g->panels ? make_tmap_panels(w, ptr, p.dtype, cols, rows, p.experts, row_pitch, expert_pitch, kTileK)
+                   : make_tmap_3d(w, ptr, p.dtype, cols, rows, p.experts, row_pitch, expert_pitch, 64, kTileK, true);
 }
 template <int MODE>
-int launch_gemm(const Layout& l, int dtype, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
-                const CUtensorMap& gu, const GemmParams& p, int64_t units, cudaStream_t stream) {
-  return l.cta_group == 2 ? launch_gemm<MODE, 2>(dtype, a, b, c, gu, p, units, stream)
-                          : launch_gemm<MODE, 1>(dtype, a, b, c, gu, p, units, stream);
+int launch_rows(const tnx_moe_problem& q, const Layout& l, const CUtensorMap& w, const RowsMaps& r, RowsParams p,
+                cudaStream_t stream) {
+  p.tiles_n = cdiv(p.cols, 2 * kRows);
+  p.max_rows = l.max_rows;
+  const int64_t units = static_cast<int64_t>(l.max_tiles) * p.tiles_n * p.splits;
+  return q.dtype == TNX_BF16
+             ? launch_pairs(moe_rows_kernel<MODE, true>, kRowsThreads, p, 0, units, stream, w, r.r128, r.r64, r.r16)
+             : launch_pairs(moe_rows_kernel<MODE, false>, kRowsThreads, p, 0, units, stream, w, r.r128, r.r64, r.r16);
+}
+// out[e] = a[rows of e]^T b[rows of e], m x n.
+int run_wgrad(const tnx_moe_problem& q, const Layout& l, const Plan& plan, const void* a, int m, const void* b, int n,
+              void* out, int32_t* status, cudaStream_t stream) {
+  WgradParams p = {};
+  p.plan = plan;
+  p.experts = q.experts;
+  p.m = m;
+  p.n = n;
+  p.tiles_m = cdiv(m, 2 * kRows);
+  p.tiles_n = cdiv(n, kTileN);
+  p.status = status;
+  p.timeout_ns = bounded_wait_limit_ns();
+  CUtensorMap ta, tb, tc;
+  p.panels_a = m % 64 == 0;
+  p.panels_b = n % 64 == 0;
+  auto operand = [&](CUtensorMap* map, const void* ptr, int cols, int panels) {
+    return panels ? make_tmap_panels(map, ptr, q.dtype, cols, l.max_rows, 1, cols, l.max_rows * cols, kTileK)
+                  : make_tmap_2d(map, ptr, q.dtype, cols, l.max_rows, cols, 64, kTileK, true);
+  };
+  int rc = operand(&ta, a, m, p.panels_a);
+  if (rc == TNX_OK) rc = operand(&tb, b, n, p.panels_b);
+  if (rc == TNX_OK)
+    rc = make_tmap_3d(&tc, out, q.dtype, n, m, q.experts, n, static_cast<int64_t>(m) * n, 64, 32, false);
+  if (rc != TNX_OK) return rc;
+  const int64_t units = static_cast<int64_t>(q.experts) * p.tiles_m * p.tiles_n;
+  const int staging = 4 * kBoxes * kBoxBytes;
+  return q.dtype == TNX_BF16 ? launch_pairs(moe_wgrad_kernel<true>, kThreads, p, staging, units, stream, ta, tb, tc)
+                             : launch_pairs(moe_wgrad_kernel<false>, kThreads, p, staging, units, stream, ta, tb, tc);
 }
 
 int run_plan(const tnx_moe_problem& p, const Layout& l, const Plan& plan, const void* ids, const float* weights,
@@ -1131,7 +1290,6 @@ int run_plan(const tnx_moe_problem& p, const Layout& l, const Plan& plan, const 
   q.experts = p.experts;
   q.top_k = p.top_k;
   q.pairs = l.pairs;
-  q.tile_rows = l.tile_rows;
   q.chunk = l.chunk;
   q.chunks = l.chunks;
   q.chunk_counts = static_cast<int*>(scratch);
@@ -1161,26 +1319,33 @@ int run_permute(const tnx_moe_problem& p, const Plan& plan, const void* in, int6
 }
 
 int run_combine(int dtype, const float* part, const int* pos, void* out, int64_t ld_out, int tokens, int top_k,
-                int cols, cudaStream_t stream) {
+                int cols, int splits, int64_t max_rows, cudaStream_t stream) {
+  const long long slice = max_rows * cols;
   const int64_t blocks = (static_cast<int64_t>(tokens) * (cols / 8) + 255) / 256;
   const int most = 16 * sm_count();
   const int grid = blocks < most ? static_cast<int>(blocks) : most;
   if (dtype == TNX_BF16)
     return launch("combining experts", combine_kernel<__nv_bfloat16>, grid, 256, 0, 1, stream, part, pos,
-                  static_cast<__nv_bfloat16*>(out), static_cast<long long>(ld_out), tokens, top_k, cols);
+                  static_cast<__nv_bfloat16*>(out), static_cast<long long>(ld_out), tokens, top_k, cols, splits, slice);
   return launch("combining experts", combine_kernel<__half>, grid, 256, 0, 1, stream, part, pos,
-                static_cast<__half*>(out), static_cast<long long>(ld_out), tokens, top_k, cols);
+                static_cast<__half*>(out), static_cast<long long>(ld_out), tokens, top_k, cols, splits, slice);
 }
 
-GemmParams gemm_params(const tnx_moe_problem& p, const Plan& plan, int32_t* status) {
-  GemmParams g = {};
+RowsParams rows_params(const tnx_moe_problem& p, const Plan& plan, int32_t* status) {
+  RowsParams g = {};
   g.plan = plan;
-  g.experts = p.experts;
   g.activation = p.activation;
+  g.train = p.train;
   g.band = 8;
   g.status = status;
   g.timeout_ns = bounded_wait_limit_ns();
   return g;
+}
+// Cuts K into `splits` slices, none of them empty.
+void split_k(RowsParams* g, int num_kb, int splits) {
+  g->num_kb = num_kb;
+  g->kb_per_split = cdiv(num_kb, splits);
+  g->splits = cdiv(num_kb, g->kb_per_split);
 }
 
 bool misaligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) != 0; }
@@ -1200,7 +1365,7 @@ int tnx_moe_query(const tnx_moe_problem* problem, tnx_moe_resources* out) {
   const int rc = moe_check(problem);
   if (rc != TNX_OK) return rc;
   const Layout l = lay_out_problem(*problem);
-  out->tile_rows = l.tile_rows;
+  out->tile_rows = kTileN;
   out->max_tiles = l.max_tiles;
   const int64_t keep = l.plan_bytes + l.hidden_bytes;
   out->saved_bytes = keep + l.gu_bytes;
@@ -1249,39 +1414,33 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   if (rc != TNX_OK) return rc;
 
   // H = w * act(x W1) * (x W2)
-  GemmParams g = gemm_params(p, plan, status_word);
-  g.num_kb = cdiv(p.d_model, kTileK);
+  RowsParams g = rows_params(p, plan, status_word);
+  split_k(&g, cdiv(p.d_model, kTileK), 1);
   g.cols = 2 * p.d_ff;
-  g.tiles_n = cdiv(g.cols, 256);
-  g.save_gu = p.train;
-  CUtensorMap ta, tb, tc, tgu;
-  rc = l.gather ? make_tmap_2d(&ta, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true)
-                : make_tmap_2d(&ta, xp, p.dtype, p.d_model, l.max_rows, p.d_model, 64, 32, true);
-  if (rc == TNX_OK)
-    rc = make_tmap_3d(&tb, w12, p.dtype, 2ll * p.d_ff, p.d_model, p.experts, p.stride_w12k, p.stride_w12e, 64, kTileK, true);
-  if (rc == TNX_OK) rc = make_tmap_2d(&tc, hidden, p.dtype, p.d_ff, l.max_rows, p.d_ff, 64, kRows, false);
-  tgu = tc;
-  if (rc == TNX_OK && p.train)
-    rc = make_tmap_2d(&tgu, gu, TNX_F32, 2ll * p.d_ff, l.max_rows, 2ll * p.d_ff, 32, kRows, false);
+  g.out = hidden;
+  g.gu = static_cast<float*>(gu);
+  CUtensorMap tw;
+  RowsMaps rows;
+  rc = weights_map(&tw, &g, p, w12, 2 * p.d_ff, p.d_model, p.stride_w12k, p.stride_w12e);
+  if (rc == TNX_OK && l.gather) {
+    rc = make_tmap_2d(&rows.r16, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true);
+    rows.r128 = rows.r64 = rows.r16;
+  } else if (rc == TNX_OK) {
+    rc = rows_maps(&rows, xp, p.dtype, p.d_model, l.max_rows);
+  }
   if (rc != TNX_OK) return rc;
-  const int64_t units = static_cast<int64_t>(l.max_tiles) * g.tiles_n;
-  rc = l.gather ? launch_gemm<kGateUpGather>(l, p.dtype, ta, tb, tc, tgu, g, units, s)
-                : launch_gemm<kGateUp>(l, p.dtype, ta, tb, tc, tgu, g, units, s);
+  rc = l.gather ? launch_rows<kGateUpGather>(p, l, tw, rows, g, s) : launch_rows<kGateUp>(p, l, tw, rows, g, s);
   if (rc != TNX_OK) return rc;
 
   // O = H W3
-  g.num_kb = cdiv(p.d_ff, kTileK);
+  split_k(&g, cdiv(p.d_ff, kTileK), l.down_splits);
   g.cols = p.n_out;
-  g.tiles_n = cdiv(g.cols, 256);
-  g.part = part;
-  rc = make_tmap_2d(&ta, hidden, p.dtype, p.d_ff, l.max_rows, p.d_ff, 64, 32, true);
-  if (rc == TNX_OK)
-    rc = make_tmap_3d(&tb, w3, p.dtype, p.n_out, p.d_ff, p.experts, p.stride_w3k, p.stride_w3e, 64, kTileK, true);
-  if (rc == TNX_OK) rc = make_tmap_2d(&tc, part, TNX_F32, p.n_out, l.max_rows, p.n_out, 32, kRows, false);
+  g.out = part;
+  rc = weights_map(&tw, &g, p, w3, p.n_out, p.d_ff, p.stride_w3k, p.stride_w3e);
+  if (rc == TNX_OK) rc = rows_maps(&rows, hidden, p.dtype, p.d_ff, l.max_rows);
+  if (rc == TNX_OK) rc = launch_rows<kDown>(p, l, tw, rows, g, s);
   if (rc != TNX_OK) return rc;
-  rc = launch_gemm<kDown>(l, p.dtype, ta, tb, tc, tc, g, static_cast<int64_t>(l.max_tiles) * g.tiles_n, s);
-  if (rc != TNX_OK) return rc;
-  return run_combine(p.dtype, part, plan.pos, y, p.stride_y, p.tokens, p.top_k, p.n_out, s);
+  return run_combine(p.dtype, part, plan.pos, y, p.stride_y, p.tokens, p.top_k, p.n_out, g.splits, l.max_rows, s);
 }
 
 int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int64_t stride_dy, const void* x,
@@ -1320,7 +1479,7 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
   char* keep = static_cast<char*>(const_cast<void*>(saved));
   const Plan plan = plan_at(l, keep);
   void* hidden = keep + l.plan_bytes;
-  void* gu = keep + l.plan_bytes + l.hidden_bytes;
+  float* gu = reinterpret_cast<float*>(keep + l.plan_bytes + l.hidden_bytes);
   char* ws = static_cast<char*>(workspace);
   void* dgu = ws;
   float* dx_part = reinterpret_cast<float*>(ws + l.dgu_bytes);
@@ -1333,74 +1492,41 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
   if (rc == TNX_OK && dw12 != nullptr) rc = run_permute(p, plan, x, p.stride_x, xp, p.d_model, true, s);
   if (rc != TNX_OK) return rc;
 
-  // dH = dy W3^T; dGU and the routing weights' gradient from it
-  GemmParams g = gemm_params(p, plan, status_word);
-  CUtensorMap ta, tb, tc, tgu;
+  // dH = dY W3^T; dGU and the routing weights' gradient from it
+  RowsParams g = rows_params(p, plan, status_word);
+  CUtensorMap tw;
+  RowsMaps rows;
   if (hidden_grad) {
-    const int n = tile_n(kDHidden, l.cta_group);
-    g.num_kb = cdiv(p.n_out, kTileK);
+    split_k(&g, cdiv(p.n_out, kTileK), 1);
     g.cols = p.d_ff;
-    g.tiles_n = cdiv(g.cols, n);
+    g.out = dgu;
+    g.gu = gu;
     g.dw_part = dw_part;
-    rc = make_tmap_2d(&ta, dyp, p.dtype, p.n_out, l.max_rows, p.n_out, 64, 32, true);
-    if (rc == TNX_OK)
-      rc = make_tmap_3d(&tb, w3, p.dtype, p.n_out, p.d_ff, p.experts, p.stride_w3k, p.stride_w3e, 64,
-                        n / l.cta_group, true);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tc, dgu, p.dtype, two_f, l.max_rows, two_f, 64, kRows, false);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tgu, gu, TNX_F32, two_f, l.max_rows, two_f, 32, kRows, true);
-    if (rc != TNX_OK) return rc;
-    rc = launch_gemm<kDHidden>(l, p.dtype, ta, tb, tc, tgu, g, static_cast<int64_t>(l.max_tiles) * g.tiles_n, s);
-    if (rc != TNX_OK) return rc;
-    if (dweights != nullptr) {
+    g.dw_parts = l.dw_parts;
+    g.train = 1;  // (the padding rows of dGU are zeros: products over K = rows read them)
+    rc = make_tmap_3d(&tw, w3, p.dtype, p.n_out, p.d_ff, p.experts, p.stride_w3k, p.stride_w3e, 64, kRows, true);
+    if (rc == TNX_OK) rc = rows_maps(&rows, dyp, p.dtype, p.n_out, l.max_rows);
+    if (rc == TNX_OK) rc = launch_rows<kDHidden>(p, l, tw, rows, g, s);
+    if (rc == TNX_OK && dweights != nullptr)
       rc = launch("routing weights' gradient", weight_grad_kernel, cdiv(l.pairs, 256), 256, 0, 1, s,
-                  static_cast<const float*>(dw_part), static_cast<const int*>(plan.pos), dweights, l.pairs, g.tiles_n);
-      if (rc != TNX_OK) return rc;
-    }
+                  static_cast<const float*>(dw_part), static_cast<const int*>(plan.pos), dweights, l.pairs, l.dw_parts);
+    if (rc != TNX_OK) return rc;
   }
   if (dx != nullptr) {
-    g.num_kb = cdiv(static_cast<int>(two_f), kTileK);
+    split_k(&g, cdiv(static_cast<int>(two_f), kTileK), l.dx_splits);
     g.cols = p.d_model;
-    g.tiles_n = cdiv(g.cols, 256);
-    g.part = dx_part;
-    rc = make_tmap_2d(&ta, dgu, p.dtype, two_f, l.max_rows, two_f, 64, 32, true);
+    g.out = dx_part;
+    rc = make_tmap_3d(&tw, w12, p.dtype, two_f, p.d_model, p.experts, p.stride_w12k, p.stride_w12e, 64, kRows, true);
+    if (rc == TNX_OK) rc = rows_maps(&rows, dgu, p.dtype, static_cast<int>(two_f), l.max_rows);
+    if (rc == TNX_OK) rc = launch_rows<kDX>(p, l, tw, rows, g, s);
     if (rc == TNX_OK)
-      rc = make_tmap_3d(&tb, w12, p.dtype, two_f, p.d_model, p.experts, p.stride_w12k, p.stride_w12e, 64,
-                        256 / l.cta_group, true);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tc, dx_part, TNX_F32, p.d_model, l.max_rows, p.d_model, 32, kRows, false);
-    if (rc != TNX_OK) return rc;
-    rc = launch_gemm<kDX>(l, p.dtype, ta, tb, tc, tc, g, static_cast<int64_t>(l.max_tiles) * g.tiles_n, s);
-    if (rc == TNX_OK)
-      rc = run_combine(p.dtype, dx_part, plan.pos, dx, p.d_model, p.tokens, p.top_k, p.d_model, s);
+      rc = run_combine(p.dtype, dx_part, plan.pos, dx, p.d_model, p.tokens, p.top_k, p.d_model, g.splits, l.max_rows, s);
     if (rc != TNX_OK) return rc;
   }
-  if (dw12 != nullptr) {
-    g.m = p.d_model;
-    g.tiles_m = cdiv(p.d_model, l.tile_rows);
-    g.cols = static_cast<int>(two_f);
-    g.tiles_n = cdiv(g.cols, 256);
-    rc = make_tmap_2d(&ta, xp, p.dtype, p.d_model, l.max_rows, p.d_model, 64, kTileK, true);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tb, dgu, p.dtype, two_f, l.max_rows, two_f, 64, kTileK, true);
-    if (rc == TNX_OK)
-      rc = make_tmap_3d(&tc, dw12, p.dtype, two_f, p.d_model, p.experts, two_f, two_f * p.d_model, 64, kRows, false);
-    if (rc != TNX_OK) return rc;
-    rc = launch_gemm<kDW12>(l, p.dtype, ta, tb, tc, tc, g, static_cast<int64_t>(p.experts) * g.tiles_m * g.tiles_n, s);
-    if (rc != TNX_OK) return rc;
-  }
-  if (dw3 != nullptr) {
-    g.m = p.d_ff;
-    g.tiles_m = cdiv(p.d_ff, l.tile_rows);
-    g.cols = p.n_out;
-    g.tiles_n = cdiv(g.cols, 256);
-    rc = make_tmap_2d(&ta, hidden, p.dtype, p.d_ff, l.max_rows, p.d_ff, 64, kTileK, true);
-    if (rc == TNX_OK) rc = make_tmap_2d(&tb, dyp, p.dtype, p.n_out, l.max_rows, p.n_out, 64, kTileK, true);
-    if (rc == TNX_OK)
-      rc = make_tmap_3d(&tc, dw3, p.dtype, p.n_out, p.d_ff, p.experts, p.n_out, static_cast<int64_t>(p.n_out) * p.d_ff,
-                        64, kRows, false);
-    if (rc != TNX_OK) return rc;
-    rc = launch_gemm<kDW3>(l, p.dtype, ta, tb, tc, tc, g, static_cast<int64_t>(p.experts) * g.tiles_m * g.tiles_n, s);
-    if (rc != TNX_OK) return rc;
-  }
-  return TNX_OK;
+  if (dw12 != nullptr)
+    rc = run_wgrad(p, l, plan, xp, p.d_model, dgu, static_cast<int>(two_f), dw12, status_word, s);
+  if (rc == TNX_OK && dw3 != nullptr) rc = run_wgrad(p, l, plan, hidden, p.d_ff, dyp, p.n_out, dw3, status_word, s);
+  return rc;
 }
 
 }  // extern "C"

@@ -1130,10 +1130,12 @@ struct TmapKey {
   int64_t cols, rows, pitch;
   int32_t dtype, box_cols, box_rows, is_operand;
   int64_t depth, matrix_pitch;  // 3-D maps; 0 for 2-D ones
+  int32_t panels;               // 1: 64-column panels as a dimension of their own
   bool operator==(const TmapKey& o) const {
     return ptr == o.ptr && cols == o.cols && rows == o.rows && pitch == o.pitch &&
            dtype == o.dtype && box_cols == o.box_cols && box_rows == o.box_rows &&
-           is_operand == o.is_operand && depth == o.depth && matrix_pitch == o.matrix_pitch;
+           is_operand == o.is_operand && depth == o.depth && matrix_pitch == o.matrix_pitch &&
+           panels == o.panels;
   }
 };
 struct TmapSlot {
@@ -1155,8 +1157,9 @@ inline unsigned tmap_hash(const TmapKey& k) {
 
 int make_tmap(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows,
               int64_t pitch_elems, int box_cols, int box_rows, bool is_operand, int64_t depth = 0,
-              int64_t matrix_pitch = 0) {
-  const TmapKey key{ptr, cols, rows, pitch_elems, dtype, box_cols, box_rows, is_operand ? 1 : 0, depth, matrix_pitch};
+              int64_t matrix_pitch = 0, bool panels = false) {
+  const TmapKey key{ptr,   cols, rows, pitch_elems, dtype, box_cols, box_rows, is_operand ? 1 : 0, depth, matrix_pitch,
+                    panels ? 1 : 0};
   const unsigned slot = tmap_hash(key);
   {
     std::lock_guard<std::mutex> lock(g_tmap_mu);
@@ -1174,18 +1177,25 @@ int make_tmap(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_
   // call yet (the one autograd runs a backward pass on) gets its device's by selecting it.
   int dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) (void)cudaSetDevice(dev);
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
-                              static_cast<cuuint64_t>(depth)};
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(depth), 1};
   // (16-bit operands and outputs everywhere, except fp32 partial outputs)
   const cuuint64_t elem_bytes = dtype == TNX_F32 ? 4 : 2;
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch_elems) * elem_bytes,
-                                 static_cast<cuuint64_t>(matrix_pitch) * elem_bytes};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(pitch_elems) * elem_bytes,
+                           static_cast<cuuint64_t>(matrix_pitch) * elem_bytes, 0};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  if (panels) {
+    dims[0] = 64;
+    dims[2] = static_cast<cuuint64_t>(cols / 64);
+    dims[3] = static_cast<cuuint64_t>(depth);
+    strides[2] = strides[1];
+    strides[1] = 64 * elem_bytes;
+    box[2] = 2;
+  }
   const CUtensorMapDataType dt = dtype == TNX_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : dtype == TNX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = encode(out, dt, depth > 0 ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr,
+  CUresult r = encode(out, dt, panels ? 4 : depth > 0 ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr,
                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                       is_operand ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1342,6 +1352,10 @@ int make_tmap_2d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int
 int make_tmap_3d(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows, int64_t depth,
                  int64_t row_pitch, int64_t matrix_pitch, int box_cols, int box_rows, bool is_operand) {
   return make_tmap(out, ptr, dtype, cols, rows, row_pitch, box_cols, box_rows, is_operand, depth, matrix_pitch);
+}
+int make_tmap_panels(CUtensorMap* out, const void* ptr, int dtype, int64_t cols, int64_t rows, int64_t depth,
+                     int64_t row_pitch, int64_t matrix_pitch, int box_rows) {
+  return make_tmap(out, ptr, dtype, cols, rows, row_pitch, 64, box_rows, true, depth, matrix_pitch, true);
 }
 int sm_count() { return device_sm_count(); }
 unsigned long long bounded_wait_limit_ns() { return wait_limit_ns(); }
