@@ -84,6 +84,24 @@ def test_cta_pairs(t, n, k, d, f, n_out, dtype):
 @pytest.mark.parametrize("activation", ["silu", "sigmoid", "none"])
 def test_activations(activation):
     check(make(50, 4, 2, 128, 96, 64, bf16), activation)
+    check(make(1, 4, 2, 128, 96, 64, bf16), activation, train=False)
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16])
+@pytest.mark.parametrize("n,k,d,f,n_out", [(64, 8, 512, 264, 2056), (16, 8, 1032, 136, 72), (2, 1, 4104, 1048, 16),
+                                           (4, 8, 72, 40, 24), (300, 32, 64, 64, 64), (40, 33, 64, 64, 64)])
+def test_one_token(n, k, d, f, n_out, dtype):
+    ids = None if k <= n else torch.randint(0, n, (1, k), generator=torch.Generator().manual_seed(n))
+    check(make(1, n, k, d, f, n_out, dtype, seed=n, ids=ids), train=False)
+
+
+@pytest.mark.parametrize("ids", [[3, 3, 3], [-1, 5, 3], [0, 6, 2 ** 31 - 1], [-1, -1, -1]])
+def test_one_token_with_ids_out_of_range_and_repeated(ids):
+    for wide in (torch.int32, torch.int64):
+        case = make(1, 6, 3, 136, 72, 40, bf16, ids=torch.tensor([ids], dtype=wide))
+        check(case, train=False)
+        if max(ids) < 0:
+            assert not tnx.moe_swiglu(*operands(case)).any()
 
 
 def test_many_pairs_use_the_chunked_plan():

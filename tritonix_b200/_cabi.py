@@ -585,6 +585,19 @@ def call(device: torch.device, fn, *args) -> None:
         raise_for(rc)
 
 
+def signature(*tensors) -> tuple:
+    """Everything about the tensors that argument checks look at, hashable; an operator checks a
+    signature once and remembers what it found."""
+    return tuple([t if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+def remember(cache: dict, key, value):
+    if len(cache) > 4096:
+        cache.clear()
+    cache[key] = value
+    return value
+
+
 def rows_view(t: torch.Tensor) -> torch.Tensor:
     """``t`` (2-D) with adjacent elements in its rows and a pitch the kernels can walk: itself
     where that holds, a copy otherwise."""

@@ -50,7 +50,10 @@ constexpr int kMaxExperts = 512;
 constexpr int kRows = 128;       // rows of the M operand per CTA (TMEM lanes); a pair has 256
 constexpr int kTileN = 256;      // columns of the N operand per pair at most
 constexpr int kPad = 16;         // an expert's rows are padded to this: one MMA's K
-constexpr int kTileK = 64;       // K elements per ring slot: one 128-byte swizzle row
+constexpr int kTileK = 128;      // K elements per ring slot: two slabs of 64, a 128-byte swizzle row each.
+                                 // (Slots of 64 wait and commit twice as often: the library's GEMM
+                                 // loses 5-13 % with them at these sizes.)
+constexpr int kSlab = 64;
 constexpr int kThreads = 192;      // producer warp, MMA warp, four epilogue warps
 constexpr int kRowsEpilogue = 16;  // epilogue warps of the rows' kernel: four per quarter of the TMEM lanes
 constexpr int kRowsThreads = 64 + 32 * kRowsEpilogue;
@@ -79,8 +82,13 @@ struct Plan {
   int* pos;          // [pairs] row of a pair, -1 where its id is no expert
 };
 
+struct RowsMaps {
+  CUtensorMap m[4];
+};
+
 struct RowsParams {
   Plan plan;
+  int k;                             // K elements
   int num_kb, splits, kb_per_split;  // K blocks; slices of K, each with its own copy of O
   int cols;         // columns of the weight operand: 2 d_ff, n_out, d_ff or d_model
   int tiles_n;      // tiles of 256 of them
@@ -585,20 +593,22 @@ __device__ __forceinline__ void write_rows(const RowsParams& p, const Unit& un, 
 }
 
 // out^T[256 columns, n rows] = W^T rows^T for one expert's rows; see the top of the file.
-// tmap_w: the weights.  kGateUp, kDown: K runs down their rows, M along them: 64 x 64 boxes, two at
+// tmap_w: the weights.  kGateUp, kDown: K runs down their rows, M along them: 64 x 128 boxes, two at
 // a time where the columns are whole panels of 64 (p.panels); kDHidden, kDX: M down, K along: 64 x
-// 128 boxes.  tmap_r128, tmap_r64, tmap_r16: the rows, 64 elements by that many (kGateUpGather:
-// tmap_r16 is x itself, one row high).  A stage is kept to two or three copies: the copy engine
-// takes some 50 to 75 cycles for each whatever its size, against 512 for the stage's products.
+// 128 boxes, one per slab.  tmap_r: the rows, 64 elements by 128, 64, 32 and 16 rows, so that a copy
+// is made of exactly the rows a tile has (kGateUpGather: tmap_r.m[3] is x itself, one row high).
+// What bounds these products is the way from L2 to the SMs: 64 KB for 1024 cycles of a full stage's
+// MMAs is the 64 bytes per cycle an SM can take at most.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(kRowsThreads, 1)
-moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_r128,
-                const __grid_constant__ CUtensorMap tmap_r64, const __grid_constant__ CUtensorMap tmap_r16,
+moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ RowsMaps tmap_r,
                 const RowsParams p) {
   constexpr bool gate_up = MODE == kGateUp || MODE == kGateUpGather;
   constexpr bool gather = MODE == kGateUpGather;
   constexpr bool w_kmajor = MODE == kDHidden || MODE == kDX;
   constexpr int operand_bytes = kRows * kTileK * 2;
+  constexpr int kSlabBytes = kRows * kSlab * 2;       // K-major: 128 rows x 64 elements
+  constexpr int kAtom = kTileK * kAtomBytes;          // M-major: 64 columns x K rows
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
   const uint32_t smem_w = (raw_addr + 1023u) & ~1023u;
@@ -614,9 +624,7 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   volatile int* abort_flag = &ctrl->abort;
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tmap_w);
-    ptx::prefetch_tensormap(&tmap_r128);
-    ptx::prefetch_tensormap(&tmap_r64);
-    ptx::prefetch_tensormap(&tmap_r16);
+    for (int i = 0; i < 4; ++i) ptx::prefetch_tensormap(&tmap_r.m[i]);
   }
   const uint32_t tmem_base = set_up_pair(ctrl, p.stages, kRowsEpilogue, warp);
   // Everything above touches no global memory and may run under the tail of the kernel before.
@@ -634,9 +642,11 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       const int half = un.n >> 1;  // rows each CTA fetches
       const int row0 = un.row0 + rank * half;
       const int w_col = un.col0 + rank * kRows;
-      // one box of 128 or 64 rows, read a little past the tile's last row, or up to two of 16
-      const int box = gather ? half : half > 64 ? 128 : half > 32 ? 64 : half;
-      const uint32_t stage_tx = 2u * static_cast<uint32_t>(operand_bytes + box * kAtomBytes);
+      const int slab_bytes = half * kAtomBytes + (w_kmajor ? kSlabBytes : 0);
+      // lanes 0 to 3 copy 128, 64, 32 and 16 rows: the binary digits of `half`, largest first
+      const int size = 128 >> (lane & 3);
+      const bool copies = lane < 4 && (half & size) != 0;
+      const int from = half & ~(2 * size - 1);
       int rows[4] = {0, 0, 0, 0};
       if (gather) {
         // rows past the last are copies of that one: addressable, and never stored
@@ -651,25 +661,30 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           break;
         }
         const uint32_t full_bar = ptx::smem_u32(&ctrl->full[ring.at]);
-        if (leader && lane == 0) ptx::mbar_arrive_expect_tx(full_bar, stage_tx);
+        const int k0 = (un.kb0 + kb) * kTileK;
+        const int slabs = p.k - k0 > kSlab ? 2 : 1;  // (nothing reads the second slab of a short last block)
+        if (leader && lane == 0)
+          ptx::mbar_arrive_expect_tx(full_bar, 2u * static_cast<uint32_t>(slabs * slab_bytes + (w_kmajor ? 0 : operand_bytes)));
         const uint32_t bar = ptx::mapa(full_bar, 0);  // both CTAs' copies complete on the leader's barrier
         __syncwarp();
         const uint32_t w_dst = smem_w + ring.at * operand_bytes;
         const uint32_t r_dst = smem_r + ring.at * operand_bytes;
-        const int k0 = (un.kb0 + kb) * kTileK;
-        if (w_kmajor) {
-          if (lane == 31) ptx::tma_load_3d_pair(w_dst, &tmap_w, k0, w_col, un.expert, bar);
-        } else if (p.panels) {
+        if (!w_kmajor && p.panels) {
           if (lane == 31) ptx::tma_load_4d_pair(w_dst, &tmap_w, 0, k0, w_col >> 6, un.expert, bar);
-        } else if (lane >= 30) {
-          ptx::tma_load_3d_pair(w_dst + (lane - 30) * 8192, &tmap_w, w_col + (lane - 30) * 64, k0, un.expert, bar);
+        } else if (!w_kmajor && lane >= 30) {
+          const int half_w = lane - 30;
+          ptx::tma_load_3d_pair(w_dst + half_w * kAtom, &tmap_w, w_col + half_w * 64, k0, un.expert, bar);
         }
-        if (gather) {
-          if (4 * lane < half) tma_gather4_pair(r_dst + lane * 512, &tmap_r16, k0, rows, bar);
-        } else if (box >= 64) {
-          if (lane == 0) ptx::tma_load_2d_pair(r_dst, box == 64 ? &tmap_r64 : &tmap_r128, k0, row0, bar);
-        } else if (16 * lane < box) {
-          ptx::tma_load_2d_pair(r_dst + lane * 2048, &tmap_r16, k0, row0 + lane * 16, bar);
+        for (int slab = 0; slab < slabs; ++slab) {
+          const int k = k0 + slab * kSlab;
+          const uint32_t dst = r_dst + slab * kSlabBytes;
+          if (w_kmajor && lane == 31)
+            ptx::tma_load_3d_pair(w_dst + slab * kSlabBytes, &tmap_w, k, w_col, un.expert, bar);
+          if (gather) {
+            if (4 * lane < half) tma_gather4_pair(dst + lane * 512, &tmap_r.m[3], k, rows, bar);
+          } else if (copies) {
+            ptx::tma_load_2d_pair(dst + from * kAtomBytes, &tmap_r.m[lane], k, row0 + from, bar);
+          }
         }
         __syncwarp();
         ring.next(p.stages);
@@ -683,11 +698,11 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       // fp32 accumulate, M = 256 weight columns, N = the tile's rows (K-major)
       const uint32_t idesc_base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((w_kmajor ? 0u : 1u) << 15) |
                                   (static_cast<uint32_t>((kRows * 2) >> 4) << 24);
-      // K-major operands: rows of 128 bytes, 16 elements of K = 32 bytes further.  An M-major one:
-      // 64-wide atoms of 64 K rows x 128 bytes, 8192 bytes apart, 16 elements of K = 16 rows.
-      const uint64_t w_desc = w_kmajor ? ptx::make_smem_desc(0, 0, 1024) : ptx::make_smem_desc(0, 8192, 1024);
+      // K-major operands: slabs of 128 rows x 128 bytes, 16 elements of K = 32 bytes further.  An
+      // M-major one: 64-wide atoms of 128 K rows x 128 bytes, 16 elements of K = 16 rows.
+      const uint64_t w_desc =
+          w_kmajor ? ptx::make_smem_desc(0, 0, 1024) : ptx::make_smem_desc(0, kAtom, 1024);
       const uint64_t r_desc = ptx::make_smem_desc(0, 0, 1024);
-      constexpr uint32_t w_step16 = (w_kmajor ? 32u : 2048u) >> 4;
       Cursor ring, acc;
       bool ok = true;
       for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
@@ -708,10 +723,13 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           ptx::tc_fence_after_sync();
           const uint32_t w16 = (smem_w + ring.at * operand_bytes) >> 4;
           const uint32_t r16 = (smem_r + ring.at * operand_bytes) >> 4;
+          const int steps = (p.k - (un.kb0 + kb) * kTileK + 15) >> 4;
 #pragma unroll
           for (int k16 = 0; k16 < kTileK / 16; ++k16) {
-            ptx::umma_f16<2>(d_tmem, w_desc | ((w16 + k16 * w_step16) & 0x3fffu), r_desc | ((r16 + k16 * 2u) & 0x3fffu),
-                             idesc, accumulate);
+            const uint32_t kmajor = (k16 >> 2) * (kSlabBytes >> 4) + (k16 & 3) * 2u;
+            if (k16 < steps)
+              ptx::umma_f16<2>(d_tmem, w_desc | ((w16 + (w_kmajor ? kmajor : k16 * 128u)) & 0x3fffu),
+                               r_desc | ((r16 + kmajor) & 0x3fffu), idesc, accumulate);
             accumulate = 1;
           }
           ptx::umma_commit_pair(ptx::smem_u32(&ctrl->empty[ring.at]), 0x3);
@@ -770,9 +788,9 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   tear_down_pair(ctrl, tmem_base, warp);
 }
 
-// out[e] (m x n) = A[rows of e]^T B[rows of e]: tmap_a and tmap_b are 64 x 64 boxes over matrices of
+// out[e] (m x n) = A[rows of e]^T B[rows of e]: tmap_a and tmap_b are 64 x 128 boxes over matrices of
 // rows in expert order, tmap_c 64 x 32 boxes over the gradients.  An expert's last K block ends at
-// the padding (zeros in both operands): one to four MMAs of 16 rows.
+// the padding (zeros in both operands): one to eight MMAs of 16 rows.
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 moe_wgrad_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -826,12 +844,12 @@ moe_wgrad_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         if (p.panels_a) {
           if (lane == 0) ptx::tma_load_4d_pair(a_dst, &tmap_a, 0, k, m0 >> 6, 0, bar);
         } else if (lane < 2) {
-          ptx::tma_load_2d_pair(a_dst + lane * 8192, &tmap_a, m0 + lane * 64, k, bar);
+          ptx::tma_load_2d_pair(a_dst + lane * (operand_bytes / 2), &tmap_a, m0 + lane * 64, k, bar);
         }
         if (p.panels_b) {
           if (lane == 2) ptx::tma_load_4d_pair(b_dst, &tmap_b, 0, k, n0 >> 6, 0, bar);
         } else if (lane == 2 || lane == 3) {
-          ptx::tma_load_2d_pair(b_dst + (lane - 2) * 8192, &tmap_b, n0 + (lane - 2) * 64, k, bar);
+          ptx::tma_load_2d_pair(b_dst + (lane - 2) * (operand_bytes / 2), &tmap_b, n0 + (lane - 2) * 64, k, bar);
         }
         __syncwarp();
         ring.next(p.stages);
@@ -844,7 +862,7 @@ moe_wgrad_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       // fp32 accumulate, both operands MN-major, 256 x 256
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
                              (static_cast<uint32_t>(kTileN >> 3) << 17) | (static_cast<uint32_t>((kRows * 2) >> 4) << 24);
-      const uint64_t desc = ptx::make_smem_desc(0, 8192, 1024);
+      const uint64_t desc = ptx::make_smem_desc(0, operand_bytes / 2, 1024);
       Cursor ring, acc;
       bool ok = true;
       for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
@@ -1006,18 +1024,185 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, const i
   }
 }
 
-// dweights[pair] = sum over the parts of the pair's row, in order.
+// dweights[pair] = sum over the parts of the pair's row: 16 lanes per pair, each adding every
+// sixteenth part, then pairwise.
 __global__ void __launch_bounds__(256) weight_grad_kernel(const float* dw_part, const int* pos, float* dweights,
                                                           int pairs, int parts) {
   dependency_wait();
   dependency_release();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= pairs) return;
-  const int row = pos[i];
+  const int i = blockIdx.x * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  const int row = i < pairs ? pos[i] : -1;
   float sum = 0.f;
   if (row >= 0)
-    for (int c = 0; c < parts; ++c) sum += dw_part[static_cast<long long>(row) * parts + c];
-  dweights[i] = sum;
+    for (int c = lane; c < parts; c += 16) sum += dw_part[static_cast<long long>(row) * parts + c];
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (i < pairs && lane == 0) dweights[i] = sum;
+}
+
+// ------------------------------------------------------------------------------------ one token
+//
+// For a single token every expert's weights are read for one row, and reading them is all there is
+// to do: 100 MB for 8 experts of 2048/1024, 15.6 us at the measured copy rate.  stream_kernel reads
+// them with 16-byte loads, eight to sixteen rows of weights per warp in flight, and multiplies on
+// the CUDA cores in fp32: a block owns one expert, 256 columns and a slice of K.  The slices fill
+// the SMs three blocks deep; their sums meet in fp32 in the next kernel, in order: the gate/up
+// slices when the down product computes its hidden activation (which is never rounded here), the
+// down slices in stream_join_kernel.  No sorting, no row tiles.  (From two tokens on the tiles win:
+// rows that share an expert would have to share a read, and four rows at a time the CUDA cores
+// bound this kernel: 2 tokens 82 us, 4 tokens 111 us against 86 us for 5 tokens in tiles.)
+constexpr int kStreamPairs = 32;
+constexpr int kStreamThreads = 256;
+constexpr int kStreamCols = 256;   // a warp's 32 lanes x 8 columns
+constexpr int kStreamMaxK = 1024;  // of a slice
+
+struct StreamParams {
+  const void* ids;
+  int wide, experts, pairs, top_k;
+  const float* weights;
+  const void* x;       // gate/up: rows of x
+  long long ld_x;
+  const float* parts;  // down: gate/up sums, [pairs][parts_n][2 k]
+  int parts_n;
+  const void* w;       // weights [experts][k][cols]
+  long long expert_pitch, row_pitch;
+  int k, cols, slices, slice_k;  // slice_k: a multiple of 64
+  int activation;
+  float* out;          // [pairs][slices][cols]
+};
+
+__device__ __forceinline__ uint4 load_streaming(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <typename T, bool DOWN>
+__global__ void __launch_bounds__(kStreamThreads, 3) stream_kernel(const StreamParams p) {
+  __shared__ float row[kStreamMaxK];  // this slice of a pair's row
+  __shared__ float sums[8][kStreamCols + 8];
+  __shared__ int list[kStreamPairs];
+  __shared__ int list_n;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slice = blockIdx.x % p.slices, chunk = blockIdx.x / p.slices;
+  const int k0 = slice * p.slice_k, k1 = min(k0 + p.slice_k, p.k);
+  const int col = chunk * kStreamCols + lane * 8;
+  // (ids and weights were complete before the kernel ahead of this one started: see
+  // dependency_release() there)
+  if (!DOWN) {
+    dependency_wait();
+    dependency_release();
+  }
+  const int pair = blockIdx.y;
+  const int e = pair_expert(p.ids, p.wide, p.experts, pair);
+  // the first pair of an expert works for all of them
+  if (warp == 0) {
+    int n = 0;
+    bool first = e >= 0;
+    for (int base = 0; base < p.pairs; base += 32) {
+      const int i = base + lane;
+      const bool same = i < p.pairs && e >= 0 && pair_expert(p.ids, p.wide, p.experts, i) == e;
+      const unsigned mask = __ballot_sync(0xffffffffu, same);
+      if (__ballot_sync(0xffffffffu, same && i < pair) != 0) first = false;
+      if (same) list[n + __popc(mask & ((1u << lane) - 1u))] = i;
+      n += __popc(mask);
+    }
+    if (lane == 0) list_n = first ? n : 0;
+  }
+  const T* w = static_cast<const T*>(p.w) + static_cast<long long>(e < 0 ? 0 : e) * p.expert_pitch + col;
+  const bool inside = col < p.cols;
+  // A warp's rows of weights: k0 + 8 warp + 64 i + (0..7).  The first eight are on their way before
+  // anything this kernel depends on is waited for.
+  uint4 v[8];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = inside && k + j < k1 ? load_streaming(w + static_cast<long long>(k + j) * p.row_pitch) : make_uint4(0, 0, 0, 0);
+  };
+  __syncthreads();
+  const int n = list_n;
+  if (n > 0) fetch(k0 + warp * 8);
+  if (DOWN) {
+    dependency_wait();
+    dependency_release();
+  }
+  for (int r = 0; r < n; ++r) {  // (more than one only where an expert stands in several slots)
+    const int q = list[r];
+    for (int i = tid; i < p.slice_k; i += kStreamThreads) {
+      const int k = k0 + i;
+      float val = 0.f;
+      if (k < k1) {
+        if (DOWN) {
+          const float2* src = reinterpret_cast<const float2*>(p.parts) + static_cast<long long>(q) * p.parts_n * p.k + k;
+          float2 gu = make_float2(0.f, 0.f);
+#pragma unroll 8
+          for (int s = 0; s < p.parts_n; ++s) {
+            const float2 part = src[static_cast<long long>(s) * p.k];
+            gu.x += part.x;
+            gu.y += part.y;
+          }
+          val = p.weights[q] * gate_act(gu.x, p.activation).x * gu.y;
+        } else {
+          val = elem::to_float(static_cast<const T*>(p.x)[q / p.top_k * p.ld_x + k]);
+        }
+      }
+      row[i] = val;
+    }
+    __syncthreads();
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r > 0) fetch(k0 + warp * 8);
+    for (int i = warp * 8; i < p.slice_k; i += 64) {
+      uint4 now[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[j] = v[j];
+      if (i + 64 < p.slice_k) fetch(k0 + i + 64);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const T* t = reinterpret_cast<const T*>(&now[j]);
+        const float a = row[i + j];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] += a * elem::to_float(t[c]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; c += 4)
+      *reinterpret_cast<float4*>(&sums[warp][lane * 8 + c]) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+    __syncthreads();
+    const int c = chunk * kStreamCols + tid;
+    if (c < p.cols) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += sums[i][tid];
+      p.out[(static_cast<long long>(q) * p.slices + slice) * p.cols + c] = sum;
+    }
+    // (the next round's writes of `row` and `sums` are a barrier away from this one's reads)
+    __syncthreads();
+  }
+}
+
+// y[t] = sum over slots and slices, in order within each of eight strands, then pairwise.
+template <typename T>
+__global__ void __launch_bounds__(256) stream_join_kernel(const StreamParams p, T* y, long long ld_y) {
+  __shared__ float sums[8][33];
+  const int c = blockIdx.x * 32 + threadIdx.x, strand = threadIdx.y, t = blockIdx.y;
+  dependency_wait();
+  dependency_release();
+  float sum = 0.f;
+  if (c < p.cols)
+#pragma unroll 8
+    for (int i = strand; i < p.top_k * p.slices; i += 8) {
+      const int q = t * p.top_k + i / p.slices;
+      if (pair_expert(p.ids, p.wide, p.experts, q) >= 0)
+        sum += p.out[(static_cast<long long>(q) * p.slices + i % p.slices) * p.cols + c];
+    }
+  sums[strand][threadIdx.x] = sum;
+  __syncthreads();
+  if (strand == 0 && c < p.cols) {
+    for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+    y[t * ld_y + c] = elem::from_float<T>(sum);
+  }
 }
 
 // ------------------------------------------------------------------------------------- host
@@ -1031,6 +1216,9 @@ struct Layout {
   int64_t max_rows;
   int chunk, chunks;
   bool gather;                 // the copy engine picks the rows of x
+  bool stream;                 // one token: stream_kernel
+  int up_slices, up_slice_k, down_slices, down_slice_k;
+  int64_t up_bytes, down_bytes;
   int down_splits, dx_splits;  // slices of K of the two products with fp32 rows
   int dw_parts;
   // The plan, the hidden activation and the gate/up products: in `saved` when training.
@@ -1084,7 +1272,7 @@ int moe_check(const tnx_moe_problem* p) {
 }
 
 // Slices of K for a product with `cols` output columns over num_kb K blocks: the number that takes
-// the least time when a K block costs 0.3 us, a tile 2 us of its own, and each slice writes and
+// the least time when a K block costs 0.6 us, a tile 2 us of its own, and each slice writes and
 // reads its copy of the rows at 6 TB/s.  With few tiles this fills the last wave (8 experts of
 // 4096/14336, 500 tokens: 128 tiles for 74 pairs of SMs).
 int pick_splits(const Layout& l, int cols, int num_kb) {
@@ -1092,9 +1280,9 @@ int pick_splits(const Layout& l, int cols, int num_kb) {
   const double units = static_cast<double>(l.max_tiles) * cdiv(cols, 2 * kRows);
   int best = 1;
   double least = 0.0;
-  for (int s = 1; s <= 8 && num_kb / s >= 4; s *= 2) {
+  for (int s = 1; s <= 8 && num_kb / s >= 2; s *= 2) {
     const int waves = static_cast<int>((units * s + clusters - 1) / clusters);
-    const double us = waves * (0.3 * cdiv(num_kb, s) + 2.0) + s * (8.0 * l.pairs * cols / 6.0e6);
+    const double us = waves * (0.6 * cdiv(num_kb, s) + 2.0) + s * (8.0 * l.pairs * cols / 6.0e6);
     if (s == 1 || us < 0.95 * least) {
       best = s;
       least = us;
@@ -1103,9 +1291,26 @@ int pick_splits(const Layout& l, int cols, int num_kb) {
   return best;
 }
 
+// Slices of K of the streamed products: three blocks for every SM, slices of 64 to kStreamMaxK.
+void pick_slices(int pairs, int cols, int k, int* slices, int* slice_k) {
+  const int blocks = pairs * cdiv(cols, kStreamCols);
+  int n = cdiv(3 * sm_count(), blocks);
+  if (n > cdiv(k, 64)) n = cdiv(k, 64);
+  if (n < cdiv(k, kStreamMaxK)) n = cdiv(k, kStreamMaxK);
+  *slice_k = cdiv(cdiv(k, n), 64) * 64;
+  *slices = cdiv(k, *slice_k);
+}
+
 Layout lay_out_problem(const tnx_moe_problem& p) {
   Layout l = {};
   l.pairs = p.tokens * p.top_k;
+  l.stream = !p.train && p.tokens == 1 && l.pairs <= kStreamPairs;
+  if (l.stream) {
+    pick_slices(l.pairs, 2 * p.d_ff, p.d_model, &l.up_slices, &l.up_slice_k);
+    pick_slices(l.pairs, p.n_out, p.d_ff, &l.down_slices, &l.down_slice_k);
+    l.up_bytes = align256(static_cast<int64_t>(l.pairs) * l.up_slices * p.d_ff * 8);
+    l.down_bytes = align256(static_cast<int64_t>(l.pairs) * l.down_slices * p.n_out * 4);
+  }
   const int hit = l.pairs < p.experts ? l.pairs : p.experts;  // experts with rows at most
   l.max_tiles = (l.pairs - hit) / kTileN + hit;
   l.max_rows = (static_cast<int64_t>(l.pairs) + static_cast<int64_t>(hit) * (kPad - 1)) / kPad * kPad;
@@ -1185,11 +1390,11 @@ cudaError_t allow_smem(const void* fn, int bytes) {
 
 // Launches with programmatic stream serialization (every kernel here calls dependency_wait()).
 template <typename... KArgs, typename... Args>
-int launch(const char* what, void (*fn)(KArgs...), int grid, int block, int smem, int cluster, cudaStream_t stream,
+int launch(const char* what, void (*fn)(KArgs...), dim3 grid, dim3 block, int smem, int cluster, cudaStream_t stream,
            Args... args) {
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  lc.blockDim = dim3(static_cast<unsigned>(block), 1, 1);
+  lc.gridDim = grid;
+  lc.blockDim = block;
   lc.dynamicSmemBytes = static_cast<size_t>(smem);
   lc.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1224,13 +1429,10 @@ int launch_pairs(Fn fn, int threads, Params p, int staging_bytes, int64_t units,
   return launch("experts' products", fn, clusters * 2, threads, p.stages * kStageBytes + fixed, 2, stream, maps..., p);
 }
 // Tensor maps over rows in expert order, as moe_rows_kernel reads them.
-struct RowsMaps {
-  CUtensorMap r128, r64, r16;
-};
-int rows_maps(RowsMaps* m, const void* rows, int dtype, int cols, int64_t max_rows) {
-  int rc = make_tmap_2d(&m->r128, rows, dtype, cols, max_rows, cols, 64, 128, true);
-  if (rc == TNX_OK) rc = make_tmap_2d(&m->r64, rows, dtype, cols, max_rows, cols, 64, 64, true);
-  if (rc == TNX_OK) rc = make_tmap_2d(&m->r16, rows, dtype, cols, max_rows, cols, 64, 16, true);
+int rows_maps(RowsMaps* maps, const void* rows, int dtype, int cols, int64_t max_rows) {
+  int rc = TNX_OK;
+  for (int i = 0; i < 4 && rc == TNX_OK; ++i)
+    rc = make_tmap_2d(&maps->m[i], rows, dtype, cols, max_rows, cols, 64, 128 >> i, true);
   return rc;
 }
 // A map over the weights [experts][rows][cols] with K down their rows.
@@ -1247,8 +1449,8 @@ int launch_rows(const tnx_moe_problem& q, const Layout& l, const CUtensorMap& w,
   p.max_rows = l.max_rows;
   const int64_t units = static_cast<int64_t>(l.max_tiles) * p.tiles_n * p.splits;
   return q.dtype == TNX_BF16
-             ? launch_pairs(moe_rows_kernel<MODE, true>, kRowsThreads, p, 0, units, stream, w, r.r128, r.r64, r.r16)
-             : launch_pairs(moe_rows_kernel<MODE, false>, kRowsThreads, p, 0, units, stream, w, r.r128, r.r64, r.r16);
+             ? launch_pairs(moe_rows_kernel<MODE, true>, kRowsThreads, p, 0, units, stream, w, r)
+             : launch_pairs(moe_rows_kernel<MODE, false>, kRowsThreads, p, 0, units, stream, w, r);
 }
 // out[e] = a[rows of e]^T b[rows of e], m x n.
 int run_wgrad(const tnx_moe_problem& q, const Layout& l, const Plan& plan, const void* a, int m, const void* b, int n,
@@ -1342,10 +1544,54 @@ RowsParams rows_params(const tnx_moe_problem& p, const Plan& plan, int32_t* stat
   return g;
 }
 // Cuts K into `splits` slices, none of them empty.
-void split_k(RowsParams* g, int num_kb, int splits) {
+void split_k(RowsParams* g, int k, int splits) {
+  const int num_kb = cdiv(k, kTileK);
+  g->k = k;
   g->num_kb = num_kb;
   g->kb_per_split = cdiv(num_kb, splits);
   g->splits = cdiv(num_kb, g->kb_per_split);
+}
+
+template <typename T>
+int run_stream(const tnx_moe_problem& p, const Layout& l, const void* x, const void* w12, const void* w3,
+               const void* ids, const float* weights, T* y, char* ws, cudaStream_t stream) {
+  StreamParams q = {};
+  q.ids = ids;
+  q.wide = p.wide_ids;
+  q.experts = p.experts;
+  q.pairs = l.pairs;
+  q.top_k = p.top_k;
+  q.weights = weights;
+  q.activation = p.activation;
+  q.x = x;
+  q.ld_x = p.stride_x;
+  q.w = w12;
+  q.expert_pitch = p.stride_w12e;
+  q.row_pitch = p.stride_w12k;
+  q.k = p.d_model;
+  q.cols = 2 * p.d_ff;
+  q.slices = l.up_slices;
+  q.slice_k = l.up_slice_k;
+  q.out = reinterpret_cast<float*>(ws);
+  dim3 grid(static_cast<unsigned>(cdiv(q.cols, kStreamCols) * q.slices), static_cast<unsigned>(l.pairs));
+  int rc = launch("streamed gate/up product", stream_kernel<T, false>, grid, dim3(kStreamThreads), 0, 1, stream, q);
+  if (rc != TNX_OK) return rc;
+  q.parts = q.out;
+  q.parts_n = q.slices;
+  q.w = w3;
+  q.expert_pitch = p.stride_w3e;
+  q.row_pitch = p.stride_w3k;
+  q.k = p.d_ff;
+  q.cols = p.n_out;
+  q.slices = l.down_slices;
+  q.slice_k = l.down_slice_k;
+  q.out = reinterpret_cast<float*>(ws + l.up_bytes);
+  grid.x = static_cast<unsigned>(cdiv(q.cols, kStreamCols) * q.slices);
+  rc = launch("streamed down product", stream_kernel<T, true>, grid, dim3(kStreamThreads), 0, 1, stream, q);
+  if (rc != TNX_OK) return rc;
+  return launch("joining streamed products", stream_join_kernel<T>,
+                dim3(static_cast<unsigned>(cdiv(p.n_out, 32)), static_cast<unsigned>(p.tokens)), dim3(32, 8), 0, 1, stream,
+                q, y, static_cast<long long>(p.stride_y));
 }
 
 bool misaligned(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15u) != 0; }
@@ -1369,7 +1615,8 @@ int tnx_moe_query(const tnx_moe_problem* problem, tnx_moe_resources* out) {
   out->max_tiles = l.max_tiles;
   const int64_t keep = l.plan_bytes + l.hidden_bytes;
   out->saved_bytes = keep + l.gu_bytes;
-  out->workspace_bytes = l.part_bytes + l.chunk_bytes + l.x_bytes + (problem->train ? 0 : keep);
+  out->workspace_bytes =
+      l.stream ? l.up_bytes + l.down_bytes : l.part_bytes + l.chunk_bytes + l.x_bytes + (problem->train ? 0 : keep);
   out->backward_workspace_bytes = l.dgu_bytes + l.dx_bytes + l.dw_bytes + l.x_bytes + l.dy_bytes;
   return TNX_OK;
 }
@@ -1401,6 +1648,10 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Layout l = lay_out_problem(p);
   char* ws = static_cast<char*>(workspace);
+  if (l.stream)
+    return p.dtype == TNX_BF16
+               ? run_stream(p, l, x, w12, w3, ids, weights, static_cast<__nv_bfloat16*>(y), ws, s)
+               : run_stream(p, l, x, w12, w3, ids, weights, static_cast<__half*>(y), ws, s);
   float* part = reinterpret_cast<float*>(ws);
   void* chunk_counts = ws + l.part_bytes;
   void* xp = ws + l.part_bytes + l.chunk_bytes;
@@ -1415,7 +1666,7 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
 
   // H = w * act(x W1) * (x W2)
   RowsParams g = rows_params(p, plan, status_word);
-  split_k(&g, cdiv(p.d_model, kTileK), 1);
+  split_k(&g, p.d_model, 1);
   g.cols = 2 * p.d_ff;
   g.out = hidden;
   g.gu = static_cast<float*>(gu);
@@ -1423,8 +1674,8 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   RowsMaps rows;
   rc = weights_map(&tw, &g, p, w12, 2 * p.d_ff, p.d_model, p.stride_w12k, p.stride_w12e);
   if (rc == TNX_OK && l.gather) {
-    rc = make_tmap_2d(&rows.r16, x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true);
-    rows.r128 = rows.r64 = rows.r16;
+    rc = make_tmap_2d(&rows.m[3], x, p.dtype, p.d_model, p.tokens, p.stride_x, 64, 1, true);
+    rows.m[0] = rows.m[1] = rows.m[2] = rows.m[3];
   } else if (rc == TNX_OK) {
     rc = rows_maps(&rows, xp, p.dtype, p.d_model, l.max_rows);
   }
@@ -1433,7 +1684,7 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
   if (rc != TNX_OK) return rc;
 
   // O = H W3
-  split_k(&g, cdiv(p.d_ff, kTileK), l.down_splits);
+  split_k(&g, p.d_ff, l.down_splits);
   g.cols = p.n_out;
   g.out = part;
   rc = weights_map(&tw, &g, p, w3, p.n_out, p.d_ff, p.stride_w3k, p.stride_w3e);
@@ -1497,7 +1748,7 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
   CUtensorMap tw;
   RowsMaps rows;
   if (hidden_grad) {
-    split_k(&g, cdiv(p.n_out, kTileK), 1);
+    split_k(&g, p.n_out, 1);
     g.cols = p.d_ff;
     g.out = dgu;
     g.gu = gu;
@@ -1508,12 +1759,12 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
     if (rc == TNX_OK) rc = rows_maps(&rows, dyp, p.dtype, p.n_out, l.max_rows);
     if (rc == TNX_OK) rc = launch_rows<kDHidden>(p, l, tw, rows, g, s);
     if (rc == TNX_OK && dweights != nullptr)
-      rc = launch("routing weights' gradient", weight_grad_kernel, cdiv(l.pairs, 256), 256, 0, 1, s,
+      rc = launch("routing weights' gradient", weight_grad_kernel, cdiv(l.pairs, 16), 256, 0, 1, s,
                   static_cast<const float*>(dw_part), static_cast<const int*>(plan.pos), dweights, l.pairs, l.dw_parts);
     if (rc != TNX_OK) return rc;
   }
   if (dx != nullptr) {
-    split_k(&g, cdiv(static_cast<int>(two_f), kTileK), l.dx_splits);
+    split_k(&g, static_cast<int>(two_f), l.dx_splits);
     g.cols = p.d_model;
     g.out = dx_part;
     rc = make_tmap_3d(&tw, w12, p.dtype, two_f, p.d_model, p.experts, p.stride_w12k, p.stride_w12e, 64, kRows, true);

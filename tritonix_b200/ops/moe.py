@@ -13,14 +13,11 @@ import torch
 from tritonix_b200 import _cabi
 
 
-def _route_problem(logits, top_k, groups, top_groups, scoring, renormalize, scale):
-    return _cabi.RouteProblem(logits.shape[0], logits.shape[1], top_k, groups, top_groups, scoring,
-                              int(renormalize), _cabi.DTYPES[logits.dtype], scale, 0, logits.stride(0))
+_route_problems: dict = {}
 
 
-def _route(logits, bias, args):
-    problem = _route_problem(logits, *args)
-    shape = (logits.shape[0], args[0])
+def _route(logits, bias, problem):
+    shape = (logits.shape[0], problem.top_k)
     weights = torch.empty(shape, device=logits.device, dtype=torch.float32)
     ids = torch.empty(shape, device=logits.device, dtype=torch.int32)
     _cabi.call(logits.device, _cabi.lib.tnx_route_experts, ctypes.byref(problem), logits.data_ptr(),
@@ -30,11 +27,11 @@ def _route(logits, bias, args):
 
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, args):
-        weights, ids = _route(logits, bias, args)
+    def forward(ctx, logits, bias, problem):
+        weights, ids = _route(logits, bias, problem)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids)
-        ctx.args = args
+        ctx.problem = problem
         ctx.mark_non_differentiable(ids)
         return weights, ids
 
@@ -44,10 +41,9 @@ class _RouteExperts(torch.autograd.Function):
         if dweights is None:
             return None, None, None
         logits, ids = ctx.saved_tensors
-        problem = _route_problem(logits, *ctx.args)
         dweights = dweights.contiguous()
         dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        _cabi.call(logits.device, _cabi.lib.tnx_route_experts_backward, ctypes.byref(problem),
+        _cabi.call(logits.device, _cabi.lib.tnx_route_experts_backward, ctypes.byref(ctx.problem),
                    logits.data_ptr(), ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
         return dlogits, None, None
 
@@ -68,6 +64,25 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     Experts are told apart as in 64-bit arithmetic, however close.  An expert whose logit is -inf
     has the score 0 (a row of nothing else has the weights 0); a NaN logit ranks last.  ``ids`` are
     always distinct and in range."""
+    key = (_cabi.signature(logits, bias), top_k, scoring, num_groups, top_groups, renormalize, scale)
+    problem = _route_problems.get(key)
+    if problem is None:
+        problem = _cabi.remember(_route_problems, key, _check_route(logits, top_k, scoring, bias, num_groups, top_groups,
+                                                                    renormalize, scale))
+    if not problem.stride_logits:
+        logits = _cabi.rows_view(logits)
+        return route_experts(logits, top_k, scoring=scoring, bias=bias, num_groups=num_groups, top_groups=top_groups,
+                             renormalize=renormalize, scale=scale)
+    if bias is not None:
+        bias = bias.detach().contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouteExperts.apply(logits, bias, problem)
+    return _route(logits, bias, problem)
+
+
+def _check_route(logits, top_k, scoring, bias, groups, top_groups, renormalize, scale) -> _cabi.RouteProblem:
+    """The C problem of a call whose arguments are sound; its stride is 0 where the logits have to be
+    copied first."""
     _cabi.require_cuda(logits, *([bias] if bias is not None else []))
     if logits.dim() != 2 or logits.dtype not in _cabi.DTYPES:
         raise ValueError("logits must be a 2-D float16, bfloat16 or float32 tensor, got "
@@ -80,27 +95,31 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
                              f"{tuple(bias.shape)} {bias.dtype}")
         if bias.device != logits.device:
             raise ValueError("logits and bias must live on the same device")
-        bias = bias.detach().contiguous()
-    logits = _cabi.rows_view(logits)
-    args = (int(top_k), int(num_groups), int(top_groups), _cabi.SCORINGS[scoring], bool(renormalize),
-            float(scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteExperts.apply(logits, bias, args)
-    return _route(logits, bias, args)
+    if logits.shape[0] >= 1 << 31:
+        raise ValueError("too many tokens")
+    stride = max(logits.stride(0), logits.shape[1]) if logits.shape[0] <= 1 else logits.stride(0)
+    if _cabi.rows_view(logits) is not logits:
+        stride = 0
+    return _cabi.RouteProblem(logits.shape[0], logits.shape[1], int(top_k), int(groups), int(top_groups),
+                              _cabi.SCORINGS[scoring], int(bool(renormalize)), _cabi.DTYPES[logits.dtype], float(scale),
+                              0, stride)
 
 
 # ------------------------------------------------------------------------------ experts' products
 
-def _pitched(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the copy engine can address it: adjacent elements in rows, 16-byte aligned base and
-    pitches, no overlapping rows or matrices; a contiguous copy of anything else."""
-    shape, stride = t.shape, t.stride()
-    fine = stride[-1] == 1 and t.data_ptr() % 16 == 0
-    extent = shape[-1]
-    for size, step in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+def _addressable(t: torch.Tensor) -> bool:
+    """Adjacent elements in rows, pitches of 16 bytes, no overlapping rows or matrices."""
+    fine, extent = t.stride(-1) == 1, t.shape[-1]
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if size > 1:
             fine = fine and step % 8 == 0 and step >= extent
         extent = size * (step if size > 1 else extent)
+    return fine
+
+
+def _pitched(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the copy engine can address it: itself, or a contiguous copy."""
+    fine = _addressable(t) and t.data_ptr() % 16 == 0
     return t if fine else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -115,39 +134,42 @@ def _pitches(t: torch.Tensor) -> list:
     return out[::-1]
 
 
+class _MoePlan:
+    """What a call signature needs, worked out once: the C problem and its resources without and with
+    gradients, or that operands have to be copied first."""
+
+    def __init__(self, x, w12, w3, ids, weights, activation):
+        act = _check_moe(x, w12, w3, ids, weights, activation)
+        self.addressable = all(_addressable(t) for t in (x, w12, w3))
+        if not self.addressable:
+            return
+        self.out = (x.shape[0], w3.shape[2])
+        self.pairs, self.device = ids.shape, x.device
+        (sx,), (s12e, s12k), (s3e, s3k) = _pitches(x), _pitches(w12), _pitches(w3)
+        self.problems, self.resources = [], []
+        for train in (0, 1):
+            problem = _cabi.MoeProblem(x.shape[0], w12.shape[0], ids.shape[1], x.shape[1], w3.shape[1], w3.shape[2],
+                                       _cabi.DTYPES[x.dtype], act, int(ids.dtype == torch.int64), train, sx, s12e, s12k,
+                                       s3e, s3k, w3.shape[2])
+            res = _cabi.MoeResources()
+            _cabi.raise_for(_cabi.lib.tnx_moe_query(ctypes.byref(problem), ctypes.byref(res)))
+            self.problems.append(problem)
+            self.resources.append(res)
+
+
 _moe_plans: dict = {}
 
 
-def _moe_plan(x, w12, w3, ids, activation, train):
-    """(problem, resources) of a call signature, validated once."""
-    key = (x.shape, w12.shape, w3.shape[2], ids.shape, x.dtype, ids.dtype, activation, train, x.stride(),
-           w12.stride(), w3.stride())
-    plan = _moe_plans.get(key)
-    if plan is None:
-        tokens, d_model = x.shape
-        experts, d_ff, n_out = w3.shape
-        (sx,), (s12e, s12k), (s3e, s3k) = _pitches(x), _pitches(w12), _pitches(w3)
-        problem = _cabi.MoeProblem(tokens, experts, ids.shape[1], d_model, d_ff, n_out, _cabi.DTYPES[x.dtype],
-                                   activation, int(ids.dtype == torch.int64), int(train), sx, s12e, s12k, s3e, s3k,
-                                   n_out)
-        res = _cabi.MoeResources()
-        _cabi.raise_for(_cabi.lib.tnx_moe_query(ctypes.byref(problem), ctypes.byref(res)))
-        if len(_moe_plans) > 4096:
-            _moe_plans.clear()
-        plan = _moe_plans[key] = (problem, res)
-    return plan
-
-
-def _moe_forward(x, w12, w3, ids, weights, activation, train):
-    problem, res = _moe_plan(x, w12, w3, ids, activation, train)
-    device = x.device
-    y = torch.empty((x.shape[0], w3.shape[2]), device=device, dtype=x.dtype)
+def _moe_forward(plan, x, w12, w3, ids, weights, train):
+    device = plan.device
+    y = torch.empty(plan.out, device=device, dtype=x.dtype)
     # (scratch of the call's own: calls on different streams or in different graphs never share it)
-    workspace = torch.empty(res.workspace_bytes, device=device, dtype=torch.uint8)
-    saved = torch.empty(res.saved_bytes, device=device, dtype=torch.uint8) if train else None
-    _cabi.call(device, _cabi.lib.tnx_moe_swiglu, ctypes.byref(problem), x.data_ptr(), w12.data_ptr(), w3.data_ptr(),
-               ids.data_ptr(), weights.data_ptr(), y.data_ptr(), saved.data_ptr() if train else None,
-               workspace.data_ptr(), workspace.numel(), _cabi.status_word(device).data_ptr())
+    nbytes = plan.resources[train].workspace_bytes
+    workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    saved = torch.empty(plan.resources[1].saved_bytes, device=device, dtype=torch.uint8) if train else None
+    _cabi.call(device, _cabi.lib.tnx_moe_swiglu, ctypes.byref(plan.problems[train]), x.data_ptr(), w12.data_ptr(),
+               w3.data_ptr(), ids.data_ptr(), weights.data_ptr(), y.data_ptr(), saved.data_ptr() if train else None,
+               workspace.data_ptr(), nbytes, _cabi.status_word(device).data_ptr())
     return y, saved
 
 
@@ -156,17 +178,17 @@ class _MoeSwiglu(torch.autograd.Function):
     (fp32): 10 bytes per pair and hidden column."""
 
     @staticmethod
-    def forward(ctx, x, w12, w3, weights, ids, activation):
-        y, saved = _moe_forward(x, w12, w3, ids, weights, activation, True)
+    def forward(ctx, x, w12, w3, weights, ids, plan):
+        y, saved = _moe_forward(plan, x, w12, w3, ids, weights, 1)
         ctx.save_for_backward(x, w12, w3, saved)
-        ctx.ids_like, ctx.activation = torch.empty(ids.shape, dtype=ids.dtype, device="meta"), activation
+        ctx.plan = plan
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w12, w3, saved = ctx.saved_tensors
-        problem, res = _moe_plan(x, w12, w3, ctx.ids_like, ctx.activation, True)
+        plan = ctx.plan
         dy = _pitched(dy)
         (stride_dy,) = _pitches(dy)
         wants = ctx.needs_input_grad
@@ -174,10 +196,10 @@ class _MoeSwiglu(torch.autograd.Function):
         dx = new(x.shape, x.dtype) if wants[0] else None
         dw12 = new(w12.shape, x.dtype) if wants[1] else None
         dw3 = new(w3.shape, x.dtype) if wants[2] else None
-        dweights = new(ctx.ids_like.shape, torch.float32) if wants[3] else None
-        workspace = new(res.backward_workspace_bytes, torch.uint8)
+        dweights = new(plan.pairs, torch.float32) if wants[3] else None
+        workspace = new(plan.resources[1].backward_workspace_bytes, torch.uint8)
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        _cabi.call(x.device, _cabi.lib.tnx_moe_swiglu_backward, ctypes.byref(problem), dy.data_ptr(), stride_dy,
+        _cabi.call(x.device, _cabi.lib.tnx_moe_swiglu_backward, ctypes.byref(plan.problems[1]), dy.data_ptr(), stride_dy,
                    x.data_ptr(), w12.data_ptr(), w3.data_ptr(), saved.data_ptr(), ptr(dx), ptr(dw12), ptr(dw3),
                    ptr(dweights), workspace.data_ptr(), workspace.numel(), _cabi.status_word(x.device).data_ptr())
         return dx, dw12, dw3, dweights, None, None
@@ -198,6 +220,20 @@ def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.
 
     Gradients flow to ``x``, ``w12``, ``w3`` and ``weights``.  The routing stays on the device: no
     call waits for it.  Results do not depend on timing (every sum has a fixed order)."""
+    key = (_cabi.signature(x, w12, w3, ids, weights), activation)
+    plan = _moe_plans.get(key)
+    if plan is None:
+        plan = _cabi.remember(_moe_plans, key, _MoePlan(x, w12, w3, ids, weights, activation))
+    if not plan.addressable or (x.data_ptr() | w12.data_ptr() | w3.data_ptr()) & 15:
+        return moe_swiglu(_pitched(x), _pitched(w12), _pitched(w3), ids, weights, activation)
+    ids, weights = ids.contiguous(), weights.contiguous()
+    if (x.requires_grad or w12.requires_grad or w3.requires_grad or weights.requires_grad) \
+            and torch.is_grad_enabled():
+        return _MoeSwiglu.apply(x, w12, w3, weights, ids, plan)
+    return _moe_forward(plan, x, w12, w3, ids, weights, 0)[0]
+
+
+def _check_moe(x, w12, w3, ids, weights, activation) -> int:
     _cabi.require_cuda(x, w12, w3, ids, weights)
     if x.dtype not in (torch.float16, torch.bfloat16) or w12.dtype != x.dtype or w3.dtype != x.dtype:
         raise ValueError(f"x, w12 and w3 must all be float16 or all bfloat16, got {x.dtype}, {w12.dtype}, {w3.dtype}")
@@ -214,9 +250,4 @@ def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.
     act = _cabi.ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(_cabi.ACTIVATIONS)}, got {activation!r}")
-    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w12, w3, weights))
-    x, w12, w3 = _pitched(x), _pitched(w12), _pitched(w3)
-    ids, weights = ids.contiguous(), weights.contiguous()
-    if needs_grad:
-        return _MoeSwiglu.apply(x, w12, w3, weights, ids, act)
-    return _moe_forward(x, w12, w3, ids, weights, act, False)[0]
+    return act

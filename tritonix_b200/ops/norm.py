@@ -36,19 +36,35 @@ def _gate_form(gate, rows: int, cols: int, lead) -> int:
     raise ValueError(f"gate must be {(cols,)}, {(*lead, 1)} or {(*lead, cols)}, got {shape}")
 
 
-def _problem(rows, cols, dtype, weight_dtype, form, residual_scale, eps, y, residual, gate):
-    return _cabi.NormProblem(rows, cols, _cabi.DTYPES[dtype], _cabi.DTYPES[weight_dtype], form,
-                             residual_scale, eps, 0, y.stride(0), residual.stride(0),
-                             gate.stride(0) if form in (_cabi.GATE_TOKEN, _cabi.GATE_FULL) else 0)
+class _NormPlan:
+    """What a call signature needs, worked out once: the C problem for operands as rows, or that they
+    have to be brought into that shape first."""
+
+    def __init__(self, y, residual, post, pre, gate, residual_scale, eps):
+        form = _check(y, residual, post, pre, gate, eps)
+        rows, cols = y.numel() // y.shape[-1], y.shape[-1]
+        parts = [y, residual] + ([gate] if form in (_cabi.GATE_TOKEN, _cabi.GATE_FULL) else [])
+        vectors = [post, pre] + ([gate] if form == _cabi.GATE_CHANNEL else [])
+        self.ready = all(t.dim() == 2 and _cabi.rows_view(t) is t for t in parts) and \
+            all(t.is_contiguous() for t in vectors)
+        self.form, self.shape = form, (rows, cols)
+        if not self.ready:
+            return
+        pitch = lambda t: t.stride(0) if rows > 1 else t.shape[1]  # noqa: E731
+        self.problem = _cabi.NormProblem(rows, cols, _cabi.DTYPES[y.dtype], _cabi.DTYPES[post.dtype], form,
+                                         residual_scale, eps, 0, pitch(y), pitch(residual),
+                                         pitch(gate) if len(parts) == 3 else 0)
+        self.workspace_bytes = max(_cabi.lib.tnx_gated_residual_norm_workspace(ctypes.byref(self.problem)), 16)
 
 
-def _forward(y, residual, post, pre, gate, form, residual_scale, eps, keep_stats):
-    rows, cols = y.shape
-    h = torch.empty((rows, cols), device=y.device, dtype=y.dtype)
+_plans: dict = {}
+
+
+def _forward(plan, y, residual, post, pre, gate, keep_stats):
+    h = torch.empty(plan.shape, device=y.device, dtype=y.dtype)
     n = torch.empty_like(h)
-    stats = torch.empty((rows, 2), device=y.device, dtype=torch.float32) if keep_stats else None
-    problem = _problem(rows, cols, y.dtype, post.dtype, form, residual_scale, eps, y, residual, gate)
-    _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm, ctypes.byref(problem), y.data_ptr(),
+    stats = torch.empty((plan.shape[0], 2), device=y.device, dtype=torch.float32) if keep_stats else None
+    _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm, ctypes.byref(plan.problem), y.data_ptr(),
                residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
                gate.data_ptr() if gate is not None else None, h.data_ptr(), n.data_ptr(),
                stats.data_ptr() if stats is not None else None)
@@ -59,36 +75,30 @@ class _GatedResidualNorm(torch.autograd.Function):
     """Over 2-D operands.  Keeps y, residual and two reciprocal norms per row."""
 
     @staticmethod
-    def forward(ctx, y, residual, post, pre, gate, form, residual_scale, eps):
-        h, n, stats = _forward(y, residual, post, pre, gate, form, residual_scale, eps, True)
+    def forward(ctx, y, residual, post, pre, gate, plan):
+        h, n, stats = _forward(plan, y, residual, post, pre, gate, True)
         ctx.save_for_backward(y, residual, post, pre, gate, stats)
-        ctx.args = (form, residual_scale, eps)
+        ctx.plan = plan
         return h, n
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dn):
         y, residual, post, pre, gate, stats = ctx.saved_tensors
-        form, residual_scale, eps = ctx.args
-        rows, cols = y.shape
+        plan, device = ctx.plan, y.device
         dh, dn = _cabi.rows_view(dh), _cabi.rows_view(dn)
-        problem = _problem(rows, cols, y.dtype, post.dtype, form, residual_scale, eps, y, residual, gate)
-        dy = torch.empty((rows, cols), device=y.device, dtype=y.dtype)
+        dy = torch.empty(plan.shape, device=device, dtype=y.dtype)
         dres = torch.empty_like(dy)
-        dpost, dpre = (torch.empty(cols, device=y.device, dtype=post.dtype) for _ in range(2))
-        dgate = None
-        if gate is not None:
-            dgate = torch.empty(gate.shape, device=y.device, dtype=gate.dtype)
-        nbytes = _cabi.lib.tnx_gated_residual_norm_workspace(ctypes.byref(problem))
-        workspace = torch.empty(max(nbytes, 16), device=y.device, dtype=torch.uint8)
-        _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm_backward, ctypes.byref(problem),
+        dpost, dpre = torch.empty((2, plan.shape[1]), device=device, dtype=post.dtype).unbind()
+        dgate = torch.empty(gate.shape, device=device, dtype=gate.dtype) if gate is not None else None
+        workspace = torch.empty(plan.workspace_bytes, device=device, dtype=torch.uint8)
+        _cabi.call(device, _cabi.lib.tnx_gated_residual_norm_backward, ctypes.byref(plan.problem),
                    dh.data_ptr(), dh.stride(0), dn.data_ptr(), dn.stride(0), y.data_ptr(),
                    residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
                    gate.data_ptr() if gate is not None else None, stats.data_ptr(), dy.data_ptr(),
                    dres.data_ptr(), dpost.data_ptr(), dpre.data_ptr(),
-                   dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(),
-                   workspace.numel())
-        return dy, dres, dpost, dpre, dgate, None, None, None
+                   dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(), plan.workspace_bytes)
+        return dy, dres, dpost, dpre, dgate, None
 
 
 def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
@@ -100,6 +110,29 @@ def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: to
     ``pre_weight``: [D], and ``gate``: [D] (per channel), [..., 1] (per token) or [..., D] (per
     element), all of one type: that of ``y`` or fp32.  Gradients flow to every tensor argument;
     rows need not be contiguous with one another."""
+    key = (_cabi.signature(y, residual, post_weight, pre_weight, gate), residual_scale, eps)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _cabi.remember(_plans, key, _NormPlan(y, residual, post_weight, pre_weight, gate, float(residual_scale),
+                                                     float(eps)))
+    if not plan.ready:  # as rows, and once more
+        rows = plan.shape[0]
+        if plan.form == _cabi.GATE_CHANNEL:
+            gate = gate.contiguous()
+        elif gate is not None:
+            gate = _cabi.rows_view(gate.reshape(rows, gate.shape[-1]))
+        h, n = gated_residual_norm(_cabi.rows_view(y.reshape(plan.shape)), _cabi.rows_view(residual.reshape(plan.shape)),
+                                   post_weight.contiguous(), pre_weight.contiguous(), gate, residual_scale, eps)
+        return h.view(y.shape), n.view(y.shape)
+    if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or post_weight.requires_grad or
+                                    pre_weight.requires_grad or (gate is not None and gate.requires_grad)):
+        return _GatedResidualNorm.apply(y, residual, post_weight, pre_weight, gate, plan)
+    h, n, _ = _forward(plan, y, residual, post_weight, pre_weight, gate, False)
+    return h, n
+
+
+def _check(y, residual, post_weight, pre_weight, gate, eps) -> int:
+    """Refuses what the kernels cannot take; returns the gate's form."""
     tensors = [t for t in (y, residual, post_weight, pre_weight, gate) if t is not None]
     _cabi.require_cuda(*tensors)
     if y.dtype not in _cabi.DTYPES or residual.dtype != y.dtype:
@@ -123,18 +156,4 @@ def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: to
     rows = y.numel() // cols
     if rows >= 1 << 31:
         raise ValueError("too many rows")
-    form = _gate_form(gate, rows, cols, lead)
-    y2, r2 = _cabi.rows_view(y.reshape(rows, cols)), _cabi.rows_view(residual.reshape(rows, cols))
-    post, pre = post_weight.contiguous(), pre_weight.contiguous()
-    if form == _cabi.GATE_CHANNEL:
-        gate = gate.contiguous()
-    elif form != _cabi.GATE_NONE:
-        gate = _cabi.rows_view(gate.reshape(rows, gate.shape[-1]))
-        if gate.stride(0) < 0:
-            gate = gate.contiguous()
-    args = (y2, r2, post, pre, gate, form, float(residual_scale), float(eps))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        h, n = _GatedResidualNorm.apply(*args)
-    else:
-        h, n, _ = _forward(*args, False)
-    return h.view(y.shape), n.view(y.shape)
+    return _gate_form(gate, rows, cols, lead)
