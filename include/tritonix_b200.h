@@ -452,7 +452,7 @@ typedef struct tnx_norm_problem {
 /* stats: fp32[rows, 2], the reciprocal norms of y and h for the backward call; NULL = not kept. */
 int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, const void* residual,
                             const void* post_weight, const void* pre_weight, const void* gate, void* h, void* n,
-                            float* stats, void* stream);
+                            float* stats, int32_t* status_word, void* stream);
 /* Bytes of workspace the backward call needs. */
 int64_t tnx_gated_residual_norm_workspace(const tnx_norm_problem* problem);
 /* Gradients of every input from those of h and n (row pitches stride_dh, stride_dn).  dy and
@@ -462,7 +462,8 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
                                      const void* dn, int64_t stride_dn, const void* y, const void* residual,
                                      const void* post_weight, const void* pre_weight, const void* gate,
                                      const float* stats, void* dy, void* dresidual, void* dpost, void* dpre,
-                                     void* dgate, void* workspace, size_t workspace_bytes, void* stream);
+                                     void* dgate, void* workspace, size_t workspace_bytes, int32_t* status_word,
+                                     void* stream);
 
 /*
  * Experts' gated products:

@@ -79,6 +79,43 @@ def test_many_rows(t):
     check(make(t, 24, f32, f32, "token", seed=t))
 
 
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("t,d,dtype,wtype", [(595, 64, bf16, bf16), (1201, 2056, f16, f32), (700, 4096, bf16, f32),
+                                             (601, 4100, f32, f32), (600, 8192, f16, f16), (613, 1001, f32, f32),
+                                             (599, 2503, bf16, f32), (640, 5001, f32, f32), (592, 33, f16, f16)])
+def test_rows_that_arrive_ahead(t, d, dtype, wtype, gate):
+    """Enough rows for the kernels that walk them with copies a few rows ahead."""
+    check(make(t, d, dtype, wtype, gate, seed=t))
+
+
+@pytest.mark.parametrize("dtype,d", [(bf16, 16384), (f32, 16384), (bf16, 16383), (f16, 9001)])
+def test_many_long_rows(dtype, d):
+    check(make(597, d, dtype, dtype, "channel"))
+
+
+def test_rows_that_arrive_ahead_from_an_odd_address():
+    """The first row starts, and the last one ends, off a 16-byte boundary."""
+    case = make(600, 301, bf16, bf16, "full", seed=8)
+    args = on_gpu(case, False)
+    want = tnx.gated_residual_norm(*args)
+    views = []
+    for i, name in enumerate(("y", "residual", "gate")):
+        store = torch.empty(1 + i + 600 * 301, device=DEV, dtype=bf16)
+        store[1 + i:].copy_(case[name].to(DEV).reshape(-1))
+        views.append(store[1 + i:].view(600, 301))
+    got = tnx.gated_residual_norm(views[0], views[1], args[2], args[3], views[2])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_rows_apart():
+    case = make(800, 520, bf16, bf16, "full", seed=4)
+    padded = lambda t: torch.nn.functional.pad(t.to(DEV), (0, 24))[:, :520]  # noqa: E731
+    args = on_gpu(case, False)
+    want = tnx.gated_residual_norm(*args)
+    got = tnx.gated_residual_norm(padded(case["y"]), padded(case["residual"]), args[2], args[3], padded(case["gate"]))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_inference_gives_the_same_values():
     case = make(9, 520, bf16, bf16, "channel")
     h, n, _ = check(case)

@@ -44,12 +44,12 @@ def norm(**kw):
 
 
 def forward(p, y=PTR, gate=PTR):
-    return lib.tnx_gated_residual_norm(ctypes.byref(p), y, PTR, PTR, PTR, gate, PTR, PTR, None, None)
+    return lib.tnx_gated_residual_norm(ctypes.byref(p), y, PTR, PTR, PTR, gate, PTR, PTR, None, None, None)
 
 
 def backward(p, workspace=PTR, nbytes=1 << 30, stats=PTR, dgate=PTR):
     return lib.tnx_gated_residual_norm_backward(ctypes.byref(p), PTR, 64, PTR, 64, PTR, PTR, PTR, PTR, PTR, stats, PTR,
-                                                PTR, PTR, PTR, dgate, workspace, nbytes, None)
+                                                PTR, PTR, PTR, dgate, workspace, nbytes, None, None)
 
 
 @pytest.mark.parametrize("bad", [dict(rows=-1), dict(cols=0), dict(cols=16385), dict(dtype=4), dict(weight_dtype=_cabi.F16),

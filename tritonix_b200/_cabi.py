@@ -203,9 +203,9 @@ def _load() -> ctypes.CDLL:
     for name, problem, args in (
             ("tnx_route_experts", RouteProblem, [ptr] * 5),
             ("tnx_route_experts_backward", RouteProblem, [ptr] * 5),
-            ("tnx_gated_residual_norm", NormProblem, [ptr] * 9),
+            ("tnx_gated_residual_norm", NormProblem, [ptr] * 10),
             ("tnx_gated_residual_norm_backward", NormProblem,
-             [ptr, ctypes.c_int64, ptr, ctypes.c_int64] + [ptr] * 12 + [ctypes.c_size_t, ptr]),
+             [ptr, ctypes.c_int64, ptr, ctypes.c_int64] + [ptr] * 12 + [ctypes.c_size_t, ptr, ptr]),
             ("tnx_moe_swiglu", MoeProblem, [ptr] * 8 + [ctypes.c_size_t, ptr, ptr]),
             ("tnx_moe_swiglu_backward", MoeProblem,
              [ptr, ctypes.c_int64] + [ptr] * 9 + [ctypes.c_size_t, ptr, ptr])):

@@ -7,13 +7,21 @@
 // Both passes are bound by HBM: forward reads y and residual and writes h and n (4 values per
 // element), backward reads dh, dn, y, residual and writes dy, dresidual (6 values; h and the
 // normalised rows are recomputed in fp32 from the saved reciprocal norms, because a weight
-// gradient summed from an h that was rounded to 16 bits would carry that rounding).  A row stays
-// in the registers of its threads between its first load and its last store, so nothing is read
-// twice; reductions and all arithmetic are fp32.
+// gradient summed from an h that was rounded to 16 bits would carry that rounding).  Nothing is
+// read from memory twice; reductions and all arithmetic are fp32.
+//
+// Many rows go through the ring kernels: a block walks its share of the rows, whole rows arrive in
+// shared memory by bulk copies a few rows ahead, so that the two reductions of a row (a barrier
+// each) never leave HBM idle.  With a block per row and plain loads the same arithmetic reached
+// 59 % (forward) and 39 % (backward) of the copy rate at 4096 bf16 columns.  Few rows take the
+// plain kernels.
 #include <cuda_runtime.h>
+
+#include <mutex>
 
 #include "tnx_elem.cuh"
 #include "tnx_internal.h"
+#include "tnx_ptx.cuh"
 
 namespace tnx {
 
@@ -32,12 +40,16 @@ struct NormParams {
   void *dy, *dres, *dgate;  // dgate: [rows] (token form) or [rows][cols] (full form), weight type
   float* partial;           // [grid][sums][cols]: column sums for post, pre and a channel gate
   int sums;
+  // ring kernels
+  int depth;                // rows in flight
+  int* status;
+  unsigned long long timeout_ns;
 };
 
 constexpr int kMaxCols = 16384;
-// Threads of a row at most.  Vectors keep eight times the values in registers, so half as many
-// threads leave them twice the registers.
-__host__ __device__ constexpr int max_threads(int vec) { return vec == 1 ? 1024 : 512; }
+// Threads of a row at most, by the values each of them holds: 256 with up to 16 values (two or
+// three blocks per SM), then 512; single elements 640.
+__host__ __device__ constexpr int max_threads(int vec, int nv) { return vec == 1 ? 640 : vec * nv <= 16 ? 256 : 512; }
 
 // Sums of two values over the `threads` threads of a row.  `slot` alternates between calls so
 // that one barrier per call is enough.  Every thread of the block takes part.
@@ -79,7 +91,7 @@ __device__ __forceinline__ void load_gate(const NormParams& p, int row, int col,
 // blockDim = (threads of a row, rows of the block).  Vector v of a row belongs to thread
 // v % threads; a thread owns up to NV vectors.
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(max_threads(VEC)) norm_forward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(max_threads(VEC, NV), 1) norm_forward_kernel(const NormParams p) {
   __shared__ float2 sums[2][32];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int row = blockIdx.x * blockDim.y + threadIdx.y;
@@ -151,7 +163,7 @@ __global__ void __launch_bounds__(max_threads(VEC)) norm_forward_kernel(const No
 // A block walks rows blockIdx.x, blockIdx.x + gridDim.x, ... and keeps the column sums of its
 // rows in registers; norm_column_sums adds the blocks' sums in a fixed order.
 template <typename T, typename W, int VEC, int NV>
-__global__ void __launch_bounds__(max_threads(VEC)) norm_backward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(max_threads(VEC, NV), 1) norm_backward_kernel(const NormParams p) {
   __shared__ float2 sums[2][32];
   const int tid = threadIdx.x, threads = blockDim.x;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
@@ -253,6 +265,360 @@ __global__ void __launch_bounds__(max_threads(VEC)) norm_backward_kernel(const N
   }
 }
 
+// ------------------------------------------------------------------------------------ ring kernels
+
+constexpr int kMaxDepth = 4;
+constexpr int kAbort = 0x401;
+struct RingCtrl {
+  uint64_t full[kMaxDepth];
+  float2 sums[2][32];
+  int abort;
+};
+constexpr int kCtrlBytes = 768;
+static_assert(sizeof(RingCtrl) <= kCtrlBytes, "control block too large");
+
+// Shared memory for one row of one source: the row, moved by up to 15 bytes, in whole 16 bytes.
+__host__ __device__ constexpr uint32_t ring_row_bytes(int cols, int size) { return (cols * size + 15 + 15) / 16 * 16; }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Sum over the block, and whether `ok` held for every thread.
+__device__ __forceinline__ float2 block_sum(float a, float b, float2* smem, bool& ok) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if ((tid & 31) == 0) smem[tid >> 5] = make_float2(a, b);
+  ok = __syncthreads_and(ok) != 0;
+  const int warps = blockDim.x >> 5, lane = tid & 31;
+  float2 v = lane < warps ? smem[lane] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  return v;
+}
+
+// The rows a block walks: blockIdx.x, blockIdx.x + gridDim.x, ...  Row number i of them lies in slot
+// i % depth, one part of the slot per source.  A bulk copy starts and ends on 16-byte boundaries, so
+// a row is copied from the boundary at or before its first byte to the one at or after its last;
+// only the very last row of a tensor could be read past its end that way: its block copies it with
+// ordinary loads.
+constexpr int kMaxSources = 5;
+struct Ring {
+  RingCtrl* ctrl;
+  char* slots;  // (shared memory)
+  int sources, depth, rows;
+  uint32_t slot_bytes;
+  const char* src[kMaxSources];
+  long long pitch[kMaxSources];  // bytes
+  uint32_t row_bytes[kMaxSources], offset[kMaxSources];
+
+  __device__ __forceinline__ Ring(char* smem, const NormParams& p)
+      : ctrl(reinterpret_cast<RingCtrl*>(smem)), slots(smem + kCtrlBytes), sources(0), depth(p.depth), rows(p.rows),
+        slot_bytes(0) {}
+  template <typename E>
+  __device__ __forceinline__ void add(const void* base, long long ld, int cols) {
+    src[sources] = static_cast<const char*>(base);
+    pitch[sources] = ld * static_cast<long long>(sizeof(E));
+    row_bytes[sources] = static_cast<uint32_t>(cols * sizeof(E));
+    offset[sources] = slot_bytes;
+    slot_bytes += ring_row_bytes(cols, sizeof(E));
+    ++sources;
+  }
+  __device__ __forceinline__ long long row_of(int i) const { return blockIdx.x + static_cast<long long>(i) * gridDim.x; }
+  __device__ __forceinline__ void issue(int i) {  // one thread
+    const long long row = row_of(i);
+    if (row >= rows - 1) return;
+    const uint32_t bar = ptx::smem_u32(&ctrl->full[i % depth]);
+    const uint32_t slot = ptx::smem_u32(slots) + (i % depth) * slot_bytes;
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kMaxSources; ++k)
+      if (k < sources) total += span(k, row);
+    ptx::mbar_arrive_expect_tx(bar, total);
+#pragma unroll
+    for (int k = 0; k < kMaxSources; ++k)
+      if (k < sources) {
+        const char* from = src[k] + row * pitch[k];
+        bulk_load(slot + offset[k], from - (reinterpret_cast<uintptr_t>(from) & 15), span(k, row), bar);
+      }
+  }
+  __device__ __forceinline__ uint32_t span(int k, long long row) const {
+    const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + row * pitch[k]) & 15);
+    return (shift + row_bytes[k] + 15) & ~15u;
+  }
+  __device__ __forceinline__ void start() {
+    if (threadIdx.x == 0) {
+      for (int d = 0; d < depth; ++d) ptx::mbar_init(ptx::smem_u32(&ctrl->full[d]), 1);
+      ctrl->abort = 0;
+      ptx::fence_mbar_init();
+      for (int d = 0; d < depth; ++d) issue(d);
+    }
+    __syncthreads();
+  }
+  // Row number i is in its slot (false: it did not come in time).
+  __device__ __forceinline__ bool wait(int i, uint64_t limit_ns) {
+    const long long r = row_of(i);
+    if (r != rows - 1)
+      return ptx::mbar_wait(ptx::smem_u32(&ctrl->full[i % depth]), (i / depth) & 1, &ctrl->abort, limit_ns);
+    // (all threads come here together, and all have left what the slot held before)
+#pragma unroll
+    for (int k = 0; k < kMaxSources; ++k)
+      if (k < sources) {
+        const char* from = src[k] + r * pitch[k];
+        char* to = slots + static_cast<size_t>(i % depth) * slot_bytes + offset[k] + (reinterpret_cast<uintptr_t>(from) & 15);
+        for (uint32_t b = threadIdx.x * 2; b < row_bytes[k]; b += blockDim.x * 2)
+          *reinterpret_cast<uint16_t*>(to + b) = *reinterpret_cast<const uint16_t*>(from + b);
+      }
+    __syncthreads();
+    return true;
+  }
+  // Byte offset of source k's row number i in the slots.
+  __device__ __forceinline__ uint32_t at(int i, int k) const {
+    return (i % depth) * slot_bytes + offset[k] +
+           static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + row_of(i) * pitch[k]) & 15);
+  }
+  // A wait gave up: copies that are still in flight land before shared memory is given back.
+  __device__ __forceinline__ void give_up(int* status) {
+    if (threadIdx.x == 0 && status != nullptr) atomicCAS(status, 0, kAbort);
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+  }
+};
+
+// Weights that every row meets stay in registers: gate * post and pre.
+// PER_ROW: the gate is a row's own (token or full form) and joins post in the row.
+template <typename T, typename W, int VEC, int NV, bool PER_ROW>
+__global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 3 : 1) norm_forward_ring_kernel(const NormParams p) {
+  extern __shared__ __align__(128) char smem[];
+  Ring ring(smem, p);
+  ring.add<T>(p.y, p.ld_y, p.cols);
+  ring.add<T>(p.res, p.ld_res, p.cols);
+  const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
+  if (full) ring.add<W>(p.gate, p.ld_gate, p.cols);
+  ring.start();
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  float pg[NV][VEC];
+  elem::Pack<W, VEC> pre[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int col = (tid + n * threads) * VEC;
+    if (col < p.cols) {
+      elem::load<W, VEC>(static_cast<const W*>(p.post) + col, pg[n]);
+      pre[n] = *reinterpret_cast<const elem::Pack<W, VEC>*>(static_cast<const W*>(p.pre) + col);
+      if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
+        float g[VEC];
+        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) pg[n][j] *= g[j];
+      }
+    }
+  }
+  bool ok = true;
+  for (int i = 0;; ++i) {
+    const long long row = ring.row_of(i);
+    if (row >= p.rows) break;
+    float token = 1.f;
+    if (PER_ROW && !full) token = elem::to_float(static_cast<const W*>(p.gate)[row * p.ld_gate]);
+    ok = ring.wait(i, p.timeout_ns);
+    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 0));
+    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 1));
+    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(i, 2) : 0u));
+    elem::Pack<T, VEC> y[NV];
+    float h[NV][VEC];  // gate * post, then h
+    float ss = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        y[n] = *reinterpret_cast<const elem::Pack<T, VEC>*>(y_row + col);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) ss += elem::to_float(y[n].v[j]) * elem::to_float(y[n].v[j]);
+      }
+    }
+    const float r1 = rsqrtf(block_sum(ss, 0.f, ring.ctrl->sums[0], ok).x * inv_cols + p.eps);
+    if (!ok) break;
+    ss = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        float r[VEC], g[VEC];
+        elem::load<T, VEC>(r_row + col, r);
+        if (full) elem::load<W, VEC>(g_row + col, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float b = elem::to_float(y[n].v[j]) * r1 * pg[n][j];
+          h[n][j] = p.alpha * r[j] + (!PER_ROW ? b : full ? g[j] * b : token * b);
+          ss += h[n][j] * h[n][j];
+        }
+      }
+    }
+    const float r2 = rsqrtf(block_sum(ss, 0.f, ring.ctrl->sums[1], ok).x * inv_cols + p.eps);
+    if (tid == 0) ring.issue(i + p.depth);  // (nobody reads this row's slot any more)
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        float out[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = h[n][j] * r2 * elem::to_float(pre[n].v[j]);
+        const long long at = row * p.cols + col;
+        elem::store<T, VEC>(static_cast<T*>(p.h) + at, h[n]);
+        elem::store<T, VEC>(static_cast<T*>(p.n) + at, out);
+      }
+    }
+    if (p.stats != nullptr && tid == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(r1, r2);
+  }
+  if (!ok) ring.give_up(p.status);
+}
+
+// The sums of norm_backward_kernel.  A gate per channel leaves the sum over rows, so that one sum
+// S = sum of dh' a gives both dpost = gate S and dgate = post S.
+template <typename T, typename W, int VEC, int NV, bool PER_ROW>
+__global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 2 : 1) norm_backward_ring_kernel(const NormParams p) {
+  extern __shared__ __align__(128) char smem[];
+  Ring ring(smem, p);
+  ring.add<T>(p.y, p.ld_y, p.cols);
+  ring.add<T>(p.res, p.ld_res, p.cols);
+  ring.add<T>(p.dh, p.ld_dh, p.cols);
+  ring.add<T>(p.dn, p.ld_dn, p.cols);
+  const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
+  if (full) ring.add<W>(p.gate, p.ld_gate, p.cols);
+  ring.start();
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  float s_a[NV][VEC], s_pre[NV][VEC];  // column sums: dh' a (times the row's gate), dn h r2
+  float pg[NV][VEC];
+  elem::Pack<W, VEC> pre[NV];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int col = (tid + n * threads) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s_a[n][j] = s_pre[n][j] = 0.f;
+    if (col < p.cols) {
+      elem::load<W, VEC>(static_cast<const W*>(p.post) + col, pg[n]);
+      pre[n] = *reinterpret_cast<const elem::Pack<W, VEC>*>(static_cast<const W*>(p.pre) + col);
+      if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
+        float g[VEC];
+        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) pg[n][j] *= g[j];
+      }
+    }
+  }
+  bool ok = true;
+  for (int i = 0;; ++i) {
+    const long long row = ring.row_of(i);
+    if (row >= p.rows) break;
+    const float2 norms = *reinterpret_cast<const float2*>(p.stats + 2 * row);
+    const float r1 = norms.x, r2 = norms.y;
+    float token = 1.f;
+    if (PER_ROW && !full) token = elem::to_float(static_cast<const W*>(p.gate)[row * p.ld_gate]);
+    ok = ring.wait(i, p.timeout_ns);
+    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 0));
+    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 1));
+    const T* dh_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 2));
+    const T* dn_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 3));
+    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(i, 4) : 0u));
+    float h[NV][VEC];
+    elem::Pack<T, VEC> y[NV];
+    float s_uh = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        float g[VEC], u[VEC];
+        y[n] = *reinterpret_cast<const elem::Pack<T, VEC>*>(y_row + col);
+        elem::load<T, VEC>(r_row + col, h[n]);
+        elem::load<T, VEC>(dn_row + col, u);
+        if (full) elem::load<W, VEC>(g_row + col, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float b = elem::to_float(y[n].v[j]) * r1 * pg[n][j];
+          h[n][j] = p.alpha * h[n][j] + (!PER_ROW ? b : full ? g[j] * b : token * b);
+          s_pre[n][j] += u[j] * (h[n][j] * r2);
+          s_uh += u[j] * elem::to_float(pre[n].v[j]) * h[n][j];
+        }
+      }
+    }
+    const float k = block_sum(s_uh, 0.f, ring.ctrl->sums[0], ok).x * inv_cols * r2 * r2;
+    if (!ok) break;
+    float s_va = 0.f, s_g = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        float g[VEC], u[VEC], d[VEC], dg[VEC];
+        elem::load<T, VEC>(dh_row + col, d);
+        elem::load<T, VEC>(dn_row + col, u);
+        if (full) elem::load<W, VEC>(g_row + col, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float a = elem::to_float(y[n].v[j]) * r1;
+          const float dh = d[j] + r2 * (u[j] * elem::to_float(pre[n].v[j]) - h[n][j] * k);
+          const float gate = !PER_ROW ? 1.f : full ? g[j] : token;
+          d[j] = p.alpha * dh;
+          s_a[n][j] += gate * dh * a;
+          if (PER_ROW) {
+            dg[j] = dh * (a * pg[n][j]);
+            s_g += dg[j];
+          }
+          h[n][j] = gate * dh * pg[n][j];  // (v from here on)
+          s_va += h[n][j] * a;
+        }
+        const long long at = row * p.cols + col;
+        elem::store<T, VEC>(static_cast<T*>(p.dres) + at, d);
+        if (full) elem::store<W, VEC>(static_cast<W*>(p.dgate) + at, dg);
+      }
+    }
+    const float2 s = block_sum(s_va, s_g, ring.ctrl->sums[1], ok);
+    if (tid == 0) ring.issue(i + p.depth);  // (nobody reads this row's slot any more)
+    const float m = s.x * inv_cols;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int col = (tid + n * threads) * VEC;
+      if (col < p.cols) {
+        float out[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = r1 * (h[n][j] - elem::to_float(y[n].v[j]) * r1 * m);
+        elem::store<T, VEC>(static_cast<T*>(p.dy) + row * p.cols + col, out);
+      }
+    }
+    if (PER_ROW && !full && tid == 0) static_cast<W*>(p.dgate)[row] = elem::from_float<W>(s.y);
+  }
+  if (!ok) ring.give_up(p.status);
+  float* mine = p.partial + static_cast<long long>(blockIdx.x) * p.sums * p.cols;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int col = (tid + n * threads) * VEC;
+    if (col < p.cols) {
+      if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
+        float g[VEC], post[VEC];
+        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
+        elem::load<W, VEC>(static_cast<const W*>(p.post) + col, post);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          post[j] *= s_a[n][j];
+          s_a[n][j] *= g[j];
+        }
+        elem::store<float, VEC>(mine + 2 * static_cast<long long>(p.cols) + col, post);
+      }
+      elem::store<float, VEC>(mine + col, s_a[n]);
+      elem::store<float, VEC>(mine + p.cols + col, s_pre[n]);
+    }
+  }
+}
+
 // out[s][c] = sum over blocks b of partial[b][s][c], b in a fixed order: 32 columns x 32 strands
 // of blocks per thread block, the strands added pairwise.
 template <typename W>
@@ -279,9 +645,10 @@ __global__ void __launch_bounds__(1024) norm_column_sums(const float* partial, i
 
 inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Vector width, threads and rows of a block for one call.
+// Vector width, vectors per thread, threads and rows of a block for one call; depth > 0: a ring
+// kernel with that many rows in flight and `smem` bytes per block.
 struct NormShape {
-  int vec, nv, threads, rows;
+  int vec, nv, threads, rows, depth, smem, blocks;
 };
 
 // A row's threads: one vector each while a block holds the row, then two, four, ... each.
@@ -289,11 +656,34 @@ void pick_shape(const tnx_norm_problem& p, bool aligned, bool backward, NormShap
   const int wide = p.dtype == TNX_F32 ? 4 : 8;
   s->vec = aligned && p.cols % wide == 0 ? wide : 1;
   const int vectors = cdiv(p.cols, s->vec);
-  const int most = max_threads(s->vec);
+  // Rows in flight: what fits a third (forward) or half (backward) of an SM's shared memory, four
+  // at most; and enough rows that a block has several.
+  const int size = p.dtype == TNX_F32 ? 4 : 2, wsize = p.weight_dtype == TNX_F32 ? 4 : 2;
+  const int slot = (backward ? 4 : 2) * static_cast<int>(ring_row_bytes(p.cols, size)) +
+                   (p.gate_form == TNX_GATE_FULL ? static_cast<int>(ring_row_bytes(p.cols, wsize)) : 0);
+  const int budget = kMaxDynamicSmem / (backward ? 2 : 3) - 1024;
+  s->depth = 0;
+  if (p.rows >= 4 * sm_count()) {
+    s->depth = (budget - kCtrlBytes) / slot;
+    if (s->depth < 2) s->depth = (kMaxDynamicSmem - kCtrlBytes) / slot;
+    if (s->depth > kMaxDepth) s->depth = kMaxDepth;
+    if (s->depth < 2) s->depth = 0;
+  }
   s->nv = 1;
-  while (cdiv(vectors, s->nv) > most) s->nv *= 2;
+  while (cdiv(vectors, s->nv) > max_threads(s->vec, s->nv)) s->nv *= 2;
   s->threads = cdiv(cdiv(vectors, s->nv), 32) * 32;
-  s->rows = backward ? 1 : s->threads >= 256 ? 1 : 256 / s->threads;
+  s->rows = backward || s->depth > 0 ? 1 : s->threads >= 256 ? 1 : 256 / s->threads;
+  s->smem = s->depth > 0 ? kCtrlBytes + s->depth * slot : 0;
+  // Blocks that walk rows: as many as are resident, by shared memory and by threads (at 64
+  // registers forward, 128 backward), never more than there are rows.
+  int per_sm = 2;
+  if (s->depth > 0) {
+    const int by_smem = (kMaxDynamicSmem + 1024) / (s->smem + 1024), by_regs = (backward ? 512 : 768) / s->threads;
+    per_sm = by_smem < by_regs ? by_smem : by_regs;
+    if (per_sm < 1) per_sm = 1;
+    if (per_sm > 8) per_sm = 8;
+  }
+  s->blocks = p.rows < per_sm * sm_count() ? p.rows : per_sm * sm_count();
 }
 
 int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs, int count,
@@ -334,35 +724,77 @@ int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs
 
 using NormFn = void (*)(const NormParams);
 
+// A kernel: plain, or a ring kernel with a gate per row or not.
+struct Pick {
+  bool ring, per_row, backward;
+};
+template <typename T, typename W, int VEC, int NV>
+NormFn pick_form(const Pick& k) {
+  if (!k.ring) return k.backward ? norm_backward_kernel<T, W, VEC, NV> : norm_forward_kernel<T, W, VEC, NV>;
+  if (k.per_row)
+    return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, true> : norm_forward_ring_kernel<T, W, VEC, NV, true>;
+  return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, false> : norm_forward_ring_kernel<T, W, VEC, NV, false>;
+}
 template <typename T, typename W, int VEC>
-NormFn pick_nv(int nv, bool backward) {
-  if (nv == 1) return backward ? norm_backward_kernel<T, W, VEC, 1> : norm_forward_kernel<T, W, VEC, 1>;
-  if (nv == 2) return backward ? norm_backward_kernel<T, W, VEC, 2> : norm_forward_kernel<T, W, VEC, 2>;
-  if (nv == 4) return backward ? norm_backward_kernel<T, W, VEC, 4> : norm_forward_kernel<T, W, VEC, 4>;
-  // (16384 columns: four vectors of eight, eight of four or sixteen single elements)
-  constexpr int kLong = VEC == 8 ? 4 : 8, kLongest = VEC == 1 ? 16 : kLong;
-  if (nv == kLong) return backward ? norm_backward_kernel<T, W, VEC, kLong> : norm_forward_kernel<T, W, VEC, kLong>;
-  if (nv == kLongest)
-    return backward ? norm_backward_kernel<T, W, VEC, kLongest> : norm_forward_kernel<T, W, VEC, kLongest>;
+NormFn pick_nv(int nv, const Pick& k) {
+  if (nv == 1) return pick_form<T, W, VEC, 1>(k);
+  if (nv == 2) return pick_form<T, W, VEC, 2>(k);
+  if (nv == 4) return pick_form<T, W, VEC, 4>(k);
+  // (16384 columns: four vectors of eight, eight of four or 32 single elements)
+  if constexpr (VEC != 8)
+    if (nv == 8) return pick_form<T, W, VEC, 8>(k);
+  if constexpr (VEC == 1) {
+    if (nv == 16) return pick_form<T, W, VEC, 16>(k);
+    if (nv == 32) return pick_form<T, W, VEC, 32>(k);
+  }
   return nullptr;
 }
 template <typename T, typename W, int WIDE>
-NormFn pick_vec(const NormShape& s, bool backward) {
-  return s.vec == 1 ? pick_nv<T, W, 1>(s.nv, backward) : pick_nv<T, W, WIDE>(s.nv, backward);
+NormFn pick_vec(const NormShape& s, const Pick& k) {
+  return s.vec == 1 ? pick_nv<T, W, 1>(s.nv, k) : pick_nv<T, W, WIDE>(s.nv, k);
 }
 NormFn pick_norm(const tnx_norm_problem& p, const NormShape& s, bool backward) {
+  const Pick k = {s.depth > 0, p.gate_form == TNX_GATE_TOKEN || p.gate_form == TNX_GATE_FULL, backward};
   const bool same = p.weight_dtype == p.dtype;
-  if (p.dtype == TNX_F32) return pick_vec<float, float, 4>(s, backward);
+  if (p.dtype == TNX_F32) return pick_vec<float, float, 4>(s, k);
   if (p.dtype == TNX_F16)
-    return same ? pick_vec<__half, __half, 8>(s, backward) : pick_vec<__half, float, 8>(s, backward);
-  return same ? pick_vec<__nv_bfloat16, __nv_bfloat16, 8>(s, backward)
-              : pick_vec<__nv_bfloat16, float, 8>(s, backward);
+    return same ? pick_vec<__half, __half, 8>(s, k) : pick_vec<__half, float, 8>(s, k);
+  return same ? pick_vec<__nv_bfloat16, __nv_bfloat16, 8>(s, k)
+              : pick_vec<__nv_bfloat16, float, 8>(s, k);
 }
 
-// Blocks of the backward pass: two per SM, never more than there are rows.
-int backward_blocks(const tnx_norm_problem& p) {
-  const int most = 2 * sm_count();
-  return p.rows < most ? p.rows : most;
+// The column sums of the backward pass at most: those of the form with the most blocks.
+int most_blocks(const tnx_norm_problem& p) {
+  NormShape plain, ring;
+  pick_shape(p, false, true, &plain);
+  pick_shape(p, true, true, &ring);
+  return plain.blocks > ring.blocks ? plain.blocks : ring.blocks;
+}
+
+// Opts a ring kernel into its dynamic shared memory, once per (kernel, device).
+int allow_smem(NormFn fn, int bytes) {
+  if (bytes <= 48 * 1024) return TNX_OK;
+  constexpr int kSlots = 64;
+  static std::mutex mu;
+  static NormFn fns[kSlots];
+  static int devs[kSlots], used = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) {
+    std::lock_guard<std::mutex> lock(mu);
+    for (int i = 0; i < used; ++i)
+      if (fns[i] == fn && devs[i] == dev) return TNX_OK;
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMaxDynamicSmem);
+    if (e == cudaSuccess && used < kSlots) {
+      fns[used] = fn;
+      devs[used++] = dev;
+    }
+  }
+  if (e == cudaSuccess) return TNX_OK;
+  set_error("gated residual norm: shared memory: %s", cudaGetErrorString(e));
+  (void)cudaGetLastError();
+  return TNX_ERR_CUDA;
 }
 
 int launched(const char* what) {
@@ -380,12 +812,12 @@ extern "C" {
 int64_t tnx_gated_residual_norm_workspace(const tnx_norm_problem* problem) {
   if (problem == nullptr || problem->rows <= 0 || problem->cols <= 0) return 0;
   const int sums = problem->gate_form == TNX_GATE_CHANNEL ? 3 : 2;
-  return static_cast<int64_t>(tnx::backward_blocks(*problem)) * sums * problem->cols * 4;
+  return static_cast<int64_t>(tnx::most_blocks(*problem)) * sums * problem->cols * 4;
 }
 
 int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, const void* residual,
                             const void* post_weight, const void* pre_weight, const void* gate, void* h, void* n,
-                            float* stats, void* stream) {
+                            float* stats, int32_t* status_word, void* stream) {
   using namespace tnx;
   const void* ptrs[] = {y, residual, post_weight, pre_weight, h, n, gate};
   NormShape s;
@@ -426,7 +858,12 @@ int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, cons
     set_error("norm kernel not built for this row length");
     return TNX_ERR_NOT_BUILT;
   }
-  fn<<<cdiv(p.rows, s.rows), dim3(s.threads, s.rows), 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.depth = s.depth;
+  p.status = status_word;
+  p.timeout_ns = bounded_wait_limit_ns();
+  rc = allow_smem(fn, s.smem);
+  if (rc != TNX_OK) return rc;
+  fn<<<s.depth > 0 ? s.blocks : cdiv(p.rows, s.rows), dim3(s.threads, s.rows), s.smem, static_cast<cudaStream_t>(stream)>>>(p);
   return launched("gated residual norm");
 }
 
@@ -434,7 +871,8 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
                                      const void* dn, int64_t stride_dn, const void* y, const void* residual,
                                      const void* post_weight, const void* pre_weight, const void* gate,
                                      const float* stats, void* dy, void* dresidual, void* dpost, void* dpre,
-                                     void* dgate, void* workspace, size_t workspace_bytes, void* stream) {
+                                     void* dgate, void* workspace, size_t workspace_bytes, int32_t* status_word,
+                                     void* stream) {
   using namespace tnx;
   const void* ptrs[] = {dh, dn, y, residual, post_weight, pre_weight, dy, dresidual, gate, dgate};
   NormShape s;
@@ -452,7 +890,7 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
     return TNX_ERR_INVALID;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int blocks = backward_blocks(*problem);
+  const int blocks = s.blocks;
   if (blocks > 0) {
     if (dh == nullptr || dn == nullptr || y == nullptr || residual == nullptr || post_weight == nullptr ||
         pre_weight == nullptr || stats == nullptr || dy == nullptr || dresidual == nullptr ||
@@ -498,7 +936,12 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
       set_error("norm kernel not built for this row length");
       return TNX_ERR_NOT_BUILT;
     }
-    fn<<<blocks, s.threads, 0, st>>>(p);
+    p.depth = s.depth;
+    p.status = status_word;
+    p.timeout_ns = bounded_wait_limit_ns();
+    rc = allow_smem(fn, s.smem);
+    if (rc != TNX_OK) return rc;
+    fn<<<blocks, s.threads, s.smem, st>>>(p);
     rc = launched("gated residual norm, backward");
     if (rc != TNX_OK) return rc;
   }

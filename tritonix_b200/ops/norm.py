@@ -67,7 +67,7 @@ def _forward(plan, y, residual, post, pre, gate, keep_stats):
     _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm, ctypes.byref(plan.problem), y.data_ptr(),
                residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
                gate.data_ptr() if gate is not None else None, h.data_ptr(), n.data_ptr(),
-               stats.data_ptr() if stats is not None else None)
+               stats.data_ptr() if stats is not None else None, _cabi.status_word(y.device).data_ptr())
     return h, n, stats
 
 
@@ -97,7 +97,8 @@ class _GatedResidualNorm(torch.autograd.Function):
                    residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
                    gate.data_ptr() if gate is not None else None, stats.data_ptr(), dy.data_ptr(),
                    dres.data_ptr(), dpost.data_ptr(), dpre.data_ptr(),
-                   dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(), plan.workspace_bytes)
+                   dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(), plan.workspace_bytes,
+                   _cabi.status_word(device).data_ptr())
         return dy, dres, dpost, dpre, dgate, None
 
 
