@@ -286,24 +286,24 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// Sum over the block, and whether `ok` held for every thread.
-__device__ __forceinline__ float2 block_sum(float a, float b, float2* smem, bool& ok) {
+// Sums of N values over the block, and whether `ok` held for every thread.  `levels`: so many times
+// two warps (blockDim.x is up to 32 << levels).
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float2* smem, int levels, bool& ok) {
   const int tid = threadIdx.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if ((tid & 31) == 0) smem[tid >> 5] = make_float2(a, b);
-  ok = __syncthreads_and(ok) != 0;
-  const int warps = blockDim.x >> 5, lane = tid & 31;
-  float2 v = lane < warps ? smem[lane] : make_float2(0.f, 0.f);
+  for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  return v;
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  if ((tid & 31) == 0) smem[tid >> 5] = make_float2(v[0], v[N - 1]);
+  ok = __syncthreads_and(ok) != 0;
+  const int warps = blockDim.x >> 5, lane = tid & ((1 << levels) - 1);
+  const float2 all = lane < warps ? smem[lane] : make_float2(0.f, 0.f);
+  v[0] = all.x;
+  v[N - 1] = N > 1 ? all.y : all.x;
+  for (int o = 1 << levels >> 1; o > 0; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
 }
 
 // The rows a block walks: blockIdx.x, blockIdx.x + gridDim.x, ...  Row number i of them lies in slot
@@ -311,7 +311,9 @@ __device__ __forceinline__ float2 block_sum(float a, float b, float2* smem, bool
 // a row is copied from the boundary at or before its first byte to the one at or after its last;
 // only the very last row of a tensor could be read past its end that way: its block copies it with
 // ordinary loads.
+// MOVED: rows may start anywhere (otherwise all start on 16-byte boundaries).
 constexpr int kMaxSources = 5;
+template <bool MOVED>
 struct Ring {
   RingCtrl* ctrl;
   char* slots;  // (shared memory)
@@ -320,10 +322,12 @@ struct Ring {
   const char* src[kMaxSources];
   long long pitch[kMaxSources];  // bytes
   uint32_t row_bytes[kMaxSources], offset[kMaxSources];
+  int row, slot;  // where the block is
+  uint32_t phase;
 
   __device__ __forceinline__ Ring(char* smem, const NormParams& p)
       : ctrl(reinterpret_cast<RingCtrl*>(smem)), slots(smem + kCtrlBytes), sources(0), depth(p.depth), rows(p.rows),
-        slot_bytes(0) {}
+        slot_bytes(0), row(blockIdx.x), slot(0), phase(0) {}
   template <typename E>
   __device__ __forceinline__ void add(const void* base, long long ld, int cols) {
     src[sources] = static_cast<const char*>(base);
@@ -333,58 +337,60 @@ struct Ring {
     slot_bytes += ring_row_bytes(cols, sizeof(E));
     ++sources;
   }
-  __device__ __forceinline__ long long row_of(int i) const { return blockIdx.x + static_cast<long long>(i) * gridDim.x; }
-  __device__ __forceinline__ void issue(int i) {  // one thread
-    const long long row = row_of(i);
-    if (row >= rows - 1) return;
-    const uint32_t bar = ptx::smem_u32(&ctrl->full[i % depth]);
-    const uint32_t slot = ptx::smem_u32(slots) + (i % depth) * slot_bytes;
+  // By how much source k's row r is moved in its slot, and the bytes its copy has.
+  __device__ __forceinline__ uint32_t shift(int k, long long r) const {
+    return MOVED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + r * pitch[k]) & 15) : 0u;
+  }
+  __device__ __forceinline__ uint32_t span(int k, long long r) const { return (shift(k, r) + row_bytes[k] + 15) & ~15u; }
+  __device__ __forceinline__ void issue(long long r, int to) {  // one thread
+    if (r >= rows || (MOVED && r == rows - 1)) return;
+    const uint32_t bar = ptx::smem_u32(&ctrl->full[to]);
+    const uint32_t at = ptx::smem_u32(slots) + to * slot_bytes;
     uint32_t total = 0;
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
-      if (k < sources) total += span(k, row);
+      if (k < sources) total += span(k, r);
     ptx::mbar_arrive_expect_tx(bar, total);
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
-      if (k < sources) {
-        const char* from = src[k] + row * pitch[k];
-        bulk_load(slot + offset[k], from - (reinterpret_cast<uintptr_t>(from) & 15), span(k, row), bar);
-      }
-  }
-  __device__ __forceinline__ uint32_t span(int k, long long row) const {
-    const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + row * pitch[k]) & 15);
-    return (shift + row_bytes[k] + 15) & ~15u;
+      if (k < sources) bulk_load(at + offset[k], src[k] + r * pitch[k] - shift(k, r), span(k, r), bar);
   }
   __device__ __forceinline__ void start() {
     if (threadIdx.x == 0) {
       for (int d = 0; d < depth; ++d) ptx::mbar_init(ptx::smem_u32(&ctrl->full[d]), 1);
       ctrl->abort = 0;
       ptx::fence_mbar_init();
-      for (int d = 0; d < depth; ++d) issue(d);
+      for (int d = 0; d < depth; ++d) issue(row + static_cast<long long>(d) * gridDim.x, d);
     }
     __syncthreads();
   }
-  // Row number i is in its slot (false: it did not come in time).
-  __device__ __forceinline__ bool wait(int i, uint64_t limit_ns) {
-    const long long r = row_of(i);
-    if (r != rows - 1)
-      return ptx::mbar_wait(ptx::smem_u32(&ctrl->full[i % depth]), (i / depth) & 1, &ctrl->abort, limit_ns);
+  // The block's row is in its slot (false: it did not come in time).
+  __device__ __forceinline__ bool wait(uint64_t limit_ns) {
+    if (!MOVED || row != rows - 1) return ptx::mbar_wait(ptx::smem_u32(&ctrl->full[slot]), phase, &ctrl->abort, limit_ns);
     // (all threads come here together, and all have left what the slot held before)
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
       if (k < sources) {
-        const char* from = src[k] + r * pitch[k];
-        char* to = slots + static_cast<size_t>(i % depth) * slot_bytes + offset[k] + (reinterpret_cast<uintptr_t>(from) & 15);
+        const char* from = src[k] + row * pitch[k];
+        char* to = slots + static_cast<size_t>(slot) * slot_bytes + offset[k] + shift(k, row);
         for (uint32_t b = threadIdx.x * 2; b < row_bytes[k]; b += blockDim.x * 2)
           *reinterpret_cast<uint16_t*>(to + b) = *reinterpret_cast<const uint16_t*>(from + b);
       }
     __syncthreads();
     return true;
   }
-  // Byte offset of source k's row number i in the slots.
-  __device__ __forceinline__ uint32_t at(int i, int k) const {
-    return (i % depth) * slot_bytes + offset[k] +
-           static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + row_of(i) * pitch[k]) & 15);
+  // Byte offset of source k's row in the slots.
+  __device__ __forceinline__ uint32_t at(int k) const { return slot * slot_bytes + offset[k] + shift(k, row); }
+  // Nobody reads the row's slot any more: it takes the row `depth` rounds ahead.
+  __device__ __forceinline__ void refill() {
+    if (threadIdx.x == 0) issue(row + static_cast<long long>(depth) * gridDim.x, slot);
+  }
+  __device__ __forceinline__ void next() {
+    row += gridDim.x;
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1u;
+    }
   }
   // A wait gave up: copies that are still in flight land before shared memory is given back.
   __device__ __forceinline__ void give_up(int* status) {
@@ -399,11 +405,11 @@ struct Ring {
 template <typename T, typename W, int VEC, int NV, bool PER_ROW>
 __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 3 : 1) norm_forward_ring_kernel(const NormParams p) {
   extern __shared__ __align__(128) char smem[];
-  Ring ring(smem, p);
-  ring.add<T>(p.y, p.ld_y, p.cols);
-  ring.add<T>(p.res, p.ld_res, p.cols);
+  Ring<VEC == 1> ring(smem, p);
+  ring.template add<T>(p.y, p.ld_y, p.cols);
+  ring.template add<T>(p.res, p.ld_res, p.cols);
   const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
-  if (full) ring.add<W>(p.gate, p.ld_gate, p.cols);
+  if (full) ring.template add<W>(p.gate, p.ld_gate, p.cols);
   ring.start();
   const int tid = threadIdx.x, threads = blockDim.x;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
@@ -423,31 +429,34 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
       }
     }
   }
+  int levels = 0;
+  while ((32 << levels) < threads) ++levels;
   bool ok = true;
-  for (int i = 0;; ++i) {
-    const long long row = ring.row_of(i);
-    if (row >= p.rows) break;
+  // (rows <= 2^30: row numbers cannot overflow)
+  for (; ring.row < p.rows; ring.next()) {
+    const long long row = ring.row;
     float token = 1.f;
     if (PER_ROW && !full) token = elem::to_float(static_cast<const W*>(p.gate)[row * p.ld_gate]);
-    ok = ring.wait(i, p.timeout_ns);
-    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 0));
-    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 1));
-    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(i, 2) : 0u));
+    ok = ring.wait(p.timeout_ns);
+    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(0));
+    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(1));
+    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(2) : 0u));
     elem::Pack<T, VEC> y[NV];
     float h[NV][VEC];  // gate * post, then h
-    float ss = 0.f;
+    float ss[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int col = (tid + n * threads) * VEC;
       if (col < p.cols) {
         y[n] = *reinterpret_cast<const elem::Pack<T, VEC>*>(y_row + col);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) ss += elem::to_float(y[n].v[j]) * elem::to_float(y[n].v[j]);
+        for (int j = 0; j < VEC; ++j) ss[0] += elem::to_float(y[n].v[j]) * elem::to_float(y[n].v[j]);
       }
     }
-    const float r1 = rsqrtf(block_sum(ss, 0.f, ring.ctrl->sums[0], ok).x * inv_cols + p.eps);
+    block_sum(ss, ring.ctrl->sums[0], levels, ok);
     if (!ok) break;
-    ss = 0.f;
+    const float r1 = rsqrtf(ss[0] * inv_cols + p.eps);
+    ss[0] = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int col = (tid + n * threads) * VEC;
@@ -459,12 +468,13 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
         for (int j = 0; j < VEC; ++j) {
           const float b = elem::to_float(y[n].v[j]) * r1 * pg[n][j];
           h[n][j] = p.alpha * r[j] + (!PER_ROW ? b : full ? g[j] * b : token * b);
-          ss += h[n][j] * h[n][j];
+          ss[0] += h[n][j] * h[n][j];
         }
       }
     }
-    const float r2 = rsqrtf(block_sum(ss, 0.f, ring.ctrl->sums[1], ok).x * inv_cols + p.eps);
-    if (tid == 0) ring.issue(i + p.depth);  // (nobody reads this row's slot any more)
+    block_sum(ss, ring.ctrl->sums[1], levels, ok);
+    const float r2 = rsqrtf(ss[0] * inv_cols + p.eps);
+    ring.refill();
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int col = (tid + n * threads) * VEC;
@@ -487,13 +497,13 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
 template <typename T, typename W, int VEC, int NV, bool PER_ROW>
 __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 2 : 1) norm_backward_ring_kernel(const NormParams p) {
   extern __shared__ __align__(128) char smem[];
-  Ring ring(smem, p);
-  ring.add<T>(p.y, p.ld_y, p.cols);
-  ring.add<T>(p.res, p.ld_res, p.cols);
-  ring.add<T>(p.dh, p.ld_dh, p.cols);
-  ring.add<T>(p.dn, p.ld_dn, p.cols);
+  Ring<VEC == 1> ring(smem, p);
+  ring.template add<T>(p.y, p.ld_y, p.cols);
+  ring.template add<T>(p.res, p.ld_res, p.cols);
+  ring.template add<T>(p.dh, p.ld_dh, p.cols);
+  ring.template add<T>(p.dn, p.ld_dn, p.cols);
   const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
-  if (full) ring.add<W>(p.gate, p.ld_gate, p.cols);
+  if (full) ring.template add<W>(p.gate, p.ld_gate, p.cols);
   ring.start();
   const int tid = threadIdx.x, threads = blockDim.x;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
@@ -516,23 +526,25 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
       }
     }
   }
+  int levels = 0;
+  while ((32 << levels) < threads) ++levels;
   bool ok = true;
-  for (int i = 0;; ++i) {
-    const long long row = ring.row_of(i);
-    if (row >= p.rows) break;
+  // (rows <= 2^30: row numbers cannot overflow)
+  for (; ring.row < p.rows; ring.next()) {
+    const long long row = ring.row;
     const float2 norms = *reinterpret_cast<const float2*>(p.stats + 2 * row);
     const float r1 = norms.x, r2 = norms.y;
     float token = 1.f;
     if (PER_ROW && !full) token = elem::to_float(static_cast<const W*>(p.gate)[row * p.ld_gate]);
-    ok = ring.wait(i, p.timeout_ns);
-    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 0));
-    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 1));
-    const T* dh_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 2));
-    const T* dn_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(i, 3));
-    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(i, 4) : 0u));
+    ok = ring.wait(p.timeout_ns);
+    const T* y_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(0));
+    const T* r_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(1));
+    const T* dh_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(2));
+    const T* dn_row = reinterpret_cast<const T*>(smem + kCtrlBytes + ring.at(3));
+    const W* g_row = reinterpret_cast<const W*>(smem + kCtrlBytes + (full ? ring.at(4) : 0u));
     float h[NV][VEC];
     elem::Pack<T, VEC> y[NV];
-    float s_uh = 0.f;
+    float s_uh[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int col = (tid + n * threads) * VEC;
@@ -547,12 +559,13 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
           const float b = elem::to_float(y[n].v[j]) * r1 * pg[n][j];
           h[n][j] = p.alpha * h[n][j] + (!PER_ROW ? b : full ? g[j] * b : token * b);
           s_pre[n][j] += u[j] * (h[n][j] * r2);
-          s_uh += u[j] * elem::to_float(pre[n].v[j]) * h[n][j];
+          s_uh[0] += u[j] * elem::to_float(pre[n].v[j]) * h[n][j];
         }
       }
     }
-    const float k = block_sum(s_uh, 0.f, ring.ctrl->sums[0], ok).x * inv_cols * r2 * r2;
+    block_sum(s_uh, ring.ctrl->sums[0], levels, ok);
     if (!ok) break;
+    const float k = s_uh[0] * inv_cols * r2 * r2;
     float s_va = 0.f, s_g = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
@@ -581,9 +594,11 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
         if (full) elem::store<W, VEC>(static_cast<W*>(p.dgate) + at, dg);
       }
     }
-    const float2 s = block_sum(s_va, s_g, ring.ctrl->sums[1], ok);
-    if (tid == 0) ring.issue(i + p.depth);  // (nobody reads this row's slot any more)
-    const float m = s.x * inv_cols;
+    float both[PER_ROW ? 2 : 1] = {s_va};
+    if (PER_ROW) both[PER_ROW ? 1 : 0] = s_g;
+    block_sum(both, ring.ctrl->sums[1], levels, ok);
+    ring.refill();
+    const float m = both[0] * inv_cols;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int col = (tid + n * threads) * VEC;
@@ -594,7 +609,7 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
         elem::store<T, VEC>(static_cast<T*>(p.dy) + row * p.cols + col, out);
       }
     }
-    if (PER_ROW && !full && tid == 0) static_cast<W*>(p.dgate)[row] = elem::from_float<W>(s.y);
+    if (PER_ROW && !full && tid == 0) static_cast<W*>(p.dgate)[row] = elem::from_float<W>(both[PER_ROW ? 1 : 0]);
   }
   if (!ok) ring.give_up(p.status);
   float* mine = p.partial + static_cast<long long>(blockIdx.x) * p.sums * p.cols;
@@ -692,8 +707,8 @@ int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs
     set_error("problem is NULL");
     return TNX_ERR_INVALID;
   }
-  if (p->rows < 0 || p->cols < 1 || p->cols > kMaxCols) {
-    set_error("the norm needs rows >= 0 and 1 <= cols <= %d (got %d x %d)", kMaxCols, p->rows, p->cols);
+  if (p->rows < 0 || p->rows > (1 << 30) || p->cols < 1 || p->cols > kMaxCols) {
+    set_error("the norm needs 0 to 2^30 rows and 1 <= cols <= %d (got %d x %d)", kMaxCols, p->rows, p->cols);
     return TNX_ERR_INVALID;
   }
   if (p->dtype < TNX_F16 || p->dtype > TNX_F32 || (p->weight_dtype != p->dtype && p->weight_dtype != TNX_F32)) {

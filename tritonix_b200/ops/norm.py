@@ -155,6 +155,6 @@ def _check(y, residual, post_weight, pre_weight, gate, eps) -> int:
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps}")
     rows = y.numel() // cols
-    if rows >= 1 << 31:
+    if rows > 1 << 30:
         raise ValueError("too many rows")
     return _gate_form(gate, rows, cols, lead)
