@@ -7,10 +7,12 @@
 //     w = scale * s[ids] (/ sum of s[ids] when renormalised)
 //
 // One warp per token: a token's experts are spread over the lanes (expert j*32 + lane in register
-// j), scores never leave the registers, and a pick is one unsigned maximum over the warp
-// (order-preserving integer keys, redux.sync) and one minimum over the indices that reach it.
-// Forward reads each logit once and writes top_k weights and ids.  At 32768 tokens x 256 experts
-// this is 36 MB, but the picks' instructions, not the bytes, bound the kernel.
+// j).  A lane sorts its own experts once (64-bit keys: the choice's order-preserving integer above,
+// the expert's number below); a pick then is the largest of the lanes' heads (two redux.sync), and
+// the lane that had it moves up its list.  Forward reads each logit once and writes top_k weights
+// and ids.  At 32768 tokens x 256 experts in 8 groups this is 36 MB (5.5 us at the measured copy
+// rate), but instructions bound the kernel: some 1000 per token, after 2100 with a search of all
+// registers for every pick (105 us).
 //
 // Which experts are chosen must not depend on how an exponential is rounded.  Without a bias the
 // logits themselves order the experts exactly.  With a bias or with groups the fp32 choices carry
@@ -33,6 +35,7 @@ constexpr unsigned kAll = 0xffffffffu;
 
 struct RouteParams {
   int tokens, experts, top_k, groups, top_groups, scoring, renormalize;
+  unsigned group_size, group_inv;  // experts of a group; ceil(2^20 / group_size): e / group_size = e * inv >> 20
   float scale;
   long long ld;  // row pitch of the logits in elements
   const void* logits;
@@ -150,6 +153,11 @@ __device__ __forceinline__ unsigned open_groups(const F* c, int groups, int size
   return open;
 }
 
+// The group of expert e < 512 (with one group its number is not asked for: all bits are set).
+__device__ __forceinline__ unsigned group_of(const RouteParams& p, int e) {
+  return p.groups == 1 ? 0u : static_cast<unsigned>(e) * p.group_inv >> 20;
+}
+
 // The same choice in 64 bits, for tokens that fp32 cannot tell apart.  Returns pick `lane`'s expert.
 template <int VPT>
 __device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RouteParams& p, int lane, float row_max,
@@ -157,7 +165,6 @@ __device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RoutePar
   double c[VPT];
   scores<double, VPT>(l, p.experts, lane, p.scoring == TNX_SCORE_SOFTMAX, row_max, c);
   unsigned open = kAll;
-  const int size = p.experts / p.groups;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int e = j * 32 + lane;
@@ -169,14 +176,14 @@ __device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RoutePar
       if (j * 32 + lane < p.experts) shared[j * 32 + lane] = c[j];
     __syncwarp();
     double gap;
-    open = open_groups(shared, p.groups, size, p.top_groups, lane, &gap);
+    open = open_groups(shared, p.groups, static_cast<int>(p.group_size), p.top_groups, lane, &gap);
     __syncwarp();
   }
   unsigned long long key[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int e = j * 32 + lane;
-    key[j] = e < p.experts && ((p.groups == 1) || ((open >> (e / size)) & 1u)) ? order_key(c[j]) : 0ull;
+    key[j] = e < p.experts && ((open >> group_of(p, e)) & 1u) ? order_key(c[j]) : 0ull;
   }
   int mine = 0;
   for (int i = 0; i < p.top_k; ++i) {
@@ -198,123 +205,135 @@ __device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RoutePar
   return mine;
 }
 
+// Sorts a lane's keys, largest first (Batcher's odd-even merge sort, unrolled).
+template <int N>
+__device__ __forceinline__ void sort_keys(unsigned long long (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const unsigned long long a = k[i + j], b = k[i + j + q];
+            k[i + j] = a > b ? a : b;
+            k[i + j + q] = a > b ? b : a;
+          }
+}
+
 template <typename T, int VPT>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(const RouteParams p) {
+  // Per warp: logits and choices by expert, or the exact choices of a token that needs them.
   __shared__ double shared[kWarps][VPT * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int token = blockIdx.x * kWarps + warp;
   if (token >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + token * p.ld;
-  float l[VPT], s[VPT];
-  float row_max = -CUDART_INF_F;
+  float* sh_logit = reinterpret_cast<float*>(shared[warp]);
+  float* sh_choice = sh_logit + VPT * 32;
+  float l[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int e = j * 32 + lane;
     l[j] = e < p.experts ? elem::to_float(row[e]) : -CUDART_INF_F;
-    row_max = fmaxf(row_max, l[j]);
   }
-  row_max = warp_max(row_max);
   const bool softmax = p.scoring == TNX_SCORE_SOFTMAX;
-  scores<float, VPT>(l, p.experts, lane, softmax, row_max, s);
-
-  // Choices and the largest error any of them can have: expf, the division and the sum are good
-  // to a few units in the last place (2^-19 relative covers them), l - max is rounded (an error of
-  // |l - max| 2^-24 in the exponent), and so is the addition of the bias.
-  unsigned key[VPT];
+  float row_max = -CUDART_INF_F, top_score = 1.f;
+  if (softmax) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) row_max = fmaxf(row_max, l[j]);
+    row_max = warp_max(row_max);
+  }
+  unsigned long long key[VPT];
   float eps = 0.f;
   unsigned open = kAll;
   bool unsure = false;
-  const int size = p.experts / p.groups;
   {
     float c[VPT];
+    scores<float, VPT>(l, p.experts, lane, softmax, row_max, c);
+    if (softmax) {
+      top_score = c[0];
+#pragma unroll
+      for (int j = 1; j < VPT; ++j) top_score = fmaxf(top_score, c[j]);
+      top_score = warp_max(top_score);
+    }
+    float far = 0.f;  // largest |bias|
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int e = j * 32 + lane;
-      c[j] = s[j];
-      if (e < p.experts) {
-        if (p.bias != nullptr) c[j] += p.bias[e];
-        const float far = softmax && s[j] > 0.f ? (row_max - l[j]) * 1.2e-7f : 0.f;
-        const float err = s[j] * (1.9e-6f + far) + fabsf(c[j]) * 1.2e-7f;
-        eps = fmaxf(eps, err);
+      sh_logit[e] = l[j];
+      if (p.bias != nullptr && e < p.experts) {
+        const float b = p.bias[e];
+        c[j] += b;
+        far = fmaxf(far, fabsf(b));
       }
+      if (p.groups > 1) sh_choice[e] = c[j];
     }
-    eps = warp_max(eps) + 1e-37f;
+    __syncwarp();
+    // The largest error a choice can have.  expf, the division and the sum are good to a few units in
+    // the last place (2^-19 of the score covers them).  l - max is rounded: an error of |l - max|
+    // 2^-24 in the exponent, and the score is at most exp(l - max), so at most 2^-25 in all.  The
+    // addition of the bias rounds once more.
+    if (p.bias != nullptr) far = warp_max(far);
+    eps = 1.91e-6f * top_score + 3e-8f + 6e-8f * (top_score + far);
     if (p.groups > 1) {
-      float* sh = reinterpret_cast<float*>(shared[warp]);
-#pragma unroll
-      for (int j = 0; j < VPT; ++j)
-        if (j * 32 + lane < p.experts) sh[j * 32 + lane] = c[j];
-      __syncwarp();
       float gap;
-      open = open_groups(sh, p.groups, size, p.top_groups, lane, &gap);
+      open = open_groups(sh_choice, p.groups, static_cast<int>(p.group_size), p.top_groups, lane, &gap);
       unsure = !(gap > 4.f * eps);  // (two choices on each side)
-      __syncwarp();
     }
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int e = j * 32 + lane;
-      const bool can = e < p.experts && ((p.groups == 1) || ((open >> (e / size)) & 1u));
-      key[j] = can ? order_key(p.bias != nullptr ? c[j] : l[j]) : 0u;
+      const bool can = e < p.experts && ((open >> group_of(p, e)) & 1u);
+      key[j] = can ? (static_cast<unsigned long long>(order_key(p.bias != nullptr ? c[j] : l[j])) << 32) |
+                         (0xffffffffu - static_cast<unsigned>(e))
+                   : 0ull;
     }
   }
+  sort_keys<VPT>(key);
 
-  int mine = 0;        // pick `lane`
-  float my_logit = 0.f, my_score = 0.f;
-  float last = 0.f, last_logit = 0.f, last_bias = 0.f;
+  int mine = 0;  // pick `lane`
+  float last = 0.f;
+  int last_e = 0;
   const int rounds = p.top_k + (p.bias != nullptr ? 1 : 0);  // one more to see the best that is left out
   for (int i = 0; i < rounds && !unsure; ++i) {
-    unsigned best = 0;
-    int at = kMaxExperts;
-#pragma unroll
-    for (int j = VPT - 1; j >= 0; --j)
-      if (key[j] >= best) {
-        best = key[j];
-        at = j * 32 + lane;
-      }
-    const unsigned top = warp_key_max(best);
+    const unsigned long long top = warp_key_max(key[0]);
     if (top == 0) break;  // (only past the last pick: nothing is left out)
-    const int e = __reduce_min_sync(kAll, best == top ? static_cast<unsigned>(at) : static_cast<unsigned>(kMaxExperts));
-    float el = 0.f, es = 0.f;
+    const int e = static_cast<int>(0xffffffffu - static_cast<unsigned>(top));
+    if (key[0] == top) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      if (e == j * 32 + lane) {
-        el = l[j];
-        es = s[j];
-        key[j] = 0;
-      }
-    el = __shfl_sync(kAll, el, e & 31);
-    es = __shfl_sync(kAll, es, e & 31);
+      for (int j = 0; j + 1 < VPT; ++j) key[j] = key[j + 1];
+      key[VPT - 1] = 0ull;
+    }
     if (p.bias != nullptr) {
-      const float v = key_value(top), b = p.bias[e];
-      if (i > 0 && !(last - v > 2.f * eps)) unsure = !(el == last_logit && b == last_bias);
+      const float v = key_value(static_cast<unsigned>(top >> 32));
+      // (copies of one another are in order already)
+      if (i > 0 && !(last - v > 2.f * eps))
+        unsure = !(sh_logit[e] == sh_logit[last_e] && p.bias[e] == p.bias[last_e]);
       last = v;
-      last_logit = el;
-      last_bias = b;
+      last_e = e;
     }
-    if (lane == i) {
-      mine = e;
-      my_logit = el;
-      my_score = es;
-    }
+    if (lane == i) mine = e;
   }
+  float my_logit, my_score;
   if (unsure) {
-    mine = choose_exactly<VPT>(l, p, lane, row_max, shared[warp]);
-    for (int i = 0; i < p.top_k; ++i) {
-      const int e = __shfl_sync(kAll, mine, i);
-      float el = 0.f, es = 0.f;
 #pragma unroll
-      for (int j = 0; j < VPT; ++j)
-        if (e == j * 32 + lane) {
-          el = l[j];
-          es = s[j];
-        }
-      el = __shfl_sync(kAll, el, e & 31);
-      es = __shfl_sync(kAll, es, e & 31);
-      if (lane == i) {
-        my_logit = el;
-        my_score = es;
-      }
-    }
+    for (int j = 0; j < VPT; ++j) l[j] = sh_logit[j * 32 + lane];
+    __syncwarp();
+    mine = choose_exactly<VPT>(l, p, lane, row_max, shared[warp]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) sh_logit[j * 32 + lane] = l[j];
+    __syncwarp();
+  }
+  my_logit = sh_logit[mine];
+  if (softmax) {
+    // (top_score = exp(0) / sum: the other scores relative to it)
+    my_score = row_max == -CUDART_INF_F ? 0.f : expf(my_logit - row_max) * top_score;
+  } else {
+    my_score = 1.f / (1.f + expf(-my_logit));
   }
 
   const bool picked = lane < p.top_k;
@@ -483,6 +502,8 @@ RouteParams route_params(const tnx_route_problem& q) {
   // (all groups open: the groups decide nothing)
   p.groups = q.top_groups == q.groups ? 1 : q.groups;
   p.top_groups = q.top_groups == q.groups ? 1 : q.top_groups;
+  p.group_size = static_cast<unsigned>(q.experts / p.groups);
+  p.group_inv = ((1u << 20) + p.group_size - 1) / p.group_size;
   p.scoring = q.scoring;
   p.renormalize = q.renormalize;
   p.scale = q.scale;
