@@ -62,9 +62,9 @@ __device__ __forceinline__ F warp_sum(F v) {
 
 // Integers in the order of the floats: NaN below everything, 0 is kept for "cannot be chosen".
 __device__ __forceinline__ unsigned order_key(float v) {
-  if (v != v) return 1u;
-  const unsigned u = __float_as_uint(v + 0.f);  // (-0 becomes +0)
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const int u = __float_as_int(v + 0.f);  // (-0 becomes +0)
+  const unsigned k = static_cast<unsigned>(u ^ ((u >> 31) | static_cast<int>(0x80000000u)));
+  return v != v ? 1u : k;
 }
 __device__ __forceinline__ float key_value(unsigned k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
@@ -103,19 +103,43 @@ __device__ __forceinline__ void scores(const float (&l)[VPT], int experts, int l
   }
 }
 
+// Scores that only take part in the choice: fast exponential and division (see the bound on their
+// error in route_kernel).
+template <int VPT>
+__device__ __forceinline__ void quick_scores(const float (&l)[VPT], int experts, int lane, bool softmax, float row_max,
+                                             float (&s)[VPT]) {
+  if (softmax) {
+    float sum = 0.f;
+    const float top = row_max == -CUDART_INF_F ? 0.f : row_max;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      s[j] = j * 32 + lane < experts ? __expf(l[j] - top) : 0.f;
+      sum += s[j];
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) s[j] *= inv;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) s[j] = __fdividef(1.f, 1.f + __expf(-l[j]));
+  }
+}
+
 // Which groups stay open, as a bit mask the whole warp agrees on, by the sum of each group's two
 // best choices (its only one in a group of one).  `c` is the warp's shared copy of the choices.
 // Lanes are dealt out to the groups in equal numbers of a power of two.  *gap: how far the worst
 // open group is from the best closed one (infinite when no group is closed).
 template <typename F>
 __device__ __forceinline__ unsigned open_groups(const F* c, int groups, int size, int top_groups, int lane, F* gap) {
-  int share = 1;
-  while (share * 2 * groups <= 32) share *= 2;
-  const int g = lane / share;
+  int bits = 0;
+  while ((2 << bits) * groups <= 32) ++bits;
+  const int share = 1 << bits;
+  const int g = lane >> bits;
   const F low = static_cast<F>(-CUDART_INF_F);
   F first = low, second = low;
   if (g < groups)
-    for (int i = lane % share; i < size; i += share) {
+    for (int i = lane & (share - 1); i < size; i += share) {
       const F v = c[g * size + i];
       if (v > first) {
         second = first;
@@ -159,9 +183,13 @@ __device__ __forceinline__ unsigned group_of(const RouteParams& p, int e) {
 }
 
 // The same choice in 64 bits, for tokens that fp32 cannot tell apart.  Returns pick `lane`'s expert.
+// `logits` and `shared` are the warp's, and do not overlap.
 template <int VPT>
-__device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RouteParams& p, int lane, float row_max,
+__device__ __noinline__ int choose_exactly(const float* logits, const RouteParams& p, int lane, float row_max,
                                            double* shared) {
+  float l[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) l[j] = logits[j * 32 + lane];
   double c[VPT];
   scores<double, VPT>(l, p.experts, lane, p.scoring == TNX_SCORE_SOFTMAX, row_max, c);
   unsigned open = kAll;
@@ -205,54 +233,62 @@ __device__ __noinline__ int choose_exactly(const float (&l)[VPT], const RoutePar
   return mine;
 }
 
-// Sorts a lane's keys, largest first (Batcher's odd-even merge sort, unrolled).
+// Sorts a lane's keys, largest first (Batcher's odd-even merge sort).  Every loop has a constant
+// trip count and every comparison of indices folds, so that the keys stay in registers.
 template <int N>
 __device__ __forceinline__ void sort_keys(unsigned long long (&k)[N]) {
 #pragma unroll
-  for (int p = 1; p < N; p *= 2)
+  for (int lp = 0; (1 << lp) < N; ++lp) {
 #pragma unroll
-    for (int q = p; q >= 1; q /= 2)
+    for (int lq = lp; lq >= 0; --lq) {
+      const int p = 1 << lp, q = 1 << lq;
 #pragma unroll
-      for (int j = q % p; j + q < N; j += 2 * q)
-#pragma unroll
-        for (int i = 0; i < q; ++i)
-          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
-            const unsigned long long a = k[i + j], b = k[i + j + q];
-            k[i + j] = a > b ? a : b;
-            k[i + j + q] = a > b ? b : a;
-          }
+      for (int t = 0; t + q < N; ++t) {
+        const int from = q % p;  // merges start here: the first element of a run, or past its first q
+        if (t >= from && (t - from) % (2 * q) < q && t / (2 * p) == (t + q) / (2 * p)) {
+          const unsigned long long a = k[t], b = k[t + q];
+          k[t] = a > b ? a : b;
+          k[t + q] = a > b ? b : a;
+        }
+      }
+    }
+  }
 }
 
 template <typename T, int VPT>
-__global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(const RouteParams p) {
-  // Per warp: logits and choices by expert, or the exact choices of a token that needs them.
+__global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(const __grid_constant__ RouteParams p) {
+  // Per warp: the logits by expert, and the choices (as doubles for a token that needs them exact).
+  __shared__ float logits[kWarps][VPT * 32];
   __shared__ double shared[kWarps][VPT * 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int token = blockIdx.x * kWarps + warp;
   if (token >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + token * p.ld;
-  float* sh_logit = reinterpret_cast<float*>(shared[warp]);
-  float* sh_choice = sh_logit + VPT * 32;
+  float* sh_logit = logits[warp];
+  float* sh_choice = reinterpret_cast<float*>(shared[warp]);
+  // (no branches in the unrolled loops: experts that do not exist are read at the last one)
   float l[VPT];
 #pragma unroll
+  for (int j = 0; j < VPT; ++j) l[j] = elem::to_float(row[min(j * 32 + lane, p.experts - 1)]);
+#pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int e = j * 32 + lane;
-    l[j] = e < p.experts ? elem::to_float(row[e]) : -CUDART_INF_F;
+    if (j * 32 + lane >= p.experts) l[j] = -CUDART_INF_F;
+    sh_logit[j * 32 + lane] = l[j];
   }
-  const bool softmax = p.scoring == TNX_SCORE_SOFTMAX;
-  float row_max = -CUDART_INF_F, top_score = 1.f;
+  const bool softmax = p.scoring == TNX_SCORE_SOFTMAX, biased = p.bias != nullptr;
+  float row_max = -CUDART_INF_F;
   if (softmax) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) row_max = fmaxf(row_max, l[j]);
     row_max = warp_max(row_max);
   }
-  unsigned long long key[VPT];
   float eps = 0.f;
   unsigned open = kAll;
   bool unsure = false;
-  {
+  if (biased || p.groups > 1) {  // (otherwise the logits order the experts)
     float c[VPT];
-    scores<float, VPT>(l, p.experts, lane, softmax, row_max, c);
+    quick_scores<VPT>(l, p.experts, lane, softmax, row_max, c);
+    float top_score = 1.f;
     if (softmax) {
       top_score = c[0];
 #pragma unroll
@@ -260,44 +296,53 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       top_score = warp_max(top_score);
     }
     float far = 0.f;  // largest |bias|
+    if (biased) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int e = j * 32 + lane;
-      sh_logit[e] = l[j];
-      if (p.bias != nullptr && e < p.experts) {
-        const float b = p.bias[e];
+      for (int j = 0; j < VPT; ++j) {
+        const float b = p.bias[min(j * 32 + lane, p.experts - 1)];
         c[j] += b;
         far = fmaxf(far, fabsf(b));
       }
-      if (p.groups > 1) sh_choice[e] = c[j];
+      far = warp_max(far);
     }
-    __syncwarp();
-    // The largest error a choice can have.  expf, the division and the sum are good to a few units in
-    // the last place (2^-19 of the score covers them).  l - max is rounded: an error of |l - max|
-    // 2^-24 in the exponent, and the score is at most exp(l - max), so at most 2^-25 in all.  The
-    // addition of the bias rounds once more.
-    if (p.bias != nullptr) far = warp_max(far);
-    eps = 1.91e-6f * top_score + 3e-8f + 6e-8f * (top_score + far);
+    // The largest error a choice can have.  Relative to the score: the exponential, the division and
+    // the sum are good to a few units in the last place each, 2^-19 together.  Rounding x = l - max
+    // (or -l) and its product with log2(e) puts an error of 2 |x| 2^-24 into the exponent; score times
+    // |x| is at most 0.37 (softmax, where the score is at most exp(x)) or 0.28 (sigmoid, whose
+    // derivative is s (1 - s)): 1.2e-7 is more than twice that.  The bias's addition rounds once more.
+    eps = 1.91e-6f * top_score + 1.2e-7f + 6e-8f * (top_score + far);
     if (p.groups > 1) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) sh_choice[j * 32 + lane] = c[j];
+      __syncwarp();
       float gap;
       open = open_groups(sh_choice, p.groups, static_cast<int>(p.group_size), p.top_groups, lane, &gap);
       unsure = !(gap > 4.f * eps);  // (two choices on each side)
     }
+    if (biased) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int e = j * 32 + lane;
-      const bool can = e < p.experts && ((open >> group_of(p, e)) & 1u);
-      key[j] = can ? (static_cast<unsigned long long>(order_key(p.bias != nullptr ? c[j] : l[j])) << 32) |
-                         (0xffffffffu - static_cast<unsigned>(e))
-                   : 0ull;
+      for (int j = 0; j < VPT; ++j) l[j] = c[j];
     }
+  }
+  __syncwarp();
+  unsigned long long key[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int e = j * 32 + lane;
+    key[j] = (static_cast<unsigned long long>(order_key(l[j])) << 32) | (0xffffffffu - static_cast<unsigned>(e));
+    if (e >= p.experts) key[j] = 0ull;
+  }
+  if (p.groups > 1) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+      if (!((open >> group_of(p, j * 32 + lane)) & 1u)) key[j] = 0ull;
   }
   sort_keys<VPT>(key);
 
   int mine = 0;  // pick `lane`
   float last = 0.f;
   int last_e = 0;
-  const int rounds = p.top_k + (p.bias != nullptr ? 1 : 0);  // one more to see the best that is left out
+  const int rounds = p.top_k + (biased ? 1 : 0);  // one more to see the best that is left out
   for (int i = 0; i < rounds && !unsure; ++i) {
     const unsigned long long top = warp_key_max(key[0]);
     if (top == 0) break;  // (only past the last pick: nothing is left out)
@@ -307,7 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       for (int j = 0; j + 1 < VPT; ++j) key[j] = key[j + 1];
       key[VPT - 1] = 0ull;
     }
-    if (p.bias != nullptr) {
+    if (biased) {
       const float v = key_value(static_cast<unsigned>(top >> 32));
       // (copies of one another are in order already)
       if (i > 0 && !(last - v > 2.f * eps))
@@ -318,20 +363,18 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
     if (lane == i) mine = e;
   }
   float my_logit, my_score;
-  if (unsure) {
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) l[j] = sh_logit[j * 32 + lane];
-    __syncwarp();
-    mine = choose_exactly<VPT>(l, p, lane, row_max, shared[warp]);
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) sh_logit[j * 32 + lane] = l[j];
-    __syncwarp();
-  }
+  if (unsure) mine = choose_exactly<VPT>(sh_logit, p, lane, row_max, shared[warp]);
   my_logit = sh_logit[mine];
   if (softmax) {
-    // (top_score = exp(0) / sum: the other scores relative to it)
-    my_score = row_max == -CUDART_INF_F ? 0.f : expf(my_logit - row_max) * top_score;
+    my_score = 0.f;
+    if (!p.renormalize) {  // (the quick scores will not do: a sum of accurate exponentials)
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (j * 32 + lane < p.experts) sum += expf(sh_logit[j * 32 + lane] - row_max);
+      sum = warp_sum(sum);
+      my_score = row_max == -CUDART_INF_F ? 0.f : expf(my_logit - row_max) / sum;
+    }
   } else {
     my_score = 1.f / (1.f + expf(-my_logit));
   }
