@@ -14,7 +14,8 @@
 //    up to 256 of them share one pass over its weights.  In the epilogue a lane then is a column
 //    of the output and a register a row: every store is a coalesced row piece, straight from
 //    registers, and unused rows cost nothing.
-//        kGateUp  H = w * act(X W1) * (X W2)          X: the rows of x in expert order
+//        kGateUp  H = w * act(X W1) * (X W2)          X: the rows of x in expert order (kGateUpKeep: with
+//                 the fp32 products kept for the backward pass)
 //        kDown    O = H W3                            fp32, one row per pair
 //        kDHidden dH = dY W3^T, then dGU and dw       dY: the rows of dy in expert order
 //        kDX      O = dGU W12^T                       fp32, one row per pair
@@ -29,6 +30,11 @@
 //    twice.  combine_kernel adds a token's rows of O in slot order (fp32) and rounds once.
 //  * The gate/up products are kept in fp32 for the backward pass: rounding them to 16 bits would
 //    add two more roundings to every gradient.
+//  * The tensor cores add to an accumulator by cutting off, not rounding: a sum over K comes out
+//    short by about 3e-9 K of its size.  That is nothing next to 16 bits, but the routing weights'
+//    gradient is fp32 and takes it from both of its factors (measured: 6e-6 at K = 2048, 2.5e-5 at
+//    8192).  So where a product feeds that gradient (kGateUpKeep, kDHidden) an accumulator only runs
+//    over kSumBlocks K blocks, and the epilogue adds those sums up in fp32.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -69,7 +75,16 @@ constexpr int kAbortProducer = 0x301;
 constexpr int kAbortMma = 0x302;
 constexpr int kAbortEpilogue = 0x303;
 
-enum Mode { kGateUp, kGateUpGather, kDown, kDHidden, kDX };
+enum Mode { kGateUp, kGateUpGather, kGateUpKeep, kDown, kDHidden, kDX };
+constexpr bool is_gate_up(int mode) { return mode == kGateUp || mode == kGateUpGather || mode == kGateUpKeep; }
+// Products whose accumulators are added up in fp32 every kSumBlocks K blocks.
+constexpr bool sums_outside(int mode) { return mode == kGateUpKeep || mode == kDHidden; }
+constexpr int kSumBlocks = 3;
+// The sums of a tile are 64 values per epilogue thread, of which 16 stay in shared memory: held in
+// registers altogether they spilled, and the spills' traffic took longer than the products (gate/up
+// product of the training step of 4095 tokens, 16 experts 2048/2040: 389 us).  Tiles of 128 rows
+// would need half of them, but fetch the weights twice as often: 395 us.
+constexpr int kParkedRows = 16;
 
 // Where the pairs went (device memory, written by the plan kernels).
 struct Plan {
@@ -95,7 +110,6 @@ struct RowsParams {
   int panels;       // the weights' map takes two 64-column panels at a time
   int band;         // row tiles per band of the tile order
   int activation;
-  int train;        // gate/up: keep the fp32 products, write padding rows as zeros
   long long max_rows;
   void* out;        // H, dGU (16 bit) or O (fp32, [splits][max_rows][cols])
   float* gu;        // [max_rows][2 d_ff]: written by gate/up, read by kDHidden
@@ -472,18 +486,18 @@ __device__ __forceinline__ Unit decode_unit(const RowsParams& p, int u, int num_
 
 // Sum over the lanes of v[t] for every t, left in lane t.  31 exchanges: each halves the values a
 // lane still carries.
-__device__ __forceinline__ float transposed_sum(float (&v)[32], int lane) {
+__device__ __forceinline__ float transposed_sum(uint32_t (&v)[32], int lane) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const bool upper = (lane & o) != 0;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
-      const float give = upper ? v[i] : v[i + o];
-      const float got = __shfl_xor_sync(0xffffffffu, give, o);
-      v[i] = (upper ? v[i + o] : v[i]) + got;
+      const uint32_t give = upper ? v[i] : v[i + o];
+      const float got = __uint_as_float(__shfl_xor_sync(0xffffffffu, give, o));
+      v[i] = __float_as_uint(__uint_as_float(upper ? v[i + o] : v[i]) + got);
     }
   }
-  return v[0];
+  return __uint_as_float(v[0]);
 }
 
 // What an epilogue warp reads from memory for 32 rows, before it needs it.
@@ -491,7 +505,7 @@ template <int MODE>
 struct Prefetched {
   float weight = 0.f;  // routing weight of row j0 + lane, 0 for padding
   __device__ __forceinline__ void fetch(const RowsParams& p, const Unit& un, int j0, int) {
-    if (MODE == kGateUp || MODE == kGateUpGather)
+    if (is_gate_up(MODE))
       weight = j0 + static_cast<int>(threadIdx.x & 31) < un.used ? p.plan.row_weight[un.row0 + j0 + (threadIdx.x & 31)] : 0.f;
   }
 };
@@ -530,8 +544,8 @@ __device__ __forceinline__ void write_rows(const RowsParams& p, const Unit& un, 
 #pragma unroll
     for (int j = 0; j < 32; ++j, dst += p.cols)
       if (WHOLE || (inside && j < write)) *dst = __uint_as_float(r[j]);
-  } else if (MODE == kGateUp || MODE == kGateUpGather) {
-    if (p.train) {
+  } else if (is_gate_up(MODE)) {
+    if (MODE == kGateUpKeep) {
       float* dst = p.gu + row * p.cols + col;
 #pragma unroll
       for (int j = 0; j < 32; ++j, dst += p.cols)
@@ -567,7 +581,7 @@ __device__ __forceinline__ void write_rows(const RowsParams& p, const Unit& un, 
     auto& first = reinterpret_cast<Prefetched<kDHidden>&>(pre);
     uint32_t* dst = static_cast<uint32_t*>(p.out) + row * p.cols + col;
     float2 other[kBatch];
-    float dw[32];
+    // (a row's part of dw takes the place of its dH)
 #pragma unroll
     for (int b = 0; b < 32; b += 2 * kBatch) {
 #pragma unroll
@@ -581,15 +595,19 @@ __device__ __forceinline__ void write_rows(const RowsParams& p, const Unit& un, 
           const float d = __uint_as_float(r[j]);
           const float2 a = gate_act(now[i].x, p.activation);
           const float wd = __shfl_sync(0xffffffffu, first.weight, j) * d;
-          dw[j] = WHOLE || (inside && j < used) ? d * (a.x * now[i].y) : 0.f;
+          r[j] = WHOLE || (inside && j < used) ? __float_as_uint(d * (a.x * now[i].y)) : 0u;
           const uint32_t pair = pack2<BF16>(wd * now[i].y * a.y, wd * a.x);
           if (WHOLE || (inside && j < write)) *dst = WHOLE || j < used ? pair : 0u;
         }
       }
     }
-    const float sum = transposed_sum(dw, lane);
+    const float sum = transposed_sum(r, lane);
     if (WHOLE || lane < used) p.dw_part[(row + lane) * p.dw_parts + (warp_col >> 5)] = sum;
   }
+}
+
+__device__ __forceinline__ uint32_t add_bits(uint32_t a, uint32_t b) {
+  return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 
 // out^T[256 columns, n rows] = W^T rows^T for one expert's rows; see the top of the file.
@@ -603,7 +621,7 @@ template <int MODE, bool BF16>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ RowsMaps tmap_r,
                 const RowsParams p) {
-  constexpr bool gate_up = MODE == kGateUp || MODE == kGateUpGather;
+  constexpr bool gate_up = is_gate_up(MODE);
   constexpr bool gather = MODE == kGateUpGather;
   constexpr bool w_kmajor = MODE == kDHidden || MODE == kDX;
   constexpr int operand_bytes = kRows * kTileK * 2;
@@ -614,6 +632,7 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   const uint32_t smem_w = (raw_addr + 1023u) & ~1023u;
   const uint32_t smem_r = smem_w + p.stages * operand_bytes;
   Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem_raw + (smem_r + p.stages * operand_bytes - raw_addr));
+  float* parked = reinterpret_cast<float*>(reinterpret_cast<char*>(ctrl) + kCtrlBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -708,14 +727,18 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
       for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
         const Unit un = decode_unit<MODE>(p, u, num_tiles);
         const uint32_t idesc = idesc_base | (static_cast<uint32_t>(un.n >> 3) << 17);
-        if (!ptx::mbar_wait<true>(ptx::smem_u32(&ctrl->tmem_empty[acc.at]), acc.phase ^ 1u, abort_flag, p.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + acc.at * kTileN;
-        uint32_t accumulate = 0;
+        uint32_t d_tmem = 0, accumulate = 0;
         for (int kb = 0; kb < un.num_kb; ++kb) {
+          if (kb == 0 || (sums_outside(MODE) && kb % kSumBlocks == 0)) {  // a fresh accumulator
+            if (!ptx::mbar_wait<true>(ptx::smem_u32(&ctrl->tmem_empty[acc.at]), acc.phase ^ 1u, abort_flag,
+                                      p.timeout_ns)) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after_sync();
+            d_tmem = tmem_base + acc.at * kTileN;
+            accumulate = 0;
+          }
           if (!ptx::mbar_wait(ptx::smem_u32(&ctrl->full[ring.at]), ring.phase, abort_flag, p.timeout_ns)) {
             ok = false;
             break;
@@ -726,18 +749,21 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
           const int steps = (p.k - (un.kb0 + kb) * kTileK + 15) >> 4;
 #pragma unroll
           for (int k16 = 0; k16 < kTileK / 16; ++k16) {
-            const uint32_t kmajor = (k16 >> 2) * (kSlabBytes >> 4) + (k16 & 3) * 2u;
+            const uint32_t in_slab = (k16 & 3) * 2u;
+            const uint32_t w_off = w_kmajor ? (k16 >> 2) * (kSlabBytes >> 4) + in_slab : k16 * 128u;
+            const uint32_t r_off = (k16 >> 2) * (kSlabBytes >> 4) + in_slab;
             if (k16 < steps)
-              ptx::umma_f16<2>(d_tmem, w_desc | ((w16 + (w_kmajor ? kmajor : k16 * 128u)) & 0x3fffu),
-                               r_desc | ((r16 + kmajor) & 0x3fffu), idesc, accumulate);
+              ptx::umma_f16<2>(d_tmem, w_desc | ((w16 + w_off) & 0x3fffu), r_desc | ((r16 + r_off) & 0x3fffu), idesc,
+                               accumulate);
             accumulate = 1;
           }
           ptx::umma_commit_pair(ptx::smem_u32(&ctrl->empty[ring.at]), 0x3);
           ring.next(p.stages);
+          if (kb + 1 == un.num_kb || (sums_outside(MODE) && (kb + 1) % kSumBlocks == 0)) {
+            ptx::umma_commit_pair(ptx::smem_u32(&ctrl->tmem_full[acc.at]), 0x3);
+            acc.next(2);
+          }
         }
-        if (!ok) break;
-        ptx::umma_commit_pair(ptx::smem_u32(&ctrl->tmem_full[acc.at]), 0x3);
-        acc.next(2);
       }
       if (!ok && p.status != nullptr) atomicCAS(p.status, 0, kAbortMma);
     }
@@ -756,32 +782,93 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
       const Unit un = decode_unit<MODE>(p, u, num_tiles);
       const int warp_col = un.col0 + rank * kRows + quarter * 32;
-      // rows to write: those in use, and in a training step the zeros that pad an expert
-      const int rows = (gate_up || MODE == kDHidden) && p.train ? un.padded : un.used;
+      // rows to write: those in use, and in a training step the zeros that pad an expert (products
+      // over K = rows read them)
+      const int rows = sums_outside(MODE) ? un.padded : un.used;
       const int mine = warp_col < p.cols ? rows : 0;  // (warp-uniform)
       Prefetched<MODE> pre;
-      if (first_row < mine) pre.fetch(p, un, first_row, warp_col + lane);
-
-      const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc.at]), acc.phase, abort_flag, p.timeout_ns);
-      if (!__all_sync(0xffffffffu, got)) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after_sync();
-      const uint32_t t_acc = tmem_base + lane_sel + acc.at * kTileN;
-      for (int j0 = first_row; j0 < mine; j0 += kStep) {
-        uint32_t r[32];
-        ptx::tmem_ld_32x32(t_acc + j0, r);
-        ptx::tmem_ld_wait(r);
-        const bool whole = j0 + 32 <= un.used && warp_col + 32 <= p.cols;
-        if (whole)
+      // Waits for the next accumulator; false if it does not come in time.
+      auto next_accumulator = [&]() -> bool {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&ctrl->tmem_full[acc.at]), acc.phase, abort_flag, p.timeout_ns);
+        if (!__all_sync(0xffffffffu, got)) return false;
+        ptx::tc_fence_after_sync();
+        return true;
+      };
+      uint32_t r[32];
+      auto write = [&](int j0) {
+        if (j0 + 32 <= un.used && warp_col + 32 <= p.cols)
           write_rows<MODE, BF16, true>(p, un, j0, rows, warp_col, lane, r, pre);
         else
           write_rows<MODE, BF16, false>(p, un, j0, rows, warp_col, lane, r, pre);
-        if (j0 + kStep < mine) pre.fetch(p, un, j0 + kStep, warp_col + lane);
+      };
+      if constexpr (sums_outside(MODE)) {
+        // The sums over kSumBlocks K blocks each, added in fp32 as they come: the first 32 rows and
+        // half of the second in registers, the other half in this thread's column of `parked`.
+        static_assert(kTileN == 2 * kStep, "a warp has two chunks of rows");
+        float* mine_parked = parked + (warp - 2) * (kParkedRows * 32) + lane;
+        const bool one = first_row < mine, two = first_row + kStep < mine;
+        uint32_t more[32 - kParkedRows];
+        const int parts = (un.num_kb + kSumBlocks - 1) / kSumBlocks;
+        for (int part = 0; part < parts; ++part) {
+          if (!next_accumulator()) {
+            ok = false;
+            break;
+          }
+          const uint32_t t_acc = tmem_base + lane_sel + acc.at * kTileN + first_row;
+          if (one) {
+            uint32_t v[16];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ptx::tmem_ld_32x16(t_acc + half * 16, v);
+              ptx::tmem_ld_wait(v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) r[half * 16 + j] = part == 0 ? v[j] : add_bits(r[half * 16 + j], v[j]);
+            }
+            if (two) {
+              ptx::tmem_ld_32x16(t_acc + kStep, v);
+              ptx::tmem_ld_wait(v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) more[j] = part == 0 ? v[j] : add_bits(more[j], v[j]);
+              ptx::tmem_ld_32x16(t_acc + kStep + 16, v);
+              ptx::tmem_ld_wait(v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                mine_parked[j * 32] = (part == 0 ? 0.f : mine_parked[j * 32]) + __uint_as_float(v[j]);
+            }
+          }
+          release_accumulator(ctrl, acc.at, leader, lane);
+          acc.next(2);
+        }
+        if (!ok) break;
+        if (one) {
+          pre.fetch(p, un, first_row, warp_col + lane);
+          write(first_row);
+        }
+        if (two) {
+          pre.fetch(p, un, first_row + kStep, warp_col + lane);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            r[j] = more[j];
+            r[16 + j] = __float_as_uint(mine_parked[j * 32]);
+          }
+          write(first_row + kStep);
+        }
+      } else {
+        if (first_row < mine) pre.fetch(p, un, first_row, warp_col + lane);
+        if (!next_accumulator()) {
+          ok = false;
+          break;
+        }
+        const uint32_t t_acc = tmem_base + lane_sel + acc.at * kTileN;
+        for (int j0 = first_row; j0 < mine; j0 += kStep) {
+          ptx::tmem_ld_32x32(t_acc + j0, r);
+          ptx::tmem_ld_wait(r);
+          write(j0);
+          if (j0 + kStep < mine) pre.fetch(p, un, j0 + kStep, warp_col + lane);
+        }
+        release_accumulator(ctrl, acc.at, leader, lane);
+        acc.next(2);
       }
-      release_accumulator(ctrl, acc.at, leader, lane);
-      acc.next(2);
     }
     if (!ok && lane == 0 && p.status != nullptr) atomicCAS(p.status, 0, kAbortEpilogue);
   }
@@ -1447,10 +1534,12 @@ int launch_rows(const tnx_moe_problem& q, const Layout& l, const CUtensorMap& w,
                 cudaStream_t stream) {
   p.tiles_n = cdiv(p.cols, 2 * kRows);
   p.max_rows = l.max_rows;
+  p.band = 8;
   const int64_t units = static_cast<int64_t>(l.max_tiles) * p.tiles_n * p.splits;
+  constexpr int staging = sums_outside(MODE) ? kRowsEpilogue * kParkedRows * 32 * 4 : 0;
   return q.dtype == TNX_BF16
-             ? launch_pairs(moe_rows_kernel<MODE, true>, kRowsThreads, p, 0, units, stream, w, r)
-             : launch_pairs(moe_rows_kernel<MODE, false>, kRowsThreads, p, 0, units, stream, w, r);
+             ? launch_pairs(moe_rows_kernel<MODE, true>, kRowsThreads, p, staging, units, stream, w, r)
+             : launch_pairs(moe_rows_kernel<MODE, false>, kRowsThreads, p, staging, units, stream, w, r);
 }
 // out[e] = a[rows of e]^T b[rows of e], m x n.
 int run_wgrad(const tnx_moe_problem& q, const Layout& l, const Plan& plan, const void* a, int m, const void* b, int n,
@@ -1537,8 +1626,6 @@ RowsParams rows_params(const tnx_moe_problem& p, const Plan& plan, int32_t* stat
   RowsParams g = {};
   g.plan = plan;
   g.activation = p.activation;
-  g.train = p.train;
-  g.band = 8;
   g.status = status;
   g.timeout_ns = bounded_wait_limit_ns();
   return g;
@@ -1680,7 +1767,9 @@ int tnx_moe_swiglu(const tnx_moe_problem* problem, const void* x, const void* w1
     rc = rows_maps(&rows, xp, p.dtype, p.d_model, l.max_rows);
   }
   if (rc != TNX_OK) return rc;
-  rc = l.gather ? launch_rows<kGateUpGather>(p, l, tw, rows, g, s) : launch_rows<kGateUp>(p, l, tw, rows, g, s);
+  rc = p.train    ? launch_rows<kGateUpKeep>(p, l, tw, rows, g, s)
+       : l.gather ? launch_rows<kGateUpGather>(p, l, tw, rows, g, s)
+                  : launch_rows<kGateUp>(p, l, tw, rows, g, s);
   if (rc != TNX_OK) return rc;
 
   // O = H W3
@@ -1754,7 +1843,6 @@ int tnx_moe_swiglu_backward(const tnx_moe_problem* problem, const void* dy, int6
     g.gu = gu;
     g.dw_part = dw_part;
     g.dw_parts = l.dw_parts;
-    g.train = 1;  // (the padding rows of dGU are zeros: products over K = rows read them)
     rc = make_tmap_3d(&tw, w3, p.dtype, p.n_out, p.d_ff, p.experts, p.stride_w3k, p.stride_w3e, 64, kRows, true);
     if (rc == TNX_OK) rc = rows_maps(&rows, dyp, p.dtype, p.n_out, l.max_rows);
     if (rc == TNX_OK) rc = launch_rows<kDHidden>(p, l, tw, rows, g, s);
