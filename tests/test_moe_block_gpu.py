@@ -1,0 +1,142 @@
+"""Routing, the experts' products and the norms in a row, as a model runs them: values, gradients,
+graphs, streams, and the torch custom ops."""
+import pytest
+import torch
+
+import tritonix_b200 as tnx
+from oracle import moe as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+bf16, f32 = torch.bfloat16, torch.float32
+NAMES = ("x", "residual", "logits", "w12", "w3", "post", "pre", "gate")
+
+
+def make(t, n, d, f, seed=0, dtype=bf16):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    return {"x": r(t, d).to(dtype), "residual": (2 * r(t, d)).to(dtype), "logits": r(t, n),
+            "w12": (r(n, d, 2 * f) * d ** -0.5).to(dtype), "w3": (r(n, f, d) * f ** -0.5).to(dtype),
+            "post": 1 + 0.1 * r(d), "pre": 1 + 0.1 * r(d), "gate": 0.5 + 0.1 * r(d), "bias": 0.1 * r(n),
+            "dh": r(t, d).to(dtype), "dn": r(t, d).to(dtype)}
+
+
+def leaves(case, grad=True):
+    return [case[k].to(DEV).requires_grad_(grad) for k in NAMES]
+
+
+KW = dict(scoring="sigmoid", num_groups=4, top_groups=2, scale=1.5, residual_scale=0.7)
+
+
+def block(args, bias, top_k=3):
+    x, residual, logits, w12, w3, post, pre, gate = args
+    return tnx.moe_block(x, residual, logits, w12, w3, post, pre, top_k, bias=bias, gate=gate, **KW)
+
+
+def reference(case, args):
+    """The same from plain operations in 64 bits with autograd; experts as the oracle picks them."""
+    x, residual, logits, w12, w3, post, pre, gate = args
+    _, ids, _ = O.route_oracle(case["logits"], 3, "sigmoid", case["bias"], 4, 2)
+    s = torch.sigmoid(logits).gather(1, ids)
+    weights = 1.5 * s / s.sum(1, keepdim=True)
+    y = torch.zeros_like(residual)
+    for e in range(w12.shape[0]):
+        token, slot = torch.nonzero(ids == e, as_tuple=True)
+        gu = x[token] @ w12[e]
+        out = (torch.nn.functional.silu(gu[:, 0::2]) * gu[:, 1::2]) @ w3[e]
+        y = y.index_add(0, token, weights[token, slot].unsqueeze(1) * out)
+    rms = lambda v: v * (v.square().mean(1, keepdim=True) + 1e-6).rsqrt()  # noqa: E731
+    h = 0.7 * residual + gate * rms(y) * post
+    return h, rms(h) * pre
+
+
+@pytest.mark.parametrize("t", [1, 7, 130, 900])
+def test_block_and_its_gradients(t):
+    case = make(t, 16, 256, 136, seed=t)
+    args = leaves(case)
+    h, n = block(args, case["bias"].to(DEV))
+    grads = torch.autograd.grad([h, n], args, [case["dh"].to(DEV), case["dn"].to(DEV)])
+    tnx.check_status(h.device)
+    plain = [case[k].double().requires_grad_(True) for k in NAMES]
+    rh, rn = reference(case, plain)
+    want = torch.autograd.grad([rh, rn], plain, [case["dh"].double(), case["dn"].double()])
+    # Values: the hidden activation, y and the result are rounded to bf16, half a step each.  On the
+    # way back the gradient of y and that of the gate/up products are rounded too, and the backward
+    # norm starts from the rounded y; each once, plus the result's own.  In the 2-norm independent
+    # roundings of at most half a step stay below their sum.
+    half = 2.0 ** -8
+    for out, ref, roundings in ((h, rh, 3), (n, rn, 3)):
+        assert (out.detach().cpu().double() - ref).norm() <= roundings * half * ref.norm()
+    for grad, ref, name in zip(grads, want, NAMES):
+        assert grad.shape == ref.shape
+        assert (grad.cpu().double() - ref).norm() <= 6 * half * ref.norm(), name
+
+
+def test_equals_the_three_operators():
+    case = make(40, 16, 128, 64)
+    args = leaves(case, False)
+    h, n = block(args, case["bias"].to(DEV))
+    w, i = tnx.route_experts(args[2], 3, scoring="sigmoid", bias=case["bias"].to(DEV), num_groups=4, top_groups=2,
+                             scale=1.5)
+    y = tnx.moe_swiglu(args[0], args[3], args[4], i, w)
+    h2, n2 = tnx.gated_residual_norm(y, args[1], args[5], args[6], args[7], residual_scale=0.7)
+    assert torch.equal(h, h2) and torch.equal(n, n2)
+
+
+def test_training_step_captured_in_a_graph():
+    case = make(200, 16, 256, 128, seed=5)
+    args, bias = leaves(case), case["bias"].to(DEV)
+    dh, dn = case["dh"].to(DEV), case["dn"].to(DEV)
+    block(leaves(case, False), bias)     # warm-up on other leaves, without a graph of these
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, n = block(args, bias)
+        grads = torch.autograd.grad([h, n], args, [dh, dn])
+    other = make(200, 16, 256, 128, seed=6)
+    with torch.no_grad():
+        for a, k in zip(args, NAMES):
+            a.copy_(other[k])
+    graph.replay()
+    fresh = leaves(other)
+    h2, n2 = block(fresh, bias)
+    want = torch.autograd.grad([h2, n2], fresh, [dh, dn])
+    assert torch.equal(h, h2) and torch.equal(n, n2)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_two_streams_at_once():
+    cases = [make(64, 16, 128, 64, seed=i) for i in (1, 2)]
+    args = [leaves(c, False) for c in cases]
+    bias = [c["bias"].to(DEV) for c in cases]
+    want = [block(a, b) for a, b in zip(args, bias)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(8):
+        for s, a, b in zip(streams, args, bias):
+            with torch.cuda.stream(s):
+                got.append(block(a, b))
+    torch.cuda.synchronize()
+    for i, (h, n) in enumerate(got):
+        assert torch.equal(h, want[i % 2][0]) and torch.equal(n, want[i % 2][1])
+
+
+def test_padding_tokens_leave_the_others_alone():
+    """Rows of -inf logits and NaN inputs behind the last sequence."""
+    case = make(50, 16, 128, 64, seed=9)
+    clean = block(leaves(case, False), case["bias"].to(DEV))
+    case["x"][40:] = float("nan")
+    case["logits"][40:] = float("-inf")
+    dirty = block(leaves(case, False), case["bias"].to(DEV))
+    assert torch.equal(clean[0][:40], dirty[0][:40]) and torch.equal(clean[1][:40], dirty[1][:40])
+
+
+def test_custom_ops():
+    case = make(20, 16, 128, 64)
+    args, bias = leaves(case, False), case["bias"].to(DEV)
+    w, i = torch.ops.tritonix.route_experts(args[2], 3, "sigmoid", bias, 4, 2, True, 1.5)
+    y = torch.ops.tritonix.moe_swiglu(args[0], args[3], args[4], i, w, "silu")
+    h, n = torch.ops.tritonix.gated_residual_norm(y, args[1], args[5], args[6], args[7], 0.7, 1e-6)
+    want = block(args, bias)
+    assert torch.equal(h, want[0]) and torch.equal(n, want[1])

@@ -2,7 +2,9 @@
 import ctypes
 
 import pytest
+import torch
 
+import tritonix_b200 as tnx
 from tritonix_b200 import _cabi
 
 lib = _cabi.lib
@@ -130,3 +132,24 @@ def test_moe_resources_and_workspace():
                dict(nbytes=need, saved=None), dict(nbytes=need, dy=None), dict(nbytes=need, stride=44),
                dict(nbytes=need, stride=40), dict(nbytes=need, dy=PTR + 8)):
         assert gradients(moe(train=1), **kw) == _cabi.ERR_INVALID
+
+
+def test_custom_ops_give_shapes_without_a_device():
+    meta = lambda *s, dt=torch.bfloat16: torch.empty(s, dtype=dt, device="meta")  # noqa: E731
+    w, i = torch.ops.tritonix.route_experts(meta(5, 8), 2, "softmax", None, 1, 1, True, 1.0)
+    assert (w.shape, w.dtype, i.shape, i.dtype) == ((5, 2), torch.float32, (5, 2), torch.int32)
+    y = torch.ops.tritonix.moe_swiglu(meta(5, 16), meta(8, 16, 48), meta(8, 24, 32), i, w, "silu")
+    assert (y.shape, y.dtype) == ((5, 32), torch.bfloat16)
+    h, n = torch.ops.tritonix.gated_residual_norm(y, y, meta(32), meta(32), None, 1.0, 1e-6)
+    assert h.shape == n.shape == (5, 32)
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tnx.route_experts(x, 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tnx.gated_residual_norm(x, x, x[0], x[0])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        tnx.moe_swiglu(x, torch.zeros(2, 8, 16), torch.zeros(2, 8, 8), torch.zeros(4, 1, dtype=torch.int32),
+                       torch.zeros(4, 1))

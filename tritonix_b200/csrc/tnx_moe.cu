@@ -511,7 +511,7 @@ struct Prefetched {
 };
 template <>
 struct Prefetched<kDHidden> {
-  static constexpr int kBatch = 8;
+  static constexpr int kBatch = 4;
   float weight = 0.f;
   float2 gu[kBatch];  // gate/up products of the first rows; write_rows fetches the others
   // Rows and columns that do not exist are read at the tile's first and not used: no branches.

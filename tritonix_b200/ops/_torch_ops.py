@@ -21,6 +21,12 @@ _lib.define("gemm_splitk(Tensor a, Tensor b, int split_k, int[] cfg) -> Tensor")
 _lib.define("glu(Tensor x, Tensor w12, int activation, int[] cfg) -> Tensor")
 _lib.define("conv2d_forward(Tensor input, Tensor weight, Tensor? bias, int[] stride, int[] padding, "
             "int[] dilation, int[] cfg) -> Tensor")
+# (scoring and activation by name, as the Python functions take them)
+_lib.define("route_experts(Tensor logits, int top_k, str scoring, Tensor? bias, int num_groups, int top_groups, "
+            "bool renormalize, float scale) -> (Tensor, Tensor)")
+_lib.define("moe_swiglu(Tensor x, Tensor w12, Tensor w3, Tensor ids, Tensor weights, str activation) -> Tensor")
+_lib.define("gated_residual_norm(Tensor y, Tensor residual, Tensor post_weight, Tensor pre_weight, Tensor? gate, "
+            "float residual_scale, float eps) -> (Tensor, Tensor)")
 
 
 def cfg_to_list(cfg: dict | None) -> List[int]:
@@ -65,6 +71,25 @@ def _conv2d_forward(input, weight, bias, stride, padding, dilation, cfg):
                           config=config or None)
 
 
+def _route_experts(logits, top_k, scoring, bias, num_groups, top_groups, renormalize, scale):
+    from tritonix_b200.ops.moe import route_experts
+    return route_experts(logits, top_k, scoring=scoring, bias=bias, num_groups=num_groups, top_groups=top_groups,
+                         renormalize=renormalize, scale=scale)
+
+
+def _moe_swiglu(x, w12, w3, ids, weights, activation):
+    from tritonix_b200.ops.moe import moe_swiglu
+    return moe_swiglu(x, w12, w3, ids, weights, activation)
+
+
+def _gated_residual_norm(y, residual, post_weight, pre_weight, gate, residual_scale, eps):
+    from tritonix_b200.ops.norm import gated_residual_norm
+    return gated_residual_norm(y, residual, post_weight, pre_weight, gate, residual_scale, eps)
+
+
+_lib.impl("route_experts", _route_experts, "CUDA")
+_lib.impl("moe_swiglu", _moe_swiglu, "CUDA")
+_lib.impl("gated_residual_norm", _gated_residual_norm, "CUDA")
 _lib.impl("gemm", _gemm, "CUDA")
 _lib.impl("conv2d_forward", _conv2d_forward, "CUDA")
 _lib.impl("gemm_splitk", _gemm_splitk, "CUDA")
@@ -94,3 +119,19 @@ def _conv2d_forward_fake(input, weight, bias, stride, padding, dilation, cfg):
                        device=input.device, dtype=input.dtype,
                        memory_format=torch.channels_last if channels_last
                        else torch.contiguous_format)
+
+
+@torch.library.register_fake("tritonix::route_experts")
+def _route_experts_fake(logits, top_k, scoring, bias, num_groups, top_groups, renormalize, scale):
+    shape = (logits.shape[0], top_k)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+
+@torch.library.register_fake("tritonix::moe_swiglu")
+def _moe_swiglu_fake(x, w12, w3, ids, weights, activation):
+    return x.new_empty((x.shape[0], w3.shape[2]))
+
+
+@torch.library.register_fake("tritonix::gated_residual_norm")
+def _gated_residual_norm_fake(y, residual, post_weight, pre_weight, gate, residual_scale, eps):
+    return y.new_empty(y.shape), y.new_empty(y.shape)

@@ -1,8 +1,9 @@
 """Mixture-of-experts layers: routing tokens to experts and the experts' gated products.
 
 ``route_experts`` turns router logits into the experts each token uses and their weights;
-``moe_swiglu`` is ``swiglu_mlp`` with many expert MLPs of which each token uses a few.  Both have
-their gradients.  The reference has no counterpart.
+``moe_swiglu`` is ``swiglu_mlp`` with many expert MLPs of which each token uses a few; ``moe_block``
+joins them with the norms around a block (ops/norm.py).  All have their gradients.  The reference
+has no counterpart.
 """
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ import ctypes
 import torch
 
 from tritonix_b200 import _cabi
+from tritonix_b200.ops.norm import gated_residual_norm
 
 
 _route_problems: dict = {}
@@ -251,3 +253,26 @@ def _check_moe(x, w12, w3, ids, weights, activation) -> int:
     if act is None:
         raise ValueError(f"activation must be one of {sorted(_cabi.ACTIVATIONS)}, got {activation!r}")
     return act
+
+
+# ---------------------------------------------------------------------------------- the whole block
+
+def moe_block(x: torch.Tensor, residual: torch.Tensor, logits: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor,
+              post_weight: torch.Tensor, pre_weight: torch.Tensor, top_k: int, *, scoring: str = "softmax",
+              bias: torch.Tensor | None = None, num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+              scale: float = 1.0, activation: str = "silu", gate: torch.Tensor | None = None,
+              residual_scale: float = 1.0, eps: float = 1e-6):
+    """A mixture-of-experts block from its normalised input to the next block's:
+
+        weights, ids = route_experts(logits, top_k, ...)
+        y = moe_swiglu(x, w12, w3, ids, weights, activation)
+        h, n = gated_residual_norm(y, residual, post_weight, pre_weight, gate, residual_scale, eps)
+
+    ``x`` [tokens, D] is the block's input, ``logits`` [tokens, experts] its router's output (``matmul``
+    of ``x`` and the router's weights, say), ``residual`` [tokens, N] the residual stream; the other
+    arguments are those of the three operators.  Returns ``(h, n)``: the new residual stream and the
+    next block's input.  Gradients flow through all of it."""
+    weights, ids = route_experts(logits, top_k, scoring=scoring, bias=bias, num_groups=num_groups,
+                                 top_groups=top_groups, renormalize=renormalize, scale=scale)
+    y = moe_swiglu(x, w12, w3, ids, weights, activation)
+    return gated_residual_norm(y, residual, post_weight, pre_weight, gate, residual_scale, eps)
