@@ -34,7 +34,7 @@
 //    short by about 3e-9 K of its size.  That is nothing next to 16 bits, but the routing weights'
 //    gradient is fp32 and takes it from both of its factors (measured: 6e-6 at K = 2048, 2.5e-5 at
 //    8192).  So where a product feeds that gradient (kGateUpKeep, kDHidden) an accumulator only runs
-//    over kSumBlocks K blocks, and the epilogue adds those sums up in fp32.
+//    over a few K blocks, and the epilogue adds those sums up in fp32.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -77,9 +77,10 @@ constexpr int kAbortEpilogue = 0x303;
 
 enum Mode { kGateUp, kGateUpGather, kGateUpKeep, kDown, kDHidden, kDX };
 constexpr bool is_gate_up(int mode) { return mode == kGateUp || mode == kGateUpGather || mode == kGateUpKeep; }
-// Products whose accumulators are added up in fp32 every kSumBlocks K blocks.
+// Products whose accumulators are added up in fp32 every so many K blocks.
 constexpr bool sums_outside(int mode) { return mode == kGateUpKeep || mode == kDHidden; }
-constexpr int kSumBlocks = 3;
+// (fp16 products lose a little more: 1.35e-6 after 512 elements of bf16 as of 384 of fp16)
+constexpr int sum_blocks(bool bf16) { return bf16 ? 4 : 3; }
 // The sums of a tile are 64 values per epilogue thread, of which 16 stay in shared memory: held in
 // registers altogether they spilled, and the spills' traffic took longer than the products (gate/up
 // product of the training step of 4095 tokens, 16 experts 2048/2040: 389 us).  Tiles of 128 rows
@@ -624,6 +625,7 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
   constexpr bool gate_up = is_gate_up(MODE);
   constexpr bool gather = MODE == kGateUpGather;
   constexpr bool w_kmajor = MODE == kDHidden || MODE == kDX;
+  constexpr int kSumBlocks = sum_blocks(BF16);
   constexpr int operand_bytes = kRows * kTileK * 2;
   constexpr int kSlabBytes = kRows * kSlab * 2;       // K-major: 128 rows x 64 elements
   constexpr int kAtom = kTileK * kAtomBytes;          // M-major: 64 columns x K rows
@@ -831,12 +833,13 @@ moe_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
               for (int j = 0; j < 16; ++j) more[j] = part == 0 ? v[j] : add_bits(more[j], v[j]);
               ptx::tmem_ld_32x16(t_acc + kStep + 16, v);
               ptx::tmem_ld_wait(v);
+              release_accumulator(ctrl, acc.at, leader, lane);
 #pragma unroll
               for (int j = 0; j < 16; ++j)
                 mine_parked[j * 32] = (part == 0 ? 0.f : mine_parked[j * 32]) + __uint_as_float(v[j]);
             }
           }
-          release_accumulator(ctrl, acc.at, leader, lane);
+          if (!two) release_accumulator(ctrl, acc.at, leader, lane);
           acc.next(2);
         }
         if (!ok) break;
