@@ -225,6 +225,22 @@ def test_captured_forward_and_backward():
     assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
+def test_offsets_past_32_bits():
+    """140000 rows of 16384: 2.3e9 elements."""
+    t, d = 140000, 16384
+    case = make(40, d, bf16, bf16, "channel", seed=1)
+    y, residual = torch.zeros(t, d, device=DEV, dtype=bf16), torch.zeros(t, d, device=DEV, dtype=bf16)
+    for part, name in ((y, "y"), (residual, "residual")):
+        part[:20].copy_(case[name][:20])
+        part[-20:].copy_(case[name][20:])
+    h, n = tnx.gated_residual_norm(y, residual, *[case[k].to(DEV) for k in ("post", "pre", "gate")], residual_scale=0.75)
+    tnx.check_status(h.device)
+    rh, rn, mh, mn = O.norm_oracle(*[case[k] for k in ("y", "residual", "post", "pre", "gate")], 0.75, 1e-6)
+    within(torch.cat([h[:20], h[-20:]]), rh, mh, FORWARD)
+    within(torch.cat([n[:20], n[-20:]]), rn, mn, FORWARD)
+    assert not h[20:-20:997].any()
+
+
 def test_refusals():
     y = torch.zeros(4, 8, device=DEV, dtype=bf16)
     w = torch.ones(8, device=DEV, dtype=bf16)

@@ -256,6 +256,21 @@ def test_captured_backward():
     assert all(torch.equal(g, w) for g, w in zip(grads, want))
 
 
+def test_offsets_past_32_bits():
+    """320000 rows x 8192 fp32 sums between the down product and the join: 2.6e9 elements."""
+    t, n, k, d, f, n_out = 40000, 8, 8, 64, 64, 8192
+    case = make(64, n, k, d, f, n_out, bf16, seed=2)
+    g = torch.Generator().manual_seed(3)
+    ids = torch.stack([torch.randperm(n, generator=g)[:k] for _ in range(t)]).to(torch.int32)
+    x = torch.randn(t, d, generator=g).to(bf16)
+    weights = torch.rand(t, k, generator=g)
+    y = tnx.moe_swiglu(x.to(DEV), case["w12"].to(DEV), case["w3"].to(DEV), ids.to(DEV), weights.to(DEV))
+    tnx.check_status(y.device)
+    pick = torch.cat([torch.arange(20), torch.randint(0, t, (40,), generator=g), torch.arange(t - 20, t)])
+    want = O.experts_oracle(x[pick], case["w12"], case["w3"], ids[pick], weights[pick])
+    close(y[pick.to(DEV)], want, 2 * torch.finfo(bf16).eps / 2, "y")
+
+
 def test_refusals():
     x, w12, w3, ids, w = operands(make(4, 4, 2, 64, 64, 64, bf16))
     for bad, match in (((x.float(), w12, w3, ids, w), "float16"), ((x, w12.half(), w3, ids, w), "float16"),

@@ -569,6 +569,11 @@ def launch_mlp(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, y: torch.Te
 # ---------------------------------------------------------------------------------------------
 # Mixture of experts, norms
 # ---------------------------------------------------------------------------------------------
+# The raw handle of torch's current stream without a Stream object around it (1.3 us less per call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
 def call(device: torch.device, fn, *args) -> None:
     """Calls an entry point whose last argument is the stream: on ``device``, with torch's current
     stream of it.  The caller's current device is left as it was."""
@@ -577,7 +582,7 @@ def call(device: torch.device, fn, *args) -> None:
     if idx != previous:
         torch.cuda.set_device(idx)
     try:
-        rc = fn(*args, torch.cuda.current_stream(idx).cuda_stream)
+        rc = fn(*args, _raw_stream(idx))
     finally:
         if idx != previous:
             torch.cuda.set_device(previous)

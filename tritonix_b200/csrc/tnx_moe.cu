@@ -79,8 +79,8 @@ enum Mode { kGateUp, kGateUpGather, kGateUpKeep, kDown, kDHidden, kDX };
 constexpr bool is_gate_up(int mode) { return mode == kGateUp || mode == kGateUpGather || mode == kGateUpKeep; }
 // Products whose accumulators are added up in fp32 every so many K blocks.
 constexpr bool sums_outside(int mode) { return mode == kGateUpKeep || mode == kDHidden; }
-// (fp16 products lose a little more: 1.35e-6 after 512 elements of bf16 as of 384 of fp16)
-constexpr int sum_blocks(bool bf16) { return bf16 ? 4 : 3; }
+// (384 elements of bf16 or 256 of fp16 lose 1e-6 of that gradient, what fp32 loses by itself)
+constexpr int sum_blocks(bool bf16) { return bf16 ? 3 : 2; }
 // The sums of a tile are 64 values per epilogue thread, of which 16 stay in shared memory: held in
 // registers altogether they spilled, and the spills' traffic took longer than the products (gate/up
 // product of the training step of 4095 tokens, 16 experts 2048/2040: 389 us).  Tiles of 128 rows
