@@ -104,6 +104,34 @@ def test_rows_that_arrive_ahead_from_an_odd_address():
         store[1 + i:].copy_(case[name].to(DEV).reshape(-1))
         views.append(store[1 + i:].view(600, 301))
     got = tnx.gated_residual_norm(views[0], views[1], args[2], args[3], views[2])
+    # (rows moved by different amounts are read element by element, and their squares added in another
+    # order: the last bit may differ)
+    for a, b in zip(want, got):
+        torch.testing.assert_close(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("dtype,wtype", [(bf16, bf16), (bf16, f32), (f32, f32)])
+@pytest.mark.parametrize("t,d", [(601, 9), (605, 68), (1203, 1022), (777, 2051), (593, 4090), (594, 8185)])
+def test_rows_that_start_between_boundaries(t, d, dtype, wtype, gate):
+    """Every tensor's rows are moved alike: whole vectors, a partial one at either end."""
+    check(make(t, d, dtype, wtype, gate, seed=t + d))
+
+
+@pytest.mark.parametrize("dtype,wtype", [(bf16, f32), (f32, f32)])
+def test_partial_vectors_leave_their_neighbours_alone(dtype, wtype):
+    """Infinities and NaN right before and after a row of a wider tensor stay out of it."""
+    case = make(640, 77, dtype, wtype, "full", seed=3)
+    args = on_gpu(case, False)
+    want = tnx.gated_residual_norm(*args)
+
+    def inside(value, fill):  # rows 80 + 5 elements apart: moved as 77's are, to a vector of 8 or of 4
+        store = torch.full((640, 85), fill, device=DEV, dtype=value.dtype)
+        store[:, :77] = value
+        return store[:, :77]
+
+    got = tnx.gated_residual_norm(inside(args[0], float("nan")), inside(args[1], float("inf")), args[2], args[3],
+                                  inside(args[4], float("-inf")))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 

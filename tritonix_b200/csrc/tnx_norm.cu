@@ -48,8 +48,18 @@ struct NormParams {
 
 constexpr int kMaxCols = 16384;
 // Threads of a row at most, by the values each of them holds: 256 with up to 16 values (two or
-// three blocks per SM), then 512; single elements 640.
-__host__ __device__ constexpr int max_threads(int vec, int nv) { return vec == 1 ? 640 : vec * nv <= 16 ? 256 : 512; }
+// three blocks per SM), then 512; single elements 640.  LED rows take a warp more, so that 608 threads
+// of 8 values (640 of two short vectors: five fp32 rows leave room for one block only) and 480 of
+// more leave each thread the registers it needs.
+__host__ __device__ constexpr int max_threads(int vec, int nv, bool led = false) {
+  if (led) return vec * nv > 8 ? 480 : nv == 2 ? 640 : 608;
+  return vec == 1 ? 640 : vec * nv <= 16 ? 256 : 512;
+}
+// Threads of a block of a ring kernel at most, and blocks per SM that its registers are limited for.
+__host__ __device__ constexpr int ring_threads(int vec, int nv, bool led) { return max_threads(vec, nv, led) + (led ? 32 : 0); }
+__host__ __device__ constexpr int ring_blocks(int vec, int nv, bool led, bool backward) {
+  return max_threads(vec, nv, led) > 256 ? 1 : backward ? 2 : 3;
+}
 
 // Sums of two values over the `threads` threads of a row.  `slot` alternates between calls so
 // that one barrier per call is enough.  Every thread of the block takes part.
@@ -286,6 +296,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// A barrier of the whole block that warps may come to from different places, and whether `ok` held for
+// every thread.
+__device__ __forceinline__ bool block_barrier(bool ok = true) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 0, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return all != 0;
+}
+
 // Sums of N values over the block, and whether `ok` held for every thread.  `levels`: so many times
 // two warps (blockDim.x is up to 32 << levels).
 template <int N>
@@ -296,7 +318,7 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float2* smem, int level
 #pragma unroll
     for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   if ((tid & 31) == 0) smem[tid >> 5] = make_float2(v[0], v[N - 1]);
-  ok = __syncthreads_and(ok) != 0;
+  ok = block_barrier(ok);
   const int warps = blockDim.x >> 5, lane = tid & ((1 << levels) - 1);
   const float2 all = lane < warps ? smem[lane] : make_float2(0.f, 0.f);
   v[0] = all.x;
@@ -308,10 +330,14 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float2* smem, int level
 
 // The rows a block walks: blockIdx.x, blockIdx.x + gridDim.x, ...  Row number i of them lies in slot
 // i % depth, one part of the slot per source.  A bulk copy starts and ends on 16-byte boundaries, so
-// a row is copied from the boundary at or before its first byte to the one at or after its last;
-// only the very last row of a tensor could be read past its end that way: its block copies it with
-// ordinary loads.
-// MOVED: rows may start anywhere (otherwise all start on 16-byte boundaries).
+// a row is copied from the boundary at or before its first byte to the one at or after its last.
+// Only the very last row of a tensor could be read past its end that way: the bytes behind its last
+// boundary follow by ordinary loads (the whole of it by ordinary loads made its block 10 to 40 us
+// late).
+// MOVED: rows may start anywhere (otherwise all start on 16-byte boundaries), but all rows of a block
+// equally far behind a boundary: the grid is a multiple of the rows after which that comes back.
+// (Working the distance out for each row cost the thread that issues the copies, and with it the
+// block, about a microsecond a row.)
 constexpr int kMaxSources = 5;
 template <bool MOVED>
 struct Ring {
@@ -322,6 +348,7 @@ struct Ring {
   const char* src[kMaxSources];
   long long pitch[kMaxSources];  // bytes
   uint32_t row_bytes[kMaxSources], offset[kMaxSources];
+  uint32_t shift[kMaxSources];  // bytes from the boundary to a row's start
   int row, slot;  // where the block is
   uint32_t phase;
 
@@ -334,16 +361,18 @@ struct Ring {
     pitch[sources] = ld * static_cast<long long>(sizeof(E));
     row_bytes[sources] = static_cast<uint32_t>(cols * sizeof(E));
     offset[sources] = slot_bytes;
+    shift[sources] =
+        MOVED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[sources] + row * pitch[sources]) & 15) : 0u;
     slot_bytes += ring_row_bytes(cols, sizeof(E));
     ++sources;
   }
-  // By how much source k's row r is moved in its slot, and the bytes its copy has.
-  __device__ __forceinline__ uint32_t shift(int k, long long r) const {
-    return MOVED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[k] + r * pitch[k]) & 15) : 0u;
+  // The bytes of source k's copy of row r.
+  __device__ __forceinline__ bool last(long long r) const { return MOVED && r == rows - 1; }
+  __device__ __forceinline__ uint32_t span(int k, long long r) const {
+    return (shift[k] + row_bytes[k] + (last(r) ? 0u : 15u)) & ~15u;
   }
-  __device__ __forceinline__ uint32_t span(int k, long long r) const { return (shift(k, r) + row_bytes[k] + 15) & ~15u; }
   __device__ __forceinline__ void issue(long long r, int to) {  // one thread
-    if (r >= rows || (MOVED && r == rows - 1)) return;
+    if (r >= rows) return;
     const uint32_t bar = ptx::smem_u32(&ctrl->full[to]);
     const uint32_t at = ptx::smem_u32(slots) + to * slot_bytes;
     uint32_t total = 0;
@@ -353,7 +382,7 @@ struct Ring {
     ptx::mbar_arrive_expect_tx(bar, total);
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
-      if (k < sources) bulk_load(at + offset[k], src[k] + r * pitch[k] - shift(k, r), span(k, r), bar);
+      if (k < sources && span(k, r) > 0) bulk_load(at + offset[k], src[k] + r * pitch[k] - shift[k], span(k, r), bar);
   }
   __device__ __forceinline__ void start() {
     if (threadIdx.x == 0) {
@@ -366,21 +395,23 @@ struct Ring {
   }
   // The block's row is in its slot (false: it did not come in time).
   __device__ __forceinline__ bool wait(uint64_t limit_ns) {
-    if (!MOVED || row != rows - 1) return ptx::mbar_wait(ptx::smem_u32(&ctrl->full[slot]), phase, &ctrl->abort, limit_ns);
-    // (all threads come here together, and all have left what the slot held before)
+    const bool ok = ptx::mbar_wait(ptx::smem_u32(&ctrl->full[slot]), phase, &ctrl->abort, limit_ns);
+    if (!last(row)) return ok;
+    // (all threads come here together; a row is a whole number of 2-byte pieces)
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
       if (k < sources) {
-        const char* from = src[k] + row * pitch[k];
-        char* to = slots + static_cast<size_t>(slot) * slot_bytes + offset[k] + shift(k, row);
-        for (uint32_t b = threadIdx.x * 2; b < row_bytes[k]; b += blockDim.x * 2)
-          *reinterpret_cast<uint16_t*>(to + b) = *reinterpret_cast<const uint16_t*>(from + b);
+        const uint32_t moved = shift[k], done = span(k, row) > moved ? span(k, row) - moved : 0u;
+        const uint32_t b = done + threadIdx.x * 2;
+        if (b < row_bytes[k])
+          *reinterpret_cast<uint16_t*>(slots + static_cast<size_t>(slot) * slot_bytes + offset[k] + moved + b) =
+              *reinterpret_cast<const uint16_t*>(src[k] + row * pitch[k] + b);
       }
-    __syncthreads();
-    return true;
+    block_barrier();
+    return ok;
   }
   // Byte offset of source k's row in the slots.
-  __device__ __forceinline__ uint32_t at(int k) const { return slot * slot_bytes + offset[k] + shift(k, row); }
+  __device__ __forceinline__ uint32_t at(int k) const { return slot * slot_bytes + offset[k] + shift[k]; }
   // Nobody reads the row's slot any more: it takes the row `depth` rounds ahead.
   __device__ __forceinline__ void refill() {
     if (threadIdx.x == 0) issue(row + static_cast<long long>(depth) * gridDim.x, slot);
@@ -400,37 +431,86 @@ struct Ring {
   }
 };
 
+// The columns of a thread: vector n of VEC columns starts at first + n * step, and is the thread's if
+// that is before limit.
+struct Columns {
+  int first, step, limit;
+};
+// Rows that do not start on 16-byte boundaries (an odd number of columns) are still read and written in
+// whole vectors where every tensor has its rows moved alike (LED): `head` elements, then vectors, then
+// a tail shorter than a vector.  Head and tail belong to a warp of their own, an element per lane: it
+// runs the same row loop with VEC = NV = 1 and meets the other warps at the barriers.  A block only
+// walks rows with one head (the grid is a multiple of the rows after which it comes back), so its
+// threads keep their columns.  (Masking the first and the last vector instead made the warps that hold
+// them late to every barrier: 55 us against 49, 8192 x 2049 bf16 forward, before the other steps.)
+struct Led {
+  int head, tail;
+  bool edge;  // this thread is of the head's and the tail's warp
+  __device__ __forceinline__ Led(int cols, int vec)
+      : head(static_cast<int>(blockIdx.x * static_cast<long long>(cols) % vec)), edge(threadIdx.x >= blockDim.x - 32) {
+    head = head == 0 ? 0 : vec - head < cols ? vec - head : cols;
+    tail = (cols - head) % vec;
+  }
+  __device__ __forceinline__ Columns edges(int cols) const {
+    const int lane = threadIdx.x & 31;
+    return {lane < head ? lane : lane < head + tail ? cols - tail + lane - head : cols, 0, cols};
+  }
+  __device__ __forceinline__ Columns vectors(int cols, int vec) const {
+    return {head + static_cast<int>(threadIdx.x) * vec, static_cast<int>(blockDim.x - 32) * vec, cols - tail};
+  }
+};
+// Weights and column sums start on a 16-byte boundary whatever the rows do.
+template <typename W, int VEC, bool LED>
+__device__ __forceinline__ elem::Pack<W, VEC> column_pack(const W* at) {
+  if constexpr (LED) {
+    elem::Pack<W, VEC> raw;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) raw.v[j] = at[j];
+    return raw;
+  } else {
+    return *reinterpret_cast<const elem::Pack<W, VEC>*>(at);
+  }
+}
+template <typename W, int VEC, bool LED>
+__device__ __forceinline__ void column_load(const W* at, float (&out)[VEC]) {
+  const elem::Pack<W, VEC> raw = column_pack<W, VEC, LED>(at);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) out[j] = elem::to_float(raw.v[j]);
+}
+template <int VEC, bool LED>
+__device__ __forceinline__ void column_store(float* at, const float (&in)[VEC]) {
+  if constexpr (LED) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) at[j] = in[j];
+  } else {
+    elem::store<float, VEC>(at, in);
+  }
+}
+
 // Weights that every row meets stay in registers: gate * post and pre.
 // PER_ROW: the gate is a row's own (token or full form) and joins post in the row.
-template <typename T, typename W, int VEC, int NV, bool PER_ROW>
-__global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 3 : 1) norm_forward_ring_kernel(const NormParams p) {
-  extern __shared__ __align__(128) char smem[];
-  Ring<VEC == 1> ring(smem, p);
-  ring.template add<T>(p.y, p.ld_y, p.cols);
-  ring.template add<T>(p.res, p.ld_res, p.cols);
+template <typename T, typename W, int VEC, int NV, bool PER_ROW, bool LED, typename R>
+__device__ __forceinline__ void norm_forward_rows(const NormParams& p, char* smem, R& ring, const Columns c) {
   const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
-  if (full) ring.template add<W>(p.gate, p.ld_gate, p.cols);
-  ring.start();
-  const int tid = threadIdx.x, threads = blockDim.x;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
   float pg[NV][VEC];
   elem::Pack<W, VEC> pre[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const int col = (tid + n * threads) * VEC;
-    if (col < p.cols) {
-      elem::load<W, VEC>(static_cast<const W*>(p.post) + col, pg[n]);
-      pre[n] = *reinterpret_cast<const elem::Pack<W, VEC>*>(static_cast<const W*>(p.pre) + col);
+    const int col = c.first + n * c.step;
+    if (col < c.limit) {
+      column_load<W, VEC, LED>(static_cast<const W*>(p.post) + col, pg[n]);
+      pre[n] = column_pack<W, VEC, LED>(static_cast<const W*>(p.pre) + col);
       if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
         float g[VEC];
-        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
+        column_load<W, VEC, LED>(static_cast<const W*>(p.gate) + col, g);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) pg[n][j] *= g[j];
       }
     }
   }
   int levels = 0;
-  while ((32 << levels) < threads) ++levels;
+  while ((32 << levels) < static_cast<int>(blockDim.x)) ++levels;
   bool ok = true;
   // (rows <= 2^30: row numbers cannot overflow)
   for (; ring.row < p.rows; ring.next()) {
@@ -446,8 +526,8 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     float ss[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         y[n] = *reinterpret_cast<const elem::Pack<T, VEC>*>(y_row + col);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) ss[0] += elem::to_float(y[n].v[j]) * elem::to_float(y[n].v[j]);
@@ -459,8 +539,8 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     ss[0] = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         float r[VEC], g[VEC];
         elem::load<T, VEC>(r_row + col, r);
         if (full) elem::load<W, VEC>(g_row + col, g);
@@ -477,57 +557,44 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     ring.refill();
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         float out[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) out[j] = h[n][j] * r2 * elem::to_float(pre[n].v[j]);
-        const long long at = row * p.cols + col;
-        elem::store<T, VEC>(static_cast<T*>(p.h) + at, h[n]);
-        elem::store<T, VEC>(static_cast<T*>(p.n) + at, out);
+        elem::store<T, VEC>(static_cast<T*>(p.h) + row * p.cols + col, h[n]);
+        elem::store<T, VEC>(static_cast<T*>(p.n) + row * p.cols + col, out);
       }
     }
-    if (p.stats != nullptr && tid == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(r1, r2);
+    if (p.stats != nullptr && threadIdx.x == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(r1, r2);
   }
   if (!ok) ring.give_up(p.status);
 }
-
-// The sums of norm_backward_kernel.  A gate per channel leaves the sum over rows, so that one sum
-// S = sum of dh' a gives both dpost = gate S and dgate = post S.
-template <typename T, typename W, int VEC, int NV, bool PER_ROW>
-__global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 256 ? 2 : 1) norm_backward_ring_kernel(const NormParams p) {
-  extern __shared__ __align__(128) char smem[];
-  Ring<VEC == 1> ring(smem, p);
-  ring.template add<T>(p.y, p.ld_y, p.cols);
-  ring.template add<T>(p.res, p.ld_res, p.cols);
-  ring.template add<T>(p.dh, p.ld_dh, p.cols);
-  ring.template add<T>(p.dn, p.ld_dn, p.cols);
+template <typename T, typename W, int VEC, int NV, bool PER_ROW, bool LED, typename R>
+__device__ __forceinline__ void norm_backward_rows(const NormParams& p, char* smem, R& ring, const Columns c) {
   const bool full = PER_ROW && p.gate_form == TNX_GATE_FULL;
-  if (full) ring.template add<W>(p.gate, p.ld_gate, p.cols);
-  ring.start();
-  const int tid = threadIdx.x, threads = blockDim.x;
   const float inv_cols = 1.f / static_cast<float>(p.cols);
   float s_a[NV][VEC], s_pre[NV][VEC];  // column sums: dh' a (times the row's gate), dn h r2
   float pg[NV][VEC];
   elem::Pack<W, VEC> pre[NV];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const int col = (tid + n * threads) * VEC;
+    const int col = c.first + n * c.step;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s_a[n][j] = s_pre[n][j] = 0.f;
-    if (col < p.cols) {
-      elem::load<W, VEC>(static_cast<const W*>(p.post) + col, pg[n]);
-      pre[n] = *reinterpret_cast<const elem::Pack<W, VEC>*>(static_cast<const W*>(p.pre) + col);
+    if (col < c.limit) {
+      column_load<W, VEC, LED>(static_cast<const W*>(p.post) + col, pg[n]);
+      pre[n] = column_pack<W, VEC, LED>(static_cast<const W*>(p.pre) + col);
       if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
         float g[VEC];
-        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
+        column_load<W, VEC, LED>(static_cast<const W*>(p.gate) + col, g);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) pg[n][j] *= g[j];
       }
     }
   }
   int levels = 0;
-  while ((32 << levels) < threads) ++levels;
+  while ((32 << levels) < static_cast<int>(blockDim.x)) ++levels;
   bool ok = true;
   // (rows <= 2^30: row numbers cannot overflow)
   for (; ring.row < p.rows; ring.next()) {
@@ -547,8 +614,8 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     float s_uh[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         float g[VEC], u[VEC];
         y[n] = *reinterpret_cast<const elem::Pack<T, VEC>*>(y_row + col);
         elem::load<T, VEC>(r_row + col, h[n]);
@@ -569,8 +636,8 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     float s_va = 0.f, s_g = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         float g[VEC], u[VEC], d[VEC], dg[VEC];
         elem::load<T, VEC>(dh_row + col, d);
         elem::load<T, VEC>(dn_row + col, u);
@@ -589,9 +656,8 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
           h[n][j] = gate * dh * pg[n][j];  // (v from here on)
           s_va += h[n][j] * a;
         }
-        const long long at = row * p.cols + col;
-        elem::store<T, VEC>(static_cast<T*>(p.dres) + at, d);
-        if (full) elem::store<W, VEC>(static_cast<W*>(p.dgate) + at, dg);
+        elem::store<T, VEC>(static_cast<T*>(p.dres) + row * p.cols + col, d);
+        if (full) elem::store<W, VEC>(static_cast<W*>(p.dgate) + row * p.cols + col, dg);
       }
     }
     float both[PER_ROW ? 2 : 1] = {s_va};
@@ -601,36 +667,79 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), max_threads(VEC, NV) == 
     const float m = both[0] * inv_cols;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int col = (tid + n * threads) * VEC;
-      if (col < p.cols) {
+      const int col = c.first + n * c.step;
+      if (col < c.limit) {
         float out[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) out[j] = r1 * (h[n][j] - elem::to_float(y[n].v[j]) * r1 * m);
         elem::store<T, VEC>(static_cast<T*>(p.dy) + row * p.cols + col, out);
       }
     }
-    if (PER_ROW && !full && tid == 0) static_cast<W*>(p.dgate)[row] = elem::from_float<W>(both[PER_ROW ? 1 : 0]);
+    if (PER_ROW && !full && threadIdx.x == 0) static_cast<W*>(p.dgate)[row] = elem::from_float<W>(both[PER_ROW ? 1 : 0]);
   }
   if (!ok) ring.give_up(p.status);
   float* mine = p.partial + static_cast<long long>(blockIdx.x) * p.sums * p.cols;
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    const int col = (tid + n * threads) * VEC;
-    if (col < p.cols) {
+    const int col = c.first + n * c.step;
+    if (col < c.limit) {
       if (!PER_ROW && p.gate_form == TNX_GATE_CHANNEL) {
         float g[VEC], post[VEC];
-        elem::load<W, VEC>(static_cast<const W*>(p.gate) + col, g);
-        elem::load<W, VEC>(static_cast<const W*>(p.post) + col, post);
+        column_load<W, VEC, LED>(static_cast<const W*>(p.gate) + col, g);
+        column_load<W, VEC, LED>(static_cast<const W*>(p.post) + col, post);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           post[j] *= s_a[n][j];
           s_a[n][j] *= g[j];
         }
-        elem::store<float, VEC>(mine + 2 * static_cast<long long>(p.cols) + col, post);
+        column_store<VEC, LED>(mine + 2 * static_cast<long long>(p.cols) + col, post);
       }
-      elem::store<float, VEC>(mine + col, s_a[n]);
-      elem::store<float, VEC>(mine + p.cols + col, s_pre[n]);
+      column_store<VEC, LED>(mine + col, s_a[n]);
+      column_store<VEC, LED>(mine + p.cols + col, s_pre[n]);
     }
+  }
+}
+template <typename T, typename W, int VEC, int NV, bool PER_ROW, bool LED>
+__global__ void __launch_bounds__(ring_threads(VEC, NV, LED), ring_blocks(VEC, NV, LED, false)) norm_forward_ring_kernel(const NormParams p) {
+  extern __shared__ __align__(128) char smem[];
+  Ring<VEC == 1 || LED> ring(smem, p);
+  ring.template add<T>(p.y, p.ld_y, p.cols);
+  ring.template add<T>(p.res, p.ld_res, p.cols);
+  if (PER_ROW && p.gate_form == TNX_GATE_FULL) ring.template add<W>(p.gate, p.ld_gate, p.cols);
+  ring.start();
+  if constexpr (LED) {
+    const Led led(p.cols, VEC);
+    if (led.edge)
+      norm_forward_rows<T, W, 1, 1, PER_ROW, false>(p, smem, ring, led.edges(p.cols));
+    else
+      norm_forward_rows<T, W, VEC, NV, PER_ROW, true>(p, smem, ring, led.vectors(p.cols, VEC));
+  } else {
+    norm_forward_rows<T, W, VEC, NV, PER_ROW, false>(
+        p, smem, ring, {static_cast<int>(threadIdx.x) * VEC, static_cast<int>(blockDim.x) * VEC, p.cols});
+  }
+}
+
+// The sums of norm_backward_kernel.  A gate per channel leaves the sum over rows, so that one sum
+// S = sum of dh' a gives both dpost = gate S and dgate = post S.
+template <typename T, typename W, int VEC, int NV, bool PER_ROW, bool LED>
+__global__ void __launch_bounds__(ring_threads(VEC, NV, LED), ring_blocks(VEC, NV, LED, true)) norm_backward_ring_kernel(const NormParams p) {
+  extern __shared__ __align__(128) char smem[];
+  Ring<VEC == 1 || LED> ring(smem, p);
+  ring.template add<T>(p.y, p.ld_y, p.cols);
+  ring.template add<T>(p.res, p.ld_res, p.cols);
+  ring.template add<T>(p.dh, p.ld_dh, p.cols);
+  ring.template add<T>(p.dn, p.ld_dn, p.cols);
+  if (PER_ROW && p.gate_form == TNX_GATE_FULL) ring.template add<W>(p.gate, p.ld_gate, p.cols);
+  ring.start();
+  if constexpr (LED) {
+    const Led led(p.cols, VEC);
+    if (led.edge)
+      norm_backward_rows<T, W, 1, 1, PER_ROW, false>(p, smem, ring, led.edges(p.cols));
+    else
+      norm_backward_rows<T, W, VEC, NV, PER_ROW, true>(p, smem, ring, led.vectors(p.cols, VEC));
+  } else {
+    norm_backward_rows<T, W, VEC, NV, PER_ROW, false>(
+        p, smem, ring, {static_cast<int>(threadIdx.x) * VEC, static_cast<int>(blockDim.x) * VEC, p.cols});
   }
 }
 
@@ -662,15 +771,19 @@ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // Vector width, vectors per thread, threads and rows of a block for one call; depth > 0: a ring
 // kernel with that many rows in flight and `smem` bytes per block.
+// led: rows do not start on 16-byte boundaries, but in all tensors alike.
 struct NormShape {
   int vec, nv, threads, rows, depth, smem, blocks;
+  int period;  // blocks that walk rows are a multiple of this
+  bool led;
 };
 
 // A row's threads: one vector each while a block holds the row, then two, four, ... each.
-void pick_shape(const tnx_norm_problem& p, bool aligned, bool backward, NormShape* s) {
+// aligned: all rows start on 16-byte boundaries.  alike: all tensors do, and row r of each starts
+// r * cols elements (to a whole vector) after that.
+void pick_shape(const tnx_norm_problem& p, bool aligned, bool alike, bool backward, NormShape* s) {
   const int wide = p.dtype == TNX_F32 ? 4 : 8;
-  s->vec = aligned && p.cols % wide == 0 ? wide : 1;
-  const int vectors = cdiv(p.cols, s->vec);
+  aligned = aligned && p.cols % wide == 0;
   // Rows in flight: what fits a third (forward) or half (backward) of an SM's shared memory, four
   // at most; and enough rows that a block has several.
   const int size = p.dtype == TNX_F32 ? 4 : 2, wsize = p.weight_dtype == TNX_F32 ? 4 : 2;
@@ -684,21 +797,37 @@ void pick_shape(const tnx_norm_problem& p, bool aligned, bool backward, NormShap
     if (s->depth > kMaxDepth) s->depth = kMaxDepth;
     if (s->depth < 2) s->depth = 0;
   }
+  // Whole vectors against single elements, fp32 weights and a channel gate, us forward/backward:
+  // 4000 x 7001 bf16 59/115 against 119/342, 32768 x 301 bf16 41/82 against 86/131; 50000 x 67 fp32
+  // 35/64 against 37/61, no gain: rows that short are a few warps either way.  (The longest rows do
+  // not fit 480 threads.)
+  const int longest = 480 * (wide == 8 ? 4 : 8) * wide;
+  s->led = !aligned && alike && s->depth > 0 && p.cols >= 16 * wide && p.cols <= longest;
+  s->vec = aligned || s->led ? wide : 1;
+  const int vectors = s->led ? p.cols / wide : cdiv(p.cols, s->vec);
   s->nv = 1;
-  while (cdiv(vectors, s->nv) > max_threads(s->vec, s->nv)) s->nv *= 2;
+  while (cdiv(vectors, s->nv) > max_threads(s->vec, s->nv, s->led)) s->nv *= 2;
   s->threads = cdiv(cdiv(vectors, s->nv), 32) * 32;
+  if (s->led) s->threads += 32;
   s->rows = backward || s->depth > 0 ? 1 : s->threads >= 256 ? 1 : 256 / s->threads;
   s->smem = s->depth > 0 ? kCtrlBytes + s->depth * slot : 0;
-  // Blocks that walk rows: as many as are resident, by shared memory and by threads (at 64
-  // registers forward, 128 backward), never more than there are rows.
+  // Blocks that walk rows: as many as can be resident (resident_blocks has the last word), never more
+  // than there are rows.
   int per_sm = 2;
   if (s->depth > 0) {
-    const int by_smem = (kMaxDynamicSmem + 1024) / (s->smem + 1024), by_regs = (backward ? 512 : 768) / s->threads;
+    const int by_smem = (kMaxDynamicSmem + 1024) / (s->smem + 1024), by_regs = (backward ? 768 : 1024) / s->threads;
     per_sm = by_smem < by_regs ? by_smem : by_regs;
     if (per_sm < 1) per_sm = 1;
-    if (per_sm > 8) per_sm = 8;
+    if (per_sm > 16) per_sm = 16;
   }
   s->blocks = p.rows < per_sm * sm_count() ? p.rows : per_sm * sm_count();
+  s->period = 1;
+  if (s->depth > 0 && !aligned) {
+    int period = wide;  // rows after which all tensors are as far behind a boundary again
+    while (s->led && period > 1 && period / 2 * static_cast<long long>(p.cols) % wide == 0) period /= 2;
+    s->period = period;
+    s->blocks -= s->blocks % period;  // (there are at least four rows per SM)
+  }
 }
 
 int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs, int count,
@@ -724,16 +853,18 @@ int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs
     return TNX_ERR_INVALID;
   }
   const int wide = p->dtype == TNX_F32 ? 4 : 8;
-  bool aligned = true;
+  bool aligned = true, alike = true;
   for (int i = 0; i < count; ++i) aligned = aligned && (reinterpret_cast<uintptr_t>(ptrs[i]) & 15u) == 0;
   for (int i = 0; i < pitch_count; ++i) {
     if (pitches[i] < 0) {
       set_error("negative row pitches are not supported");
       return TNX_ERR_INVALID;
     }
-    aligned = aligned && pitches[i] % wide == 0;
+    alike = alike && pitches[i] % wide == p->cols % wide;
   }
-  pick_shape(*p, aligned, backward, s);
+  alike = alike && aligned;
+  for (int i = 0; i < pitch_count; ++i) aligned = aligned && pitches[i] % wide == 0;
+  pick_shape(*p, aligned, alike, backward, s);
   return TNX_OK;
 }
 
@@ -741,14 +872,20 @@ using NormFn = void (*)(const NormParams);
 
 // A kernel: plain, or a ring kernel with a gate per row or not.
 struct Pick {
-  bool ring, per_row, backward;
+  bool ring, per_row, led, backward;
 };
+template <typename T, typename W, int VEC, int NV, bool LED>
+NormFn pick_ring(const Pick& k) {
+  if (k.per_row)
+    return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, true, LED> : norm_forward_ring_kernel<T, W, VEC, NV, true, LED>;
+  return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, false, LED> : norm_forward_ring_kernel<T, W, VEC, NV, false, LED>;
+}
 template <typename T, typename W, int VEC, int NV>
 NormFn pick_form(const Pick& k) {
   if (!k.ring) return k.backward ? norm_backward_kernel<T, W, VEC, NV> : norm_forward_kernel<T, W, VEC, NV>;
-  if (k.per_row)
-    return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, true> : norm_forward_ring_kernel<T, W, VEC, NV, true>;
-  return k.backward ? norm_backward_ring_kernel<T, W, VEC, NV, false> : norm_forward_ring_kernel<T, W, VEC, NV, false>;
+  if constexpr (VEC > 1)
+    if (k.led) return pick_ring<T, W, VEC, NV, true>(k);
+  return pick_ring<T, W, VEC, NV, false>(k);
 }
 template <typename T, typename W, int VEC>
 NormFn pick_nv(int nv, const Pick& k) {
@@ -769,7 +906,7 @@ NormFn pick_vec(const NormShape& s, const Pick& k) {
   return s.vec == 1 ? pick_nv<T, W, 1>(s.nv, k) : pick_nv<T, W, WIDE>(s.nv, k);
 }
 NormFn pick_norm(const tnx_norm_problem& p, const NormShape& s, bool backward) {
-  const Pick k = {s.depth > 0, p.gate_form == TNX_GATE_TOKEN || p.gate_form == TNX_GATE_FULL, backward};
+  const Pick k = {s.depth > 0, p.gate_form == TNX_GATE_TOKEN || p.gate_form == TNX_GATE_FULL, s.led, backward};
   const bool same = p.weight_dtype == p.dtype;
   if (p.dtype == TNX_F32) return pick_vec<float, float, 4>(s, k);
   if (p.dtype == TNX_F16)
@@ -780,10 +917,13 @@ NormFn pick_norm(const tnx_norm_problem& p, const NormShape& s, bool backward) {
 
 // The column sums of the backward pass at most: those of the form with the most blocks.
 int most_blocks(const tnx_norm_problem& p) {
-  NormShape plain, ring;
-  pick_shape(p, false, true, &plain);
-  pick_shape(p, true, true, &ring);
-  return plain.blocks > ring.blocks ? plain.blocks : ring.blocks;
+  int most = 0;
+  for (int form = 0; form < 3; ++form) {
+    NormShape s;
+    pick_shape(p, form == 1, form == 2, true, &s);
+    if (s.blocks > most) most = s.blocks;
+  }
+  return most;
 }
 
 // Opts a ring kernel into its dynamic shared memory, once per (kernel, device).
@@ -812,6 +952,17 @@ int allow_smem(NormFn fn, int bytes) {
   return TNX_ERR_CUDA;
 }
 
+// The blocks of a ring kernel that are resident together: one that started only after another had
+// finished would double the time.
+int resident_blocks(NormFn fn, const NormShape& s) {
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, reinterpret_cast<const void*>(fn), s.threads, s.smem) != cudaSuccess)
+    (void)cudaGetLastError();
+  if (per_sm < 1 || per_sm * sm_count() >= s.blocks) return s.blocks;
+  const int blocks = per_sm * sm_count();
+  return blocks - blocks % s.period;
+}
+
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return TNX_OK;
@@ -836,11 +987,11 @@ int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, cons
   using namespace tnx;
   const void* ptrs[] = {y, residual, post_weight, pre_weight, h, n, gate};
   NormShape s;
-  long long pitches[3] = {0, 0, 0};
+  long long pitches[3] = {};
   if (problem != nullptr) {
     pitches[0] = problem->stride_y;
     pitches[1] = problem->stride_residual;
-    pitches[2] = problem->gate_form == TNX_GATE_FULL ? problem->stride_gate : 0;
+    pitches[2] = problem->gate_form == TNX_GATE_FULL ? problem->stride_gate : problem->cols;
   }
   int rc = norm_check(problem, false, ptrs, problem != nullptr && problem->gate_form == TNX_GATE_TOKEN ? 6 : 7,
                       pitches, 3, &s);
@@ -878,7 +1029,7 @@ int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, cons
   p.timeout_ns = bounded_wait_limit_ns();
   rc = allow_smem(fn, s.smem);
   if (rc != TNX_OK) return rc;
-  fn<<<s.depth > 0 ? s.blocks : cdiv(p.rows, s.rows), dim3(s.threads, s.rows), s.smem, static_cast<cudaStream_t>(stream)>>>(p);
+  fn<<<s.depth > 0 ? resident_blocks(fn, s) : cdiv(p.rows, s.rows), dim3(s.threads, s.rows), s.smem, static_cast<cudaStream_t>(stream)>>>(p);
   return launched("gated residual norm");
 }
 
@@ -895,7 +1046,7 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
   if (problem != nullptr) {
     pitches[2] = problem->stride_y;
     pitches[3] = problem->stride_residual;
-    pitches[4] = problem->gate_form == TNX_GATE_FULL ? problem->stride_gate : 0;
+    pitches[4] = problem->gate_form == TNX_GATE_FULL ? problem->stride_gate : problem->cols;
   }
   int rc = norm_check(problem, true, ptrs, problem != nullptr && problem->gate_form == TNX_GATE_TOKEN ? 8 : 10,
                       pitches, 5, &s);
@@ -905,7 +1056,7 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
     return TNX_ERR_INVALID;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int blocks = s.blocks;
+  int blocks = s.blocks;
   if (blocks > 0) {
     if (dh == nullptr || dn == nullptr || y == nullptr || residual == nullptr || post_weight == nullptr ||
         pre_weight == nullptr || stats == nullptr || dy == nullptr || dresidual == nullptr ||
@@ -956,6 +1107,7 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
     p.timeout_ns = bounded_wait_limit_ns();
     rc = allow_smem(fn, s.smem);
     if (rc != TNX_OK) return rc;
+    if (s.depth > 0) blocks = resident_blocks(fn, s);
     fn<<<blocks, s.threads, s.smem, st>>>(p);
     rc = launched("gated residual norm, backward");
     if (rc != TNX_OK) return rc;
