@@ -135,6 +135,19 @@ def test_partial_vectors_leave_their_neighbours_alone(dtype, wtype):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_one_row_for_many():
+    """Rows that repeat (a pitch of zero) or overlap, off the 16-byte boundaries and on them."""
+    for d in (301, 304):
+        case = make(700, d, bf16, bf16, "full", seed=9)
+        args = on_gpu(case, False)
+        store = torch.randn(3 * 699 + d, device=DEV).to(bf16)
+        views = [args[0][:1].expand(700, d), store.as_strided((700, d), (3, 1)), args[2], args[3], args[4][:1].expand(700, d)]
+        want = tnx.gated_residual_norm(*[v.contiguous() for v in views])
+        got = tnx.gated_residual_norm(*views)
+        for a, b in zip(want, got):   # (another order of a row's sum: the last bit may differ)
+            torch.testing.assert_close(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
 def test_rows_apart():
     case = make(800, 520, bf16, bf16, "full", seed=4)
     padded = lambda t: torch.nn.functional.pad(t.to(DEV), (0, 24))[:, :520]  # noqa: E731

@@ -779,20 +779,25 @@ struct NormShape {
 };
 
 // A row's threads: one vector each while a block holds the row, then two, four, ... each.
-// aligned: all rows start on 16-byte boundaries.  alike: all tensors do, and row r of each starts
-// r * cols elements (to a whole vector) after that.
-void pick_shape(const tnx_norm_problem& p, bool aligned, bool alike, bool backward, NormShape* s) {
+// How the rows lie.
+enum Rows {
+  kAligned,  // all start on 16-byte boundaries
+  kAlike,    // all tensors do, and row r of each starts r * cols elements (to a whole vector) after that
+  kAnyhow,
+  kRepeated  // anyhow, and a tensor's rows overlap: a copy to the next boundary could pass its end
+};
+void pick_shape(const tnx_norm_problem& p, Rows how, bool backward, NormShape* s) {
   const int wide = p.dtype == TNX_F32 ? 4 : 8;
-  aligned = aligned && p.cols % wide == 0;
+  const bool aligned = how == kAligned;
   // Rows in flight: what fits a third (forward) or half (backward) of an SM's shared memory, four
   // at most; and enough rows that a block has several.
   const int size = p.dtype == TNX_F32 ? 4 : 2, wsize = p.weight_dtype == TNX_F32 ? 4 : 2;
   const int slot = (backward ? 4 : 2) * static_cast<int>(ring_row_bytes(p.cols, size)) +
                    (p.gate_form == TNX_GATE_FULL ? static_cast<int>(ring_row_bytes(p.cols, wsize)) : 0);
-  const int budget = kMaxDynamicSmem / (backward ? 2 : 3) - 1024;
+  const int share = kMaxDynamicSmem / (backward ? 2 : 3) - 1024;
   s->depth = 0;
-  if (p.rows >= 4 * sm_count()) {
-    s->depth = (budget - kCtrlBytes) / slot;
+  if (p.rows >= 4 * sm_count() && how != kRepeated) {
+    s->depth = (share - kCtrlBytes) / slot;
     if (s->depth < 2) s->depth = (kMaxDynamicSmem - kCtrlBytes) / slot;
     if (s->depth > kMaxDepth) s->depth = kMaxDepth;
     if (s->depth < 2) s->depth = 0;
@@ -802,7 +807,7 @@ void pick_shape(const tnx_norm_problem& p, bool aligned, bool alike, bool backwa
   // 35/64 against 37/61, no gain: rows that short are a few warps either way.  (The longest rows do
   // not fit 480 threads.)
   const int longest = 480 * (wide == 8 ? 4 : 8) * wide;
-  s->led = !aligned && alike && s->depth > 0 && p.cols >= 16 * wide && p.cols <= longest;
+  s->led = how == kAlike && s->depth > 0 && p.cols >= 16 * wide && p.cols <= longest;
   s->vec = aligned || s->led ? wide : 1;
   const int vectors = s->led ? p.cols / wide : cdiv(p.cols, s->vec);
   s->nv = 1;
@@ -853,18 +858,18 @@ int norm_check(const tnx_norm_problem* p, bool backward, const void* const* ptrs
     return TNX_ERR_INVALID;
   }
   const int wide = p->dtype == TNX_F32 ? 4 : 8;
-  bool aligned = true, alike = true;
-  for (int i = 0; i < count; ++i) aligned = aligned && (reinterpret_cast<uintptr_t>(ptrs[i]) & 15u) == 0;
+  bool based = true, aligned = p->cols % wide == 0, alike = true, apart = true;
+  for (int i = 0; i < count; ++i) based = based && (reinterpret_cast<uintptr_t>(ptrs[i]) & 15u) == 0;
   for (int i = 0; i < pitch_count; ++i) {
     if (pitches[i] < 0) {
       set_error("negative row pitches are not supported");
       return TNX_ERR_INVALID;
     }
+    aligned = aligned && pitches[i] % wide == 0;
     alike = alike && pitches[i] % wide == p->cols % wide;
+    apart = apart && pitches[i] >= p->cols;
   }
-  alike = alike && aligned;
-  for (int i = 0; i < pitch_count; ++i) aligned = aligned && pitches[i] % wide == 0;
-  pick_shape(*p, aligned, alike, backward, s);
+  pick_shape(*p, based && aligned ? kAligned : !apart ? kRepeated : based && alike ? kAlike : kAnyhow, backward, s);
   return TNX_OK;
 }
 
@@ -918,9 +923,9 @@ NormFn pick_norm(const tnx_norm_problem& p, const NormShape& s, bool backward) {
 // The column sums of the backward pass at most: those of the form with the most blocks.
 int most_blocks(const tnx_norm_problem& p) {
   int most = 0;
-  for (int form = 0; form < 3; ++form) {
+  for (const Rows how : {kAligned, kAlike, kAnyhow, kRepeated}) {
     NormShape s;
-    pick_shape(p, form == 1, form == 2, true, &s);
+    pick_shape(p, how, true, &s);
     if (s.blocks > most) most = s.blocks;
   }
   return most;
