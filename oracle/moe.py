@@ -10,8 +10,8 @@ import torch
 
 def route_oracle(logits, top_k, scoring="softmax", bias=None, groups=1, top_groups=1,
                  renormalize=True, scale=1.0):
-    """(weights, ids, scores) in 64 bits, one token at a time; NaN ranks last, ties to the lowest
-    index, a row of -inf scores 0."""
+    """(weights, ids, scores) in 64 bits, one token at a time; NaN ranks last and the others are told
+    apart without it, ties go to the lowest index, a row of -inf scores 0."""
     z = logits.double()
     t, n = z.shape
     if scoring == "softmax":
@@ -20,9 +20,12 @@ def route_oracle(logits, top_k, scoring="softmax", bias=None, groups=1, top_grou
         e = torch.exp(z - top)
         total = e.sum(1, keepdim=True)
         s = torch.where(total == 0, torch.zeros_like(e), e / total)
+        e = torch.where(z == top, torch.ones_like(e), e)  # (infinity minus infinity)
+        total = e.nansum(1, keepdim=True)
+        rank_by = torch.where(total == 0, e * 0, e / total)
     else:
-        s = torch.sigmoid(z)
-    choice = z if bias is None and groups in (1, top_groups) else s if bias is None else s + bias.double()
+        s = rank_by = torch.sigmoid(z)
+    choice = z if bias is None and groups in (1, top_groups) else rank_by if bias is None else rank_by + bias.double()
     ids = torch.empty(t, top_k, dtype=torch.int64)
     size = n // groups
     for i in range(t):
@@ -31,7 +34,7 @@ def route_oracle(logits, top_k, scoring="softmax", bias=None, groups=1, top_grou
         if groups > top_groups:
             best = []
             for g in range(groups):
-                part = sorted(c[g * size:(g + 1) * size], reverse=True)
+                part = sorted((float("-inf") if v != v else v for v in c[g * size:(g + 1) * size]), reverse=True)
                 best.append((-sum(part[:2]), g))
             kept = [g for _, g in sorted(best)[:top_groups]]
             open_ = {g * size + j for g in kept for j in range(size)}

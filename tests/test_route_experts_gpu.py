@@ -190,3 +190,47 @@ def test_refusals():
         tnx.route_experts(torch.zeros(1, 513, device=DEV), 2)
     with pytest.raises(RuntimeError, match="CUDA"):
         tnx.route_experts(x.cpu(), 2)
+
+
+def nan_logits(at):
+    """Rows with a NaN among good logits, two of them, only four numbers, a +inf, and copies in front."""
+    logits = torch.randn(6, 256, generator=torch.Generator().manual_seed(at))
+    nan = float("nan")
+    logits[0, at] = nan
+    logits[1, [at, (at + 1) % 256]] = nan
+    keep = logits[2, [3, 77, 130, 201]].clone()
+    logits[2] = nan
+    logits[2, [3, 77, 130, 201]] = keep
+    logits[3, [at, 90]] = torch.tensor([nan, float("inf")])
+    logits[4, :16] = 0.5
+    logits[4, 200 + at % 50] = nan
+    return logits
+
+
+@pytest.mark.parametrize("at", [0, 31, 200, 255])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("form", ["bias", "groups", "both", "none"])
+def test_nan_ranks_last_however_experts_are_chosen(form, scoring, at):
+    """Choices by the scores of the other experts; the oracle leaves a NaN out of their sum."""
+    logits = nan_logits(at)
+    bias = 0.01 * torch.randn(256, generator=torch.Generator().manual_seed(1)) if form in ("bias", "both") else None
+    groups = dict(num_groups=8, top_groups=3) if form in ("groups", "both") else {}
+    for k in (1, 8):
+        weights, ids = tnx.route_experts(logits.to(DEV), k, scoring=scoring,
+                                         bias=None if bias is None else bias.to(DEV), **groups)
+        w, want, _ = O.route_oracle(logits, k, scoring, bias, groups.get("num_groups", 1), groups.get("top_groups", 1))
+        assert torch.equal(ids.cpu().long(), want)
+        picked = logits.gather(1, want)
+        good = [0, 1, 4, 5]
+        assert torch.isfinite(picked[good]).all()
+        torch.testing.assert_close(weights.cpu().double()[good], w[good], rtol=WEIGHT_RTOL, atol=1e-37)
+
+
+def test_scores_next_to_a_nan_are_nan_unless_renormalised():
+    logits = nan_logits(7)
+    for kw in ({}, {"bias": torch.zeros(256, device=DEV)}):
+        for scoring, lost in (("softmax", True), ("sigmoid", False)):
+            w, ids = tnx.route_experts(logits.to(DEV), 4, scoring=scoring, renormalize=False, **kw)
+            assert torch.isnan(w[0]).all().item() is lost
+            assert 7 not in ids[0].tolist()
+            assert torch.isfinite(tnx.route_experts(logits.to(DEV), 4, scoring=scoring, **kw)[0][0]).all()

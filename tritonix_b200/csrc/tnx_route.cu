@@ -82,7 +82,9 @@ __device__ __forceinline__ unsigned long long warp_key_max(unsigned long long k)
 }
 
 // Scores of the lane's experts in F = float or double.  A row of -infinities alone scores 0.
-template <typename F, int VPT>
+// TO_CHOOSE: a NaN is left out of the softmax's sum, so that the others can still be told apart by
+// their scores, and infinity is the limit of a large logit.
+template <typename F, int VPT, bool TO_CHOOSE = false>
 __device__ __forceinline__ void scores(const float (&l)[VPT], int experts, int lane, bool softmax, float row_max,
                                        F (&s)[VPT]) {
   if (softmax) {
@@ -91,7 +93,8 @@ __device__ __forceinline__ void scores(const float (&l)[VPT], int experts, int l
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       s[j] = j * 32 + lane < experts ? exp(static_cast<F>(l[j]) - static_cast<F>(top)) : static_cast<F>(0);
-      sum += s[j];
+      if (TO_CHOOSE && l[j] == top) s[j] = static_cast<F>(1);  // (infinity minus infinity)
+      if (!TO_CHOOSE || s[j] == s[j]) sum += s[j];
     }
     sum = warp_sum(sum);
     const F inv = sum == static_cast<F>(0) ? static_cast<F>(0) : static_cast<F>(1) / sum;
@@ -104,9 +107,10 @@ __device__ __forceinline__ void scores(const float (&l)[VPT], int experts, int l
 }
 
 // Scores that only take part in the choice: fast exponential and division (see the bound on their
-// error in route_kernel).
+// error in route_kernel).  False where the row's sum is not a number, and no score with it: a logit is
+// NaN or infinity.
 template <int VPT>
-__device__ __forceinline__ void quick_scores(const float (&l)[VPT], int experts, int lane, bool softmax, float row_max,
+__device__ __forceinline__ bool quick_scores(const float (&l)[VPT], int experts, int lane, bool softmax, float row_max,
                                              float (&s)[VPT]) {
   if (softmax) {
     float sum = 0.f;
@@ -120,10 +124,11 @@ __device__ __forceinline__ void quick_scores(const float (&l)[VPT], int experts,
     const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) s[j] *= inv;
-  } else {
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) s[j] = __fdividef(1.f, 1.f + __expf(-l[j]));
+    return sum == sum;
   }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) s[j] = __fdividef(1.f, 1.f + __expf(-l[j]));
+  return true;
 }
 
 // Which groups stay open, as a bit mask the whole warp agrees on, by the sum of each group's two
@@ -191,7 +196,7 @@ __device__ __noinline__ int choose_exactly(const float* logits, const RouteParam
 #pragma unroll
   for (int j = 0; j < VPT; ++j) l[j] = logits[j * 32 + lane];
   double c[VPT];
-  scores<double, VPT>(l, p.experts, lane, p.scoring == TNX_SCORE_SOFTMAX, row_max, c);
+  scores<double, VPT, true>(l, p.experts, lane, p.scoring == TNX_SCORE_SOFTMAX, row_max, c);
   unsigned open = kAll;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
   bool unsure = false;
   if (biased || p.groups > 1) {  // (otherwise the logits order the experts)
     float c[VPT];
-    quick_scores<VPT>(l, p.experts, lane, softmax, row_max, c);
+    unsure = !quick_scores<VPT>(l, p.experts, lane, softmax, row_max, c);
     float top_score = 1.f;
     if (softmax) {
       top_score = c[0];
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       __syncwarp();
       float gap;
       open = open_groups(sh_choice, p.groups, static_cast<int>(p.group_size), p.top_groups, lane, &gap);
-      unsure = !(gap > 4.f * eps);  // (two choices on each side)
+      unsure = unsure || !(gap > 4.f * eps);  // (two choices on each side)
     }
     if (biased) {
 #pragma unroll

@@ -64,8 +64,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     the chosen experts' scores, divided by their sum if ``renormalize``, times ``scale``.
 
     Experts are told apart as in 64-bit arithmetic, however close.  An expert whose logit is -inf
-    has the score 0 (a row of nothing else has the weights 0); a NaN logit ranks last.  ``ids`` are
-    always distinct and in range."""
+    has the score 0 (a row of nothing else has the weights 0).  A NaN logit ranks last, and the other
+    experts are told apart as if it were not there; a softmax that is not renormalised still gives
+    its token NaN weights.  ``ids`` are always distinct and in range."""
     key = (_cabi.signature(logits, bias), top_k, scoring, num_groups, top_groups, renormalize, scale)
     problem = _route_problems.get(key)
     if problem is None:
