@@ -55,6 +55,7 @@ def route_gradient_oracle(logits, ids, dweights, scoring, renormalize, scale):
     z, dw = logits.double(), dweights.double() * scale
     s = torch.softmax(z, 1) if scoring == "softmax" else torch.sigmoid(z)
     picked = s.gather(1, ids)
+    rest = torch.sigmoid(-z)  # 1 - sigmoid, to its own last place
     if renormalize:
         total = picked.sum(1, keepdim=True)
         r = picked / total
@@ -64,7 +65,7 @@ def route_gradient_oracle(logits, ids, dweights, scoring, renormalize, scale):
     full = torch.zeros_like(s).scatter_(1, ids, ds)
     if scoring == "softmax":
         return s * (full - (full * s).sum(1, keepdim=True))
-    return full * s * (1 - s)
+    return full * s * rest
 
 
 # -------------------------------------------------------------------------------------- norm

@@ -234,3 +234,59 @@ def test_scores_next_to_a_nan_are_nan_unless_renormalised():
             assert torch.isnan(w[0]).all().item() is lost
             assert 7 not in ids[0].tolist()
             assert torch.isfinite(tnx.route_experts(logits.to(DEV), 4, scoring=scoring, **kw)[0][0]).all()
+
+
+def far_logits(dtype):
+    """Logits at which a sigmoid or its complement leaves fp32."""
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn(12, 24, generator=g)
+    logits[0] -= 100.0
+    logits[1] += 30.0
+    logits[2] = logits[2] * 10 - 95
+    logits[3] = logits[3] * 20 - 300
+    logits[4, ::2] -= 120.0
+    logits[5, ::3] += 60.0
+    logits[6] = logits[6] * 0.5 - 700
+    logits[7] = logits[7] * 40 - 720      # on both sides of where 64-bit scores end
+    logits[8] -= 2000.0
+    logits[9] = torch.finfo(dtype).min
+    logits[10, 5:] = torch.finfo(dtype).min
+    logits[11, 2:] = float("-inf")
+    logits[11, :2] -= 150.0
+    return logits.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [bf16, f32])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_sigmoid_scores_far_from_zero(renormalize, biased, dtype):
+    """Renormalised weights are ratios: they do not depend on whether fp32 holds the scores.  A score
+    that is 0 in 64 bits is 0, a mask of the type's lowest value among them."""
+    logits = far_logits(dtype)
+    check(logits, 6, scoring="sigmoid", renormalize=renormalize, scale=1.5,
+          **({"bias": torch.linspace(0.3, 0.0, 24)} if biased else {}))
+
+
+@pytest.mark.parametrize("dtype", [bf16, f32])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_sigmoid_gradient_far_from_zero(renormalize, dtype):
+    logits = far_logits(dtype)[[0, 1, 2, 3, 4, 5, 6]]
+    dw = torch.randn(7, 6, generator=torch.Generator().manual_seed(2))
+    leaf = logits.to(DEV).requires_grad_(True)
+    weights, ids = tnx.route_experts(leaf, 6, scoring="sigmoid", renormalize=renormalize, scale=1.5)
+    (grad,) = torch.autograd.grad(weights, leaf, dw.to(DEV))
+    i = ids.cpu().long()
+    ref = O.route_gradient_oracle(logits, i, dw, "sigmoid", renormalize, 1.5)
+    # dl = 1.5 r (dw - sum dw r)(1 - s): every factor to 64 roundings of fp32 at most, the difference
+    # against its terms' absolute values; one rounding to the type, subnormals of fp32 included
+    z = logits.double()
+    r = torch.sigmoid(z)
+    if renormalize:
+        r = r / r.gather(1, i).sum(1, keepdim=True)
+    picks = torch.zeros_like(z).scatter_(1, i, 1.0)
+    size = 1.5 * picks * r * torch.sigmoid(-z) * 2 * dw.abs().double().sum(1, keepdim=True)
+    tol = 64 * 2.0 ** -24 * size + torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -133
+    assert torch.isfinite(grad).all()
+    assert ((grad.cpu().double() - ref).abs() <= tol).all()
+    if renormalize:
+        assert (grad[0].cpu()[i[0]] != 0).any()

@@ -106,6 +106,27 @@ __device__ __forceinline__ void scores(const float (&l)[VPT], int experts, int l
   }
 }
 
+// sigmoid(l) and 1 - sigmoid(l), both to a few units in the last place however far l is from 0.
+__device__ __forceinline__ float2 sigmoid_and_rest(float l) {
+  const float e = expf(-fabsf(l)), near = 1.f / (1.f + e), far = e * near;
+  return l >= 0.f ? make_float2(near, far) : make_float2(far, near);
+}
+// A renormalised sigmoid's weight of the lane's pick, before the division by the warp's sum of them:
+// sigmoid(l) / exp(m), m the largest of the picks' min(l, 0), so that it does not matter whether fp32
+// holds the scores (below l = -103 it does not).  Scores that are 0 in 64 bits (1 / (1 + exp(-l)) with
+// an exponential that overflows: l < -709.78, a type's lowest value among them) stay 0.
+__device__ __forceinline__ float sigmoid_share(float l, bool picked) {
+  const bool zero = !picked || l < -709.78265f;
+  const float a = fminf(l, 0.f);
+  const float m = warp_max(zero || l != l ? -CUDART_INF_F : a);
+  if (zero) return 0.f;
+  if (l != l) return l;
+  // (the rounding of a - m would be an error of the weight's 80 units in the last place at a - m = -80)
+  const float d = a - m, b = d - a, rest = (a - (d - b)) - (m + b);
+  const float e = expf(d);
+  return fmaf(e, rest, e) / (1.f + expf(-fabsf(l)));
+}
+
 // Scores that only take part in the choice: fast exponential and division (see the bound on their
 // error in route_kernel).  False where the row's sum is not a number, and no score with it: a logit is
 // NaN or infinity.
@@ -381,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       my_score = row_max == -CUDART_INF_F ? 0.f : expf(my_logit - row_max) / sum;
     }
   } else {
-    my_score = 1.f / (1.f + expf(-my_logit));
+    my_score = sigmoid_and_rest(my_logit).x;
   }
 
   const bool picked = lane < p.top_k;
@@ -391,6 +412,8 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       // a softmax over the picks alone: the same ratio, and no score underflows in it
       const float top = warp_max(picked ? my_logit : -CUDART_INF_F);
       w = picked ? expf(my_logit - (top == -CUDART_INF_F ? 0.f : top)) : 0.f;
+    } else {
+      w = sigmoid_share(my_logit, picked);
     }
     const float sum = warp_sum(picked ? w : 0.f);
     w = sum == 0.f ? 0.f : w / sum;
@@ -459,21 +482,21 @@ __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(const Route
       out[j] = score * (d - base);
     }
   } else {
-    const float s = softmax ? 0.f : 1.f / (1.f + expf(-logit));
+    const float2 s = softmax ? make_float2(0.f, 1.f) : sigmoid_and_rest(logit);  // s, 1 - s
     if (p.renormalize) {
       float r;
       if (softmax) {
         const float top = warp_max(logit);
         r = picked ? expf(logit - (top == -CUDART_INF_F ? 0.f : top)) : 0.f;
       } else {
-        r = picked ? s : 0.f;
+        r = sigmoid_share(logit, picked);
       }
       const float sum = warp_sum(r);
       r = sum == 0.f ? 0.f : r / sum;
       base = warp_sum(picked ? dw * r : 0.f);
-      g = r * (dw - base) * (softmax ? 1.f : 1.f - s);
+      g = r * (dw - base) * s.y;
     } else {
-      g = dw * s * (1.f - s);
+      g = dw * s.x * s.y;
     }
     for (int i = 0; i < p.top_k; ++i) {
       const int pick = __shfl_sync(kAll, e, i);
