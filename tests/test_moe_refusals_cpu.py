@@ -153,3 +153,19 @@ def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError, match="CUDA"):
         tnx.moe_swiglu(x, torch.zeros(2, 8, 16), torch.zeros(2, 8, 8), torch.zeros(4, 1, dtype=torch.int32),
                        torch.zeros(4, 1))
+
+
+@pytest.mark.parametrize("n,d,f,n_out,match", [(4, 60, 32, 48, "multiples of 8"), (4, 64, 30, 48, "multiples of 8"),
+                                               (4, 64, 32, 60, "multiples of 8"), (4, 0, 32, 48, "multiples of 8"),
+                                               (4, 64, 0, 48, "multiples of 8"), (4, 64, 32, 0, "multiples of 8"),
+                                               (4, 4, 32, 48, "multiples of 8"), (0, 64, 32, 48, "experts"),
+                                               (513, 64, 32, 48, "experts")])
+@pytest.mark.parametrize("t", [0, 1, 4])
+def test_sizes_that_no_copy_could_mend_are_refused(monkeypatch, t, n, d, f, n_out, match):
+    """Contiguous operands of sizes that the products do not take: refused before any of them is copied."""
+    monkeypatch.setattr(_cabi, "require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(torch.Tensor, "clone", None)
+    half = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ValueError, match=match):
+        tnx.moe_swiglu(half(t, d), half(n, d, 2 * f), half(n, f, n_out), torch.zeros(t, 2, dtype=torch.int32),
+                       torch.zeros(t, 2))

@@ -288,3 +288,9 @@ def test_refusals():
         tnx.moe_swiglu(x, w12[:1].expand(513, -1, -1), w3[:1].expand(513, -1, -1), ids, w)
     with pytest.raises(RuntimeError, match="CUDA"):
         tnx.moe_swiglu(x.cpu(), w12, w3, ids, w)
+
+
+@pytest.mark.parametrize("d,f,n_out", [(60, 32, 48), (64, 30, 48), (64, 32, 60)])
+def test_contiguous_operands_of_odd_sizes_are_refused(d, f, n_out):
+    with pytest.raises(ValueError, match="multiples of 8"):
+        tnx.moe_swiglu(*operands(make(4, 4, 2, d, f, n_out, bf16)))

@@ -110,6 +110,9 @@ def _check_route(logits, top_k, scoring, bias, groups, top_groups, renormalize, 
 
 # ------------------------------------------------------------------------------ experts' products
 
+_MAX_EXPERTS = 512
+
+
 def _addressable(t: torch.Tensor) -> bool:
     """Adjacent elements in rows, pitches of 16 bytes, no overlapping rows or matrices."""
     fine, extent = t.stride(-1) == 1, t.shape[-1]
@@ -244,6 +247,13 @@ def _check_moe(x, w12, w3, ids, weights, activation) -> int:
         raise ValueError("moe_swiglu expects x (tokens, D), w12 (experts, D, 2F) and w3 (experts, F, N)")
     if w12.shape[0] != w3.shape[0] or w12.shape[1] != x.shape[1] or w12.shape[2] != 2 * w3.shape[1]:
         raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w12 {tuple(w12.shape)}, w3 {tuple(w3.shape)}")
+    # (the library's own limits, refused here because operands of other sizes have no pitch that the
+    # copy engine can address, however they are copied)
+    if not 1 <= w12.shape[0] <= _MAX_EXPERTS:
+        raise ValueError(f"1 to {_MAX_EXPERTS} experts, got {w12.shape[0]}")
+    if any(size < 8 or size % 8 for size in (x.shape[1], w3.shape[1], w3.shape[2])):
+        raise ValueError("d_model, d_ff and n_out must be positive multiples of 8, got "
+                         f"{x.shape[1]}, {w3.shape[1]}, {w3.shape[2]}")
     if ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape[1] < 1 or ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"ids must be int32 or int64 (tokens, top_k), got {tuple(ids.shape)} {ids.dtype}")
     if weights.shape != ids.shape or weights.dtype != torch.float32:
