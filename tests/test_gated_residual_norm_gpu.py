@@ -298,3 +298,16 @@ def test_refusals():
         tnx.gated_residual_norm(long, long, long[0], long[0])
     with pytest.raises(RuntimeError, match="CUDA"):
         tnx.gated_residual_norm(y.cpu(), y, w, w)
+
+
+def test_a_scale_held_in_a_tensor_is_read_by_every_call():
+    case = make(5, 96, f32, f32, "none")
+    args, scale, eps = on_gpu(case, False), torch.tensor(1.0), torch.tensor(1e-6)
+    for value in (1.0, 2.0, -0.5):
+        scale.fill_(value)
+        eps.fill_(abs(value) * 1e-3)
+        want = tnx.gated_residual_norm(*args, residual_scale=value, eps=eps.item())
+        got = tnx.gated_residual_norm(*args, residual_scale=scale, eps=eps)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(ValueError, match="residual_scale"):
+        tnx.gated_residual_norm(*args, residual_scale=scale.requires_grad_(True))

@@ -290,3 +290,16 @@ def test_sigmoid_gradient_far_from_zero(renormalize, dtype):
     assert ((grad.cpu().double() - ref).abs() <= tol).all()
     if renormalize:
         assert (grad[0].cpu()[i[0]] != 0).any()
+
+
+def test_numbers_held_in_tensors_are_read_by_every_call():
+    logits = torch.randn(4, 16, generator=torch.Generator().manual_seed(0)).to(DEV)
+    scale, top_k = torch.tensor(1.0), torch.tensor(2)
+    for value in (1, 3):
+        scale.fill_(0.5 * value)
+        top_k.fill_(value)
+        want = tnx.route_experts(logits, value, scale=0.5 * value)
+        got = tnx.route_experts(logits, top_k, scale=scale)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(ValueError, match="scale"):
+        tnx.route_experts(logits, 2, scale=scale.requires_grad_(True))

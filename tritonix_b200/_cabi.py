@@ -596,6 +596,14 @@ def signature(*tensors) -> tuple:
     return tuple([t if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
+def number(name: str, value) -> float:
+    """An argument that is a plain number to the kernels.  A tensor's value is read now: remembered by
+    its identity it would be the first call's for good."""
+    if isinstance(value, torch.Tensor) and value.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is a plain number and gets no gradient: detach it")
+    return float(value)
+
+
 def remember(cache: dict, key, value):
     if len(cache) > 4096:
         cache.clear()

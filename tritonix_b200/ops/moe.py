@@ -67,6 +67,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     has the score 0 (a row of nothing else has the weights 0).  A NaN logit ranks last, and the other
     experts are told apart as if it were not there; a softmax that is not renormalised still gives
     its token NaN weights.  ``ids`` are always distinct and in range."""
+    top_k, num_groups, top_groups = int(top_k), int(num_groups), int(top_groups)
+    renormalize, scale = bool(renormalize), _cabi.number("scale", scale)
     key = (_cabi.signature(logits, bias), top_k, scoring, num_groups, top_groups, renormalize, scale)
     problem = _route_problems.get(key)
     if problem is None:
@@ -103,9 +105,8 @@ def _check_route(logits, top_k, scoring, bias, groups, top_groups, renormalize, 
     stride = max(logits.stride(0), logits.shape[1]) if logits.shape[0] <= 1 else logits.stride(0)
     if _cabi.rows_view(logits) is not logits:
         stride = 0
-    return _cabi.RouteProblem(logits.shape[0], logits.shape[1], int(top_k), int(groups), int(top_groups),
-                              _cabi.SCORINGS[scoring], int(bool(renormalize)), _cabi.DTYPES[logits.dtype], float(scale),
-                              0, stride)
+    return _cabi.RouteProblem(logits.shape[0], logits.shape[1], top_k, groups, top_groups,
+                              _cabi.SCORINGS[scoring], int(renormalize), _cabi.DTYPES[logits.dtype], scale, 0, stride)
 
 
 # ------------------------------------------------------------------------------ experts' products

@@ -111,11 +111,11 @@ def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: to
     ``pre_weight``: [D], and ``gate``: [D] (per channel), [..., 1] (per token) or [..., D] (per
     element), all of one type: that of ``y`` or fp32.  Gradients flow to every tensor argument;
     rows need not be contiguous with one another."""
+    residual_scale, eps = _cabi.number("residual_scale", residual_scale), _cabi.number("eps", eps)
     key = (_cabi.signature(y, residual, post_weight, pre_weight, gate), residual_scale, eps)
     plan = _plans.get(key)
     if plan is None:
-        plan = _cabi.remember(_plans, key, _NormPlan(y, residual, post_weight, pre_weight, gate, float(residual_scale),
-                                                     float(eps)))
+        plan = _cabi.remember(_plans, key, _NormPlan(y, residual, post_weight, pre_weight, gate, residual_scale, eps))
     if not plan.ready:  # as rows, and once more
         rows = plan.shape[0]
         if plan.form == _cabi.GATE_CHANNEL:
