@@ -456,6 +456,11 @@ typedef struct tnx_norm_problem {
 int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, const void* residual,
                             const void* post_weight, const void* pre_weight, const void* gate, void* h, void* n,
                             float* stats, int32_t* status_word, void* stream);
+/* Without a device: how many bytes before the first or past the last of y, residual and a full gate
+ * the forward call's bulk copies read (0: none); -1 where it makes no bulk copies, -2 for a problem it
+ * refuses.  No pointer is dereferenced. */
+int64_t tnx_selftest_norm_copies(const tnx_norm_problem* problem, const void* y, const void* residual,
+                                 const void* gate);
 /* Bytes of workspace the backward call needs. */
 int64_t tnx_gated_residual_norm_workspace(const tnx_norm_problem* problem);
 /* Gradients of every input from those of h and n (row pitches stride_dh, stride_dn).  dy and

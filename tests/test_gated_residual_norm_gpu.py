@@ -311,3 +311,29 @@ def test_a_scale_held_in_a_tensor_is_read_by_every_call():
         assert all(torch.equal(a, b) for a, b in zip(want, got))
     with pytest.raises(ValueError, match="residual_scale"):
         tnx.gated_residual_norm(*args, residual_scale=scale.requires_grad_(True))
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "full"])
+@pytest.mark.parametrize("dtype,wtype", [(bf16, bf16), (f16, f32), (f32, f32)])
+@pytest.mark.parametrize("t,d", [(594, 1), (600, 2), (601, 3), (598, 5), (1203, 7), (700, 8)])
+def test_many_rows_shorter_than_a_copy(t, d, dtype, wtype, gate):
+    """Several rows share the 16 bytes at either end of a tensor."""
+    check(make(t, d, dtype, wtype, gate, seed=t + d))
+
+
+@pytest.mark.parametrize("dtype,d", [(bf16, 3), (bf16, 301), (f32, 2), (f32, 77)])
+def test_first_and_last_rows_between_boundaries(dtype, d):
+    """Tensors that start and end anywhere, NaN and infinities right before and behind them."""
+    case = make(640, d, dtype, dtype, "full", seed=d)
+    args = on_gpu(case, False)
+    want = tnx.gated_residual_norm(*args)
+    for at in range(1, 16 // case["y"].element_size()):
+        views = []
+        for value, name in zip((float("nan"), float("inf"), float("-inf")), ("y", "residual", "gate")):
+            store = torch.full((at + 640 * d + 9,), value, device=DEV, dtype=dtype)
+            store[at:at + 640 * d] = case[name].to(DEV).reshape(-1)
+            views.append(store[at:at + 640 * d].view(640, d))
+        got = tnx.gated_residual_norm(views[0], views[1], args[2], args[3], views[2])
+        # (another order of a row's sum: the last bit may differ)
+        for a, b in zip(want, got):
+            torch.testing.assert_close(a.float(), b.float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)

@@ -169,3 +169,25 @@ def test_sizes_that_no_copy_could_mend_are_refused(monkeypatch, t, n, d, f, n_ou
     with pytest.raises(ValueError, match=match):
         tnx.moe_swiglu(half(t, d), half(n, d, 2 * f), half(n, f, n_out), torch.zeros(t, 2, dtype=torch.int32),
                        torch.zeros(t, 2))
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(_cabi.BF16, _cabi.BF16), (_cabi.F16, _cabi.F32), (_cabi.F32, _cabi.F32)])
+@pytest.mark.parametrize("rows", [592, 593, 594, 598, 601, 1203])
+@pytest.mark.parametrize("gate_form", [0, 3])
+def test_bulk_copies_stay_inside_their_tensors(gate_form, rows, dtype, wdtype):
+    """Rows from one element on, pitches from the row's own length on, tensors that start anywhere."""
+    size, wsize = (4 if dtype == _cabi.F32 else 2), (4 if wdtype == _cabi.F32 else 2)
+    copied = set()
+    for cols in (*range(1, 40), 63, 64, 301, 2049, 4096):
+        for apart in (0, 1, 3, 8):
+            for at in range(0, 16, 2):
+                p = norm(rows=rows, cols=cols, dtype=dtype, weight_dtype=wdtype, gate_form=gate_form,
+                         stride_y=cols + apart, stride_residual=cols, stride_gate=cols + apart)
+                base = (PTR + at // size * size, PTR + (at + 6) // size * size, PTR + at // wsize * wsize)
+                n = lib.tnx_selftest_norm_copies(ctypes.byref(p), *base)
+                assert n in (0, -1), (cols, apart, at, n)
+                if n == 0:
+                    copied.add(cols)
+    assert {64, 301, 2049} <= copied
+    assert lib.tnx_selftest_norm_copies(ctypes.byref(norm(rows=rows, cols=0)), PTR, PTR, PTR) == -2
+    assert lib.tnx_selftest_norm_copies(ctypes.byref(norm(rows=500, cols=64)), PTR, PTR, PTR) == -1

@@ -137,7 +137,7 @@ EXPORTS = ("tnx_version", "tnx_last_error", "tnx_sm_count", "tnx_gemm_query", "t
            "tnx_conv2d_pack_weights", "tnx_swiglu_mlp_query", "tnx_swiglu_mlp",
            "tnx_swiglu_mlp_unit_order", "tnx_route_experts", "tnx_route_experts_backward",
            "tnx_gated_residual_norm", "tnx_gated_residual_norm_workspace",
-           "tnx_gated_residual_norm_backward", "tnx_moe_query", "tnx_moe_swiglu",
+           "tnx_gated_residual_norm_backward", "tnx_selftest_norm_copies", "tnx_moe_query", "tnx_moe_swiglu",
            "tnx_moe_swiglu_backward")
 STATIC_SCRATCH_BYTES = 16 * 1024 * 1024 + 65536
 
@@ -214,6 +214,8 @@ def _load() -> ctypes.CDLL:
         fn.argtypes = [ctypes.POINTER(problem)] + args
     lib.tnx_moe_query.restype = ctypes.c_int
     lib.tnx_moe_query.argtypes = [ctypes.POINTER(MoeProblem), ctypes.POINTER(MoeResources)]
+    lib.tnx_selftest_norm_copies.restype = ctypes.c_int64
+    lib.tnx_selftest_norm_copies.argtypes = [ctypes.POINTER(NormProblem), ptr, ptr, ptr]
     lib.tnx_gated_residual_norm_workspace.restype = ctypes.c_int64
     lib.tnx_gated_residual_norm_workspace.argtypes = [ctypes.POINTER(NormProblem)]
     return lib

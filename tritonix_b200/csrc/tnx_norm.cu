@@ -331,14 +331,26 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float2* smem, int level
 // The rows a block walks: blockIdx.x, blockIdx.x + gridDim.x, ...  Row number i of them lies in slot
 // i % depth, one part of the slot per source.  A bulk copy starts and ends on 16-byte boundaries, so
 // a row is copied from the boundary at or before its first byte to the one at or after its last.
-// Only the very last row of a tensor could be read past its end that way: the bytes behind its last
-// boundary follow by ordinary loads (the whole of it by ordinary loads made its block 10 to 40 us
-// late).
+// Only a tensor's first and last rows (one each, or as many as start within 15 bytes of an end) could
+// be read past its ends that way: of those the copy brings what lies between two boundaries inside
+// them, the bytes before and behind follow by ordinary loads (the whole of a last row by ordinary
+// loads made its block 10 to 40 us late).
 // MOVED: rows may start anywhere (otherwise all start on 16-byte boundaries), but all rows of a block
 // equally far behind a boundary: the grid is a multiple of the rows after which that comes back.
 // (Working the distance out for each row cost the thread that issues the copies, and with it the
 // block, about a microsecond a row.)
 constexpr int kMaxSources = 5;
+// The part of a row that its bulk copy brings, in bytes from the boundary at or before the row's first
+// byte; `shift`: the row's own distance from there.
+struct CopyPart {
+  uint32_t from, to;
+};
+__host__ __device__ constexpr CopyPart copy_part(uint32_t shift, uint32_t row_bytes, bool first, bool last) {
+  const uint32_t from = first && shift > 0 ? 16u : 0u, to = (shift + row_bytes + (last ? 0u : 15u)) & ~15u;
+  return {from, to > from ? to : from};
+}
+// Rows at either end of a tensor that lie within 15 bytes of it (pitch in bytes, not 0).
+__host__ __device__ constexpr int edge_rows(long long pitch) { return pitch > 14 ? 1 : 14 / static_cast<int>(pitch) + 1; }
 template <bool MOVED>
 struct Ring {
   RingCtrl* ctrl;
@@ -349,12 +361,13 @@ struct Ring {
   long long pitch[kMaxSources];  // bytes
   uint32_t row_bytes[kMaxSources], offset[kMaxSources];
   uint32_t shift[kMaxSources];  // bytes from the boundary to a row's start
+  int edge;       // rows at either end that are copied in part
   int row, slot;  // where the block is
   uint32_t phase;
 
   __device__ __forceinline__ Ring(char* smem, const NormParams& p)
       : ctrl(reinterpret_cast<RingCtrl*>(smem)), slots(smem + kCtrlBytes), sources(0), depth(p.depth), rows(p.rows),
-        slot_bytes(0), row(blockIdx.x), slot(0), phase(0) {}
+        slot_bytes(0), edge(1), row(blockIdx.x), slot(0), phase(0) {}
   template <typename E>
   __device__ __forceinline__ void add(const void* base, long long ld, int cols) {
     src[sources] = static_cast<const char*>(base);
@@ -363,49 +376,60 @@ struct Ring {
     offset[sources] = slot_bytes;
     shift[sources] =
         MOVED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[sources] + row * pitch[sources]) & 15) : 0u;
+    if (MOVED && edge_rows(pitch[sources]) > edge) edge = edge_rows(pitch[sources]);
     slot_bytes += ring_row_bytes(cols, sizeof(E));
     ++sources;
   }
-  // The bytes of source k's copy of row r.
-  __device__ __forceinline__ bool last(long long r) const { return MOVED && r == rows - 1; }
-  __device__ __forceinline__ uint32_t span(int k, long long r) const {
-    return (shift[k] + row_bytes[k] + (last(r) ? 0u : 15u)) & ~15u;
+  // Source k's copy of row r.
+  __device__ __forceinline__ CopyPart part(int k, long long r, bool first) const {
+    return copy_part(shift[k], row_bytes[k], MOVED && first, MOVED && r >= rows - edge);
   }
-  __device__ __forceinline__ void issue(long long r, int to) {  // one thread
+  // One thread; first: the row is one of the tensors' first.
+  __device__ __forceinline__ void issue(long long r, int to, bool first) {
     if (r >= rows) return;
     const uint32_t bar = ptx::smem_u32(&ctrl->full[to]);
     const uint32_t at = ptx::smem_u32(slots) + to * slot_bytes;
     uint32_t total = 0;
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
-      if (k < sources) total += span(k, r);
+      if (k < sources) total += part(k, r, first).to - part(k, r, first).from;
     ptx::mbar_arrive_expect_tx(bar, total);
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
-      if (k < sources && span(k, r) > 0) bulk_load(at + offset[k], src[k] + r * pitch[k] - shift[k], span(k, r), bar);
+      if (k < sources) {
+        const CopyPart c = part(k, r, first);
+        if (c.to > c.from)
+          bulk_load(at + offset[k] + c.from, src[k] + r * pitch[k] - shift[k] + c.from, c.to - c.from, bar);
+      }
   }
   __device__ __forceinline__ void start() {
     if (threadIdx.x == 0) {
       for (int d = 0; d < depth; ++d) ptx::mbar_init(ptx::smem_u32(&ctrl->full[d]), 1);
       ctrl->abort = 0;
       ptx::fence_mbar_init();
-      for (int d = 0; d < depth; ++d) issue(row + static_cast<long long>(d) * gridDim.x, d);
+      // (there are more blocks than rows at an end: only a block's own first row can be one of the first)
+      for (int d = 0; d < depth; ++d) issue(row + static_cast<long long>(d) * gridDim.x, d, d == 0 && row < edge);
     }
     __syncthreads();
   }
   // The block's row is in its slot (false: it did not come in time).
   __device__ __forceinline__ bool wait(uint64_t limit_ns) {
     const bool ok = ptx::mbar_wait(ptx::smem_u32(&ctrl->full[slot]), phase, &ctrl->abort, limit_ns);
-    if (!last(row)) return ok;
-    // (all threads come here together; a row is a whole number of 2-byte pieces)
+    if (!MOVED || (row >= edge && row < rows - edge)) return ok;
+    // (all threads come here together; a row is a whole number of 2-byte pieces, and there are at most 15
+    // bytes before and 15 behind)
 #pragma unroll
     for (int k = 0; k < kMaxSources; ++k)
       if (k < sources) {
-        const uint32_t moved = shift[k], done = span(k, row) > moved ? span(k, row) - moved : 0u;
-        const uint32_t b = done + threadIdx.x * 2;
-        if (b < row_bytes[k])
-          *reinterpret_cast<uint16_t*>(slots + static_cast<size_t>(slot) * slot_bytes + offset[k] + moved + b) =
-              *reinterpret_cast<const uint16_t*>(src[k] + row * pitch[k] + b);
+        const uint32_t moved = shift[k];
+        const CopyPart c = part(k, row, row < edge);
+        const uint32_t before = c.from > moved ? c.from - moved : 0u, behind = c.to > moved ? c.to - moved : 0u;
+        const char* from = src[k] + row * pitch[k];
+        char* to = slots + static_cast<size_t>(slot) * slot_bytes + offset[k] + moved;
+        uint32_t b = threadIdx.x * 2;
+        if (b < before && b < row_bytes[k]) *reinterpret_cast<uint16_t*>(to + b) = *reinterpret_cast<const uint16_t*>(from + b);
+        b += behind;
+        if (b < row_bytes[k]) *reinterpret_cast<uint16_t*>(to + b) = *reinterpret_cast<const uint16_t*>(from + b);
       }
     block_barrier();
     return ok;
@@ -414,7 +438,7 @@ struct Ring {
   __device__ __forceinline__ uint32_t at(int k) const { return slot * slot_bytes + offset[k] + shift[k]; }
   // Nobody reads the row's slot any more: it takes the row `depth` rounds ahead.
   __device__ __forceinline__ void refill() {
-    if (threadIdx.x == 0) issue(row + static_cast<long long>(depth) * gridDim.x, slot);
+    if (threadIdx.x == 0) issue(row + static_cast<long long>(depth) * gridDim.x, slot, false);
   }
   __device__ __forceinline__ void next() {
     row += gridDim.x;
@@ -975,10 +999,54 @@ int launched(const char* what) {
   return TNX_ERR_CUDA;
 }
 
+// Bytes that the bulk copies of a tensor's rows read before its first or past its last byte, at most.
+int64_t outside(const void* base, int64_t rows, int64_t pitch, uint32_t row_bytes, int edge, bool moved) {
+  const int64_t start = static_cast<int64_t>(reinterpret_cast<uintptr_t>(base)), end = start + (rows - 1) * pitch + row_bytes;
+  int64_t most = 0;
+  for (int64_t r = 0; r < rows; ++r) {
+    const int64_t at = start + r * pitch, shift = moved ? at & 15 : 0;
+    const CopyPart part = copy_part(static_cast<uint32_t>(shift), row_bytes, moved && r < edge, moved && r >= rows - edge);
+    if (part.to == part.from) continue;
+    if (start - (at - shift + part.from) > most) most = start - (at - shift + part.from);
+    if (at - shift + part.to - end > most) most = at - shift + part.to - end;
+  }
+  return most;
+}
+
 }  // namespace
 }  // namespace tnx
 
 extern "C" {
+
+int64_t tnx_selftest_norm_copies(const tnx_norm_problem* problem, const void* y, const void* residual,
+                                 const void* gate) {
+  using namespace tnx;
+  const void* ptrs[] = {y, residual, gate};
+  const bool full = problem != nullptr && problem->gate_form == TNX_GATE_FULL;
+  NormShape s;
+  long long pitches[3] = {};
+  if (problem != nullptr) {
+    pitches[0] = problem->stride_y;
+    pitches[1] = problem->stride_residual;
+    pitches[2] = problem->stride_gate;
+  }
+  const int sources = full ? 3 : 2;
+  if (norm_check(problem, false, ptrs, sources, pitches, sources, &s) != TNX_OK) return -2;
+  if (s.depth == 0) return -1;
+  int edge = 1;
+  for (int k = 0; k < sources; ++k) {
+    const int rows = edge_rows(pitches[k] * ((k == 2 ? problem->weight_dtype : problem->dtype) == TNX_F32 ? 4 : 2));
+    if (rows > edge) edge = rows;
+  }
+  int64_t most = 0;
+  for (int k = 0; k < sources; ++k) {
+    const int size = (k == 2 ? problem->weight_dtype : problem->dtype) == TNX_F32 ? 4 : 2;
+    const int64_t here = outside(ptrs[k], problem->rows, pitches[k] * size, static_cast<uint32_t>(problem->cols * size),
+                                 edge, s.vec == 1 || s.led);
+    if (here > most) most = here;
+  }
+  return most;
+}
 
 int64_t tnx_gated_residual_norm_workspace(const tnx_norm_problem* problem) {
   if (problem == nullptr || problem->rows <= 0 || problem->cols <= 0) return 0;
