@@ -42,6 +42,7 @@ struct NormParams {
   int sums;
   // ring kernels
   int depth;                // rows in flight
+  int edge, inner;          // rows at either end of a tensor that are copied in part, and those between
   int* status;
   unsigned long long timeout_ns;
 };
@@ -349,8 +350,8 @@ __host__ __device__ constexpr CopyPart copy_part(uint32_t shift, uint32_t row_by
   const uint32_t from = first && shift > 0 ? 16u : 0u, to = (shift + row_bytes + (last ? 0u : 15u)) & ~15u;
   return {from, to > from ? to : from};
 }
-// Rows at either end of a tensor that lie within 15 bytes of it (pitch in bytes, not 0).
-__host__ __device__ constexpr int edge_rows(long long pitch) { return pitch > 14 ? 1 : 14 / static_cast<int>(pitch) + 1; }
+// Rows at either end of a tensor that lie within 15 bytes of it.
+inline int edge_rows(long long pitch_bytes) { return pitch_bytes > 14 ? 1 : 14 / static_cast<int>(pitch_bytes) + 1; }
 template <bool MOVED>
 struct Ring {
   RingCtrl* ctrl;
@@ -361,13 +362,13 @@ struct Ring {
   long long pitch[kMaxSources];  // bytes
   uint32_t row_bytes[kMaxSources], offset[kMaxSources];
   uint32_t shift[kMaxSources];  // bytes from the boundary to a row's start
-  int edge;       // rows at either end that are copied in part
+  int edge, inner;  // as in NormParams
   int row, slot;  // where the block is
   uint32_t phase;
 
   __device__ __forceinline__ Ring(char* smem, const NormParams& p)
       : ctrl(reinterpret_cast<RingCtrl*>(smem)), slots(smem + kCtrlBytes), sources(0), depth(p.depth), rows(p.rows),
-        slot_bytes(0), edge(1), row(blockIdx.x), slot(0), phase(0) {}
+        slot_bytes(0), edge(p.edge), inner(p.inner), row(blockIdx.x), slot(0), phase(0) {}
   template <typename E>
   __device__ __forceinline__ void add(const void* base, long long ld, int cols) {
     src[sources] = static_cast<const char*>(base);
@@ -376,13 +377,12 @@ struct Ring {
     offset[sources] = slot_bytes;
     shift[sources] =
         MOVED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[sources] + row * pitch[sources]) & 15) : 0u;
-    if (MOVED && edge_rows(pitch[sources]) > edge) edge = edge_rows(pitch[sources]);
     slot_bytes += ring_row_bytes(cols, sizeof(E));
     ++sources;
   }
   // Source k's copy of row r.
   __device__ __forceinline__ CopyPart part(int k, long long r, bool first) const {
-    return copy_part(shift[k], row_bytes[k], MOVED && first, MOVED && r >= rows - edge);
+    return copy_part(shift[k], row_bytes[k], MOVED && first, MOVED && r >= edge + inner);
   }
   // One thread; first: the row is one of the tensors' first.
   __device__ __forceinline__ void issue(long long r, int to, bool first) {
@@ -415,7 +415,7 @@ struct Ring {
   // The block's row is in its slot (false: it did not come in time).
   __device__ __forceinline__ bool wait(uint64_t limit_ns) {
     const bool ok = ptx::mbar_wait(ptx::smem_u32(&ctrl->full[slot]), phase, &ctrl->abort, limit_ns);
-    if (!MOVED || (row >= edge && row < rows - edge)) return ok;
+    if (!MOVED || static_cast<unsigned>(row - edge) < static_cast<unsigned>(inner)) return ok;
     // (all threads come here together; a row is a whole number of 2-byte pieces, and there are at most 15
     // bytes before and 15 behind)
 #pragma unroll
@@ -999,6 +999,13 @@ int launched(const char* what) {
   return TNX_ERR_CUDA;
 }
 
+// edge_rows() of the tensor with the most, all of them at least as wide as the rows are long.
+int most_edge_rows(const tnx_norm_problem& p, const long long* pitches, int count) {
+  long long least = pitches[0];
+  for (int k = 1; k < count; ++k) least = pitches[k] < least ? pitches[k] : least;
+  return edge_rows(least * (p.dtype == TNX_F32 ? 4 : 2));  // (a gate of fp32 has fewer)
+}
+
 // Bytes that the bulk copies of a tensor's rows read before its first or past its last byte, at most.
 int64_t outside(const void* base, int64_t rows, int64_t pitch, uint32_t row_bytes, int edge, bool moved) {
   const int64_t start = static_cast<int64_t>(reinterpret_cast<uintptr_t>(base)), end = start + (rows - 1) * pitch + row_bytes;
@@ -1033,11 +1040,7 @@ int64_t tnx_selftest_norm_copies(const tnx_norm_problem* problem, const void* y,
   const int sources = full ? 3 : 2;
   if (norm_check(problem, false, ptrs, sources, pitches, sources, &s) != TNX_OK) return -2;
   if (s.depth == 0) return -1;
-  int edge = 1;
-  for (int k = 0; k < sources; ++k) {
-    const int rows = edge_rows(pitches[k] * ((k == 2 ? problem->weight_dtype : problem->dtype) == TNX_F32 ? 4 : 2));
-    if (rows > edge) edge = rows;
-  }
+  const int edge = most_edge_rows(*problem, pitches, sources);
   int64_t most = 0;
   for (int k = 0; k < sources; ++k) {
     const int size = (k == 2 ? problem->weight_dtype : problem->dtype) == TNX_F32 ? 4 : 2;
@@ -1098,6 +1101,8 @@ int tnx_gated_residual_norm(const tnx_norm_problem* problem, const void* y, cons
     return TNX_ERR_NOT_BUILT;
   }
   p.depth = s.depth;
+  if (s.depth > 0) p.edge = most_edge_rows(*problem, pitches, 3);
+  p.inner = p.rows - 2 * p.edge;
   p.status = status_word;
   p.timeout_ns = bounded_wait_limit_ns();
   rc = allow_smem(fn, s.smem);
@@ -1176,6 +1181,8 @@ int tnx_gated_residual_norm_backward(const tnx_norm_problem* problem, const void
       return TNX_ERR_NOT_BUILT;
     }
     p.depth = s.depth;
+    if (s.depth > 0) p.edge = most_edge_rows(*problem, pitches, 5);
+    p.inner = p.rows - 2 * p.edge;
     p.status = status_word;
     p.timeout_ns = bounded_wait_limit_ns();
     rc = allow_smem(fn, s.smem);
