@@ -1,9 +1,12 @@
 """The gated residual norm and its gradients against the 64-bit oracle."""
+import ctypes
+
 import pytest
 import torch
 
 import tritonix_b200 as tnx
 from oracle import moe as O
+from tritonix_b200 import _cabi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -337,3 +340,37 @@ def test_first_and_last_rows_between_boundaries(dtype, d):
         # (another order of a row's sum: the last bit may differ)
         for a, b in zip(want, got):
             torch.testing.assert_close(a.float(), b.float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
+
+
+@pytest.mark.parametrize("pitch", [0, 3, 8])
+@pytest.mark.parametrize("d", [301, 304])
+def test_c_entry_points_take_rows_that_overlap(d, pitch):
+    """The Python function copies such rows first; the C functions read them as they lie."""
+    rows = 700
+    case = make(rows, d, bf16, f32, "full", seed=d)
+    _, residual, post, pre, gate = on_gpu(case, False)
+    store = torch.randn(pitch * (rows - 1) + d, generator=torch.Generator().manual_seed(pitch)).to(bf16)
+    case["y"] = store.as_strided((rows, d), (pitch, 1)).contiguous()
+    y = store.to(DEV)
+    dh, dn = case["dh"].to(DEV), case["dn"].to(DEV)
+    problem = _cabi.NormProblem(rows, d, _cabi.BF16, _cabi.F32, _cabi.GATE_FULL, 0.75, 1e-5, 0, pitch, d, d)
+    h, n, dy, dres = (torch.full((rows, d), float("nan"), device=DEV, dtype=bf16) for _ in range(4))
+    dgate = torch.full((rows, d), float("nan"), device=DEV)
+    dpost, dpre = torch.empty(d, device=DEV), torch.empty(d, device=DEV)
+    stats = torch.empty(rows, 2, device=DEV)
+    status = _cabi.status_word(y.device).data_ptr()
+    size = _cabi.lib.tnx_gated_residual_norm_workspace(ctypes.byref(problem))
+    workspace = torch.empty(size, device=DEV, dtype=torch.uint8)
+    at = lambda *tensors: [t.data_ptr() for t in tensors]  # noqa: E731
+    _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm, ctypes.byref(problem),
+               *at(y, residual, post, pre, gate, h, n, stats), status)
+    _cabi.call(y.device, _cabi.lib.tnx_gated_residual_norm_backward, ctypes.byref(problem), dh.data_ptr(), d,
+               dn.data_ptr(), d, *at(y, residual, post, pre, gate, stats, dy, dres, dpost, dpre, dgate, workspace), size,
+               status)
+    ref = [case[k] for k in ("y", "residual", "post", "pre", "gate")]
+    rh, rn, mh, mn = O.norm_oracle(*ref, 0.75, 1e-5)
+    within(h, rh, mh, FORWARD)
+    within(n, rn, mn, FORWARD)
+    want = O.norm_gradient_oracle(*ref, 0.75, 1e-5, case["dh"], case["dn"])
+    for grad, name in ((dy, "y"), (dres, "residual"), (dpost, "post"), (dpre, "pre"), (dgate, "gate")):
+        within(grad, *want[name], BACKWARD + (rows * 2.0 ** -24 if name in ("post", "pre") else 0))

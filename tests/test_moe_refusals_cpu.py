@@ -191,3 +191,10 @@ def test_bulk_copies_stay_inside_their_tensors(gate_form, rows, dtype, wdtype):
     assert {64, 301, 2049} <= copied
     assert lib.tnx_selftest_norm_copies(ctypes.byref(norm(rows=rows, cols=0)), PTR, PTR, PTR) == -2
     assert lib.tnx_selftest_norm_copies(ctypes.byref(norm(rows=500, cols=64)), PTR, PTR, PTR) == -1
+
+
+@pytest.mark.parametrize("pitch", [0, 8])
+def test_bulk_copies_of_one_row_for_many(pitch):
+    p = norm(rows=700, cols=304, stride_y=pitch, stride_residual=304)
+    assert lib.tnx_selftest_norm_copies(ctypes.byref(p), PTR, PTR, None) == 0
+    assert lib.tnx_selftest_norm_copies(ctypes.byref(p), PTR + 2, PTR, None) == -1

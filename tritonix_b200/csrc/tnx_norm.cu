@@ -350,8 +350,11 @@ __host__ __device__ constexpr CopyPart copy_part(uint32_t shift, uint32_t row_by
   const uint32_t from = first && shift > 0 ? 16u : 0u, to = (shift + row_bytes + (last ? 0u : 15u)) & ~15u;
   return {from, to > from ? to : from};
 }
-// Rows at either end of a tensor that lie within 15 bytes of it.
-inline int edge_rows(long long pitch_bytes) { return pitch_bytes > 14 ? 1 : 14 / static_cast<int>(pitch_bytes) + 1; }
+// Rows at either end of a tensor that lie within 15 bytes of it.  (Pitches below a row's length, 0 among
+// them, only come here where all rows start and end on boundaries and are copied whole.)
+inline int edge_rows(long long pitch_bytes) {
+  return pitch_bytes < 1 || pitch_bytes > 14 ? 1 : 14 / static_cast<int>(pitch_bytes) + 1;
+}
 template <bool MOVED>
 struct Ring {
   RingCtrl* ctrl;
