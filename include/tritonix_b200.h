@@ -402,10 +402,10 @@ int tnx_conv2d_forward(const tnx_conv2d_problem* problem, const tnx_config* conf
  * groups whose two best c have the largest sum can be chosen.  ids = the top_k by c, best first,
  * ties to the lowest index; weights = scale * s[ids], divided by the sum of s[ids] when
  * `renormalize` is set (0 when that sum is 0 in 64 bits, as for masks of a type's lowest value under
- * a sigmoid; sums that only fp32 cannot hold are no such case).  Which experts are chosen is decided as in 64-bit
- * arithmetic.  A NaN logit ranks below every other, and those are told apart as if it were not there
- * (a softmax that is not renormalised still gives its token NaN weights); ids are always distinct
- * and in range.
+ * a sigmoid; sums that only fp32 cannot hold are no such case).  Which experts are chosen is decided
+ * as in 64-bit arithmetic.  A NaN logit ranks below every other, and those are told apart as if it
+ * were not there (a softmax that is not renormalised still gives its token NaN weights); ids are
+ * always distinct and in range.
  */
 typedef struct tnx_route_problem {
   int32_t tokens, experts; /* experts <= 512                                               */

@@ -1,9 +1,12 @@
 """Experts' gated products and their gradients against the 64-bit oracle."""
+import ctypes
+
 import pytest
 import torch
 
 import tritonix_b200 as tnx
 from oracle import moe as O
+from tritonix_b200 import _cabi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -294,3 +297,47 @@ def test_refusals():
 def test_contiguous_operands_of_odd_sizes_are_refused(d, f, n_out):
     with pytest.raises(ValueError, match="multiples of 8"):
         tnx.moe_swiglu(*operands(make(4, 4, 2, d, f, n_out, bf16)))
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16])
+@pytest.mark.parametrize("t,d,f,n_out", [(500, 4096, 136, 2048), (340, 2056, 72, 4104), (270, 2048, 264, 2048)])
+def test_long_sums_that_feed_the_routing_weights_gradient(t, d, f, n_out, dtype):
+    """Sums over thousands of elements in many parts, for more rows of an expert than a warp holds in
+    registers at once.  An accumulator that ran over all of K would be short by 3e-9 K of its size
+    (6e-6 at K = 2048) in each of the gradient's factors, past the bound of 2.95e-6."""
+    ids = (torch.arange(t) % 2).to(torch.int32).unsqueeze(1)
+    check(make(t, 2, 1, d, f, n_out, dtype, seed=d, ids=ids))
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16])
+@pytest.mark.parametrize("t,n,k,d,f,n_out", [(5, 2, 1, 264, 2048, 256), (40, 3, 2, 64, 1160, 72), (2, 4, 2, 128, 4104, 264)])
+def test_down_products_in_slices(t, n, k, d, f, n_out, dtype):
+    """Few tiles and a long K: slices of it (the last one short) are added by the join."""
+    case = make(t, n, k, d, f, n_out, dtype, seed=f)
+    problem = _cabi.MoeProblem(t, n, k, d, f, n_out, _cabi.DTYPES[dtype], _cabi.EPI_GLU_SILU, 0, 1, d, d * 2 * f, 2 * f,
+                               f * n_out, n_out, n_out)
+    res = _cabi.MoeResources()
+    assert _cabi.lib.tnx_moe_query(ctypes.byref(problem), ctypes.byref(res)) == _cabi.OK
+    rows = t * k // 16 * 16   # (at least; a copy of the rows of x and one of the fp32 rows per slice)
+    assert res.workspace_bytes >= (t * k + min(n, t * k) * 15) // 16 * 16 * (2 * d + 2 * 4 * n_out) > rows * 4 * n_out
+    check(case)
+
+
+@pytest.mark.parametrize("t", [1, 70])
+def test_small_weights_in_fp16(t):
+    """The hidden activation is rounded with its weight: where that leaves fp16's normal range, to
+    half its smallest step (2^-25) instead of half a step of the value."""
+    case = make(t, 4, 2, 128, 96, 64, f16, seed=t)
+    case["weights"] = 10.0 ** -torch.linspace(1, 7, 2 * t).view(t, 2)
+    y = tnx.moe_swiglu(*operands(case)).cpu().double()
+    ref, tol = O.experts_oracle(*[case[n] for n in ("x", "w12", "w3", "ids", "weights")]), torch.zeros(t, 64).double()
+    half, step = 2.0 ** -11, 2.0 ** -25
+    x, w12, w3 = (case[n].double() for n in ("x", "w12", "w3"))
+    for e in range(4):
+        token, slot = torch.nonzero(case["ids"] == e, as_tuple=True)
+        gu = x[token] @ w12[e]
+        hidden = case["weights"][token, slot].double().unsqueeze(1) * torch.nn.functional.silu(gu[:, 0::2]) * gu[:, 1::2]
+        # (and 2^-18 for sums of 128 and 96 terms in fp32, the exponential and the division)
+        tol.index_add_(0, token, ((half + 2.0 ** -18) * hidden.abs() + step) @ w3[e].abs())
+    tol += half * ref.abs() + step
+    assert ((y - ref).abs() <= tol).all()
