@@ -2,6 +2,7 @@
 graphs, streams, and the torch custom ops."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import tritonix_b200 as tnx
 from oracle import moe as O
@@ -140,3 +141,22 @@ def test_custom_ops():
     h, n = torch.ops.tritonix.gated_residual_norm(y, args[1], args[5], args[6], args[7], 0.7, 1e-6)
     want = block(args, bias)
     assert torch.equal(h, want[0]) and torch.equal(n, want[1])
+
+
+def test_forward_mode_differentiation_is_refused():
+    """A tangent must not get lost, with gradients asked for and without, by itself or through a transform."""
+    case = make(6, 16, 128, 64)
+    args, bias = leaves(case, False), case["bias"].to(DEV)
+    w, i = tnx.route_experts(args[2], 3)
+    calls = ((args[2], lambda v: tnx.route_experts(v, 3)), (args[0], lambda v: tnx.moe_swiglu(v, args[3], args[4], i, w)),
+             (w, lambda v: tnx.moe_swiglu(args[0], args[3], args[4], i, v)),
+             *((args[j], lambda v, j=j: block(args[:j] + [v] + args[j + 1:], bias)) for j in range(8)))
+    for value, call in calls:
+        for grad in (False, True):
+            with fwad.dual_level():
+                dual = fwad.make_dual(value.clone().requires_grad_(grad), torch.ones_like(value))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(dual)
+                call(value)  # (others are not disturbed by an open level)
+        with pytest.raises(RuntimeError, match="forward-mode|storage"):  # (or torch's: a wrapped tensor has none)
+            torch.func.jvp(call, (value,), (torch.ones_like(value),))

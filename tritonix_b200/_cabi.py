@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 import os
 
@@ -596,6 +597,15 @@ def signature(*tensors) -> tuple:
     """Everything about the tensors that argument checks look at, hashable; an operator checks a
     signature once and remembers what it found."""
     return tuple([t if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
+
+
+def refuse_tangents(*tensors) -> None:
+    """Forward-mode differentiation has no formulas here; without this a dual tensor's tangent would be
+    lost where no operand asks for a gradient."""
+    if forward_ad._current_level < 0:  # (no dual level is open: the usual case, one comparison)
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode differentiation is not supported")
 
 
 def number(name: str, value) -> float:

@@ -67,6 +67,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     has the score 0 (a row of nothing else has the weights 0).  A NaN logit ranks last, and the other
     experts are told apart as if it were not there; a softmax that is not renormalised still gives
     its token NaN weights.  ``ids`` are always distinct and in range."""
+    _cabi.refuse_tangents(logits)
     top_k, num_groups, top_groups = int(top_k), int(num_groups), int(top_groups)
     renormalize, scale = bool(renormalize), _cabi.number("scale", scale)
     key = (_cabi.signature(logits, bias), top_k, scoring, num_groups, top_groups, renormalize, scale)
@@ -227,6 +228,7 @@ def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.
 
     Gradients flow to ``x``, ``w12``, ``w3`` and ``weights``.  The routing stays on the device: no
     call waits for it.  Results do not depend on timing (every sum has a fixed order)."""
+    _cabi.refuse_tangents(x, w12, w3, weights)
     key = (_cabi.signature(x, w12, w3, ids, weights), activation)
     plan = _moe_plans.get(key)
     if plan is None:

@@ -111,6 +111,7 @@ def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: to
     ``pre_weight``: [D], and ``gate``: [D] (per channel), [..., 1] (per token) or [..., D] (per
     element), all of one type: that of ``y`` or fp32.  Gradients flow to every tensor argument;
     rows need not be contiguous with one another."""
+    _cabi.refuse_tangents(y, residual, post_weight, pre_weight, gate)
     residual_scale, eps = _cabi.number("residual_scale", residual_scale), _cabi.number("eps", eps)
     key = (_cabi.signature(y, residual, post_weight, pre_weight, gate), residual_scale, eps)
     plan = _plans.get(key)
