@@ -1,5 +1,7 @@
 """Routing, the experts' products and the norms in a row, as a model runs them: values, gradients,
 graphs, streams, and the torch custom ops."""
+import warnings
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -160,3 +162,79 @@ def test_forward_mode_differentiation_is_refused():
                 call(value)  # (others are not disturbed by an open level)
         with pytest.raises(RuntimeError, match="forward-mode|storage"):  # (or torch's: a wrapped tensor has none)
             torch.func.jvp(call, (value,), (torch.ones_like(value),))
+
+
+def block_of_ops(args, bias, top_k=3):
+    x, residual, logits, w12, w3, post, pre, gate = args
+    ops = torch.ops.tritonix
+    w, i = ops.route_experts(logits, top_k, "sigmoid", bias, 4, 2, True, 1.5)
+    return ops.gated_residual_norm(ops.moe_swiglu(x, w12, w3, i, w, "silu"), residual, post, pre, gate, 0.7, 1e-6)
+
+
+@pytest.mark.parametrize("traced", [False, True])
+def test_custom_ops_train(traced):
+    """Through the custom operators, called and traced: the gradients of the Python functions."""
+    case = make(60, 16, 256, 136, seed=8)
+    bias, outs = case["bias"].to(DEV), [case["dh"].to(DEV), case["dn"].to(DEV)]
+    args = leaves(case)
+    want = block(args, bias)
+    want_grads = torch.autograd.grad(want, args, outs)
+    fn = torch.compile(block_of_ops, backend="aot_eager", fullgraph=True) if traced else block_of_ops
+    args = leaves(case)
+    with warnings.catch_warnings():
+        warnings.filterwarnings("error", message=".*autograd kernel was not registered.*")
+        got = fn(args, bias)
+        grads = torch.autograd.grad(got, args, outs)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(fn(args, bias), want))
+
+
+def test_custom_ops_pass_torchs_own_checks():
+    case = make(12, 16, 64, 32)
+    x, residual, logits, w12, w3, post, pre, gate = leaves(case)
+    w, i = tnx.route_experts(logits.detach(), 3)
+    w.requires_grad_(True)
+    ops = torch.ops.tritonix
+    for op, args in ((ops.route_experts, (logits, 3, "softmax", None, 1, 1, False, 1.5)),
+                     (ops.moe_swiglu, (x, w12, w3, i, w, "silu")),
+                     (ops.moe_swiglu, (x.detach(), w12, w3.detach(), i.long(), w.detach(), "none")),
+                     (ops.gated_residual_norm, (x, residual, post, pre, gate, 0.7, 1e-6)),
+                     (ops.gated_residual_norm, (x, residual, post, pre, None, 0.7, 1e-6))):
+        torch.library.opcheck(op.default, args)
+
+
+def test_custom_ops_take_any_strides_and_leading_dimensions():
+    case = make(24, 16, 64, 32, seed=3)
+    x, residual, logits, w12, w3, post, pre, gate = leaves(case)
+    out = [case["dh"].to(DEV), case["dn"].to(DEV)]
+    ops = torch.ops.tritonix
+    cols = lambda t: t.detach().mT.contiguous().mT.requires_grad_(True)  # noqa: E731
+    w, i = tnx.route_experts(logits.detach(), 3)
+    a = [x, w12, w3, w.requires_grad_(True)]
+    b = [cols(x), cols(w12), cols(w3), cols(w)]
+    grads = [torch.autograd.grad(ops.moe_swiglu(*v[:3], i, v[3], "silu"), v, out[0]) for v in (a, b)]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    grads = [torch.autograd.grad(ops.route_experts(v, 3, "softmax", None, 1, 1, False, 1.0)[0], v, torch.ones_like(w))
+             for v in (logits, cols(logits))]
+    assert torch.equal(grads[0][0], grads[1][0])
+    a, b = [x, residual, post, pre, gate], [t.detach().view(2, 12, 64).requires_grad_(True) for t in (x, residual)]
+    ga = torch.autograd.grad(ops.gated_residual_norm(*a, 0.7, 1e-6), a, out)
+    gb = torch.autograd.grad(ops.gated_residual_norm(*b, *a[2:], 0.7, 1e-6), b + a[2:], [t.view(2, 12, 64) for t in out])
+    assert all(torch.equal(p, q.view(p.shape)) for p, q in zip(ga, gb))
+
+
+def test_custom_ops_refuse_second_derivatives_and_tangents():
+    case = make(6, 16, 64, 32)
+    args = leaves(case)
+    h, n = block_of_ops(args, case["bias"].to(DEV))
+    with pytest.raises(RuntimeError, match="gradient of its own"):
+        torch.autograd.grad(n.float().square().sum(), args, create_graph=True)
+    for grad in (False, True):
+        for j in range(8):
+            with fwad.dual_level():
+                dual = fwad.make_dual(args[j].detach().requires_grad_(grad), torch.ones_like(args[j]))
+                others = [a.detach() for a in args]
+                with pytest.raises(RuntimeError):
+                    block_of_ops(others[:j] + [dual] + others[j + 1:], case["bias"].to(DEV))

@@ -198,3 +198,26 @@ def test_bulk_copies_of_one_row_for_many(pitch):
     p = norm(rows=700, cols=304, stride_y=pitch, stride_residual=304)
     assert lib.tnx_selftest_norm_copies(ctypes.byref(p), PTR, PTR, None) == 0
     assert lib.tnx_selftest_norm_copies(ctypes.byref(p), PTR + 2, PTR, None) == -1
+
+
+def test_custom_ops_carry_gradients_without_a_device():
+    """Traced with tensors that hold no data, outputs ask for gradients and their shapes come back."""
+    meta = lambda *s, dt=torch.bfloat16: torch.empty(s, dtype=dt, device="meta", requires_grad=True)  # noqa: E731
+    ops = torch.ops.tritonix
+    logits, x, w12, w3 = meta(5, 8, dt=torch.float32), meta(5, 16), meta(8, 16, 48), meta(8, 24, 32)
+    res, post, pre, gate = meta(5, 32), meta(32, dt=torch.float32), meta(32, dt=torch.float32), meta(5, 1, dt=torch.float32)
+    w, i = ops.route_experts(logits, 2, "softmax", None, 1, 1, True, 1.0)
+    assert w.requires_grad and not i.requires_grad
+    y = ops.moe_swiglu(x, w12, w3, i, w, "silu")
+    h, n = ops.gated_residual_norm(y, res, post, pre, gate, 1.0, 1e-6)
+    leaves = [logits, x, w12, w3, res, post, pre, gate]
+    grads = torch.autograd.grad([h, n], leaves, [torch.empty_like(h), torch.empty_like(n)])
+    assert [(g.shape, g.dtype) for g in grads] == [(v.shape, v.dtype) for v in leaves]
+    # one leaf alone, none at all
+    y = ops.moe_swiglu(x.detach(), w12, w3.detach(), i, w.detach(), "silu")
+    assert torch.autograd.grad(y, w12, torch.empty_like(y))[0].shape == w12.shape
+    assert not ops.moe_swiglu(x.detach(), w12.detach(), w3.detach(), i, w.detach(), "silu").requires_grad
+    with torch.no_grad():
+        assert not ops.moe_swiglu(x, w12, w3, i, w, "silu").requires_grad
+    with torch.inference_mode():
+        assert ops.moe_swiglu(x, w12, w3, i, w, "silu").shape == (5, 32)

@@ -43,11 +43,22 @@ class _RouteExperts(torch.autograd.Function):
         if dweights is None:
             return None, None, None
         logits, ids = ctx.saved_tensors
-        dweights = dweights.contiguous()
-        dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        _cabi.call(logits.device, _cabi.lib.tnx_route_experts_backward, ctypes.byref(ctx.problem),
-                   logits.data_ptr(), ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
-        return dlogits, None, None
+        return _route_backward(dweights, logits, ids, ctx.problem), None, None
+
+
+def _route_backward(dweights, logits, ids, problem):
+    dweights = dweights.contiguous()
+    dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    _cabi.call(logits.device, _cabi.lib.tnx_route_experts_backward, ctypes.byref(problem), logits.data_ptr(),
+               ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
+    return dlogits
+
+
+def route_gradient(dweights, logits, ids, scoring, renormalize, scale):
+    """Gradient of the logits from that of the weights (the custom operator's backward pass)."""
+    logits = _cabi.rows_view(logits)
+    problem = _check_route(logits, ids.shape[1], scoring, None, 1, 1, renormalize, scale)
+    return _route_backward(dweights, logits, ids.contiguous(), problem)
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
@@ -195,22 +206,24 @@ class _MoeSwiglu(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w12, w3, saved = ctx.saved_tensors
-        plan = ctx.plan
-        dy = _pitched(dy)
-        (stride_dy,) = _pitches(dy)
-        wants = ctx.needs_input_grad
-        new = lambda shape, dtype: torch.empty(shape, device=x.device, dtype=dtype)  # noqa: E731
-        dx = new(x.shape, x.dtype) if wants[0] else None
-        dw12 = new(w12.shape, x.dtype) if wants[1] else None
-        dw3 = new(w3.shape, x.dtype) if wants[2] else None
-        dweights = new(plan.pairs, torch.float32) if wants[3] else None
-        workspace = new(plan.resources[1].backward_workspace_bytes, torch.uint8)
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        _cabi.call(x.device, _cabi.lib.tnx_moe_swiglu_backward, ctypes.byref(plan.problems[1]), dy.data_ptr(), stride_dy,
-                   x.data_ptr(), w12.data_ptr(), w3.data_ptr(), saved.data_ptr(), ptr(dx), ptr(dw12), ptr(dw3),
-                   ptr(dweights), workspace.data_ptr(), workspace.numel(), _cabi.status_word(x.device).data_ptr())
-        return dx, dw12, dw3, dweights, None, None
+        return *_moe_backward(ctx.plan, dy, *ctx.saved_tensors, ctx.needs_input_grad[:4]), None, None
+
+
+def _moe_backward(plan, dy, x, w12, w3, saved, wants):
+    """Gradients of x, w12, w3 and the weights; None where not wanted."""
+    dy = _pitched(dy)
+    (stride_dy,) = _pitches(dy)
+    new = lambda shape, dtype: torch.empty(shape, device=x.device, dtype=dtype)  # noqa: E731
+    dx = new(x.shape, x.dtype) if wants[0] else None
+    dw12 = new(w12.shape, x.dtype) if wants[1] else None
+    dw3 = new(w3.shape, x.dtype) if wants[2] else None
+    dweights = new(plan.pairs, torch.float32) if wants[3] else None
+    workspace = new(plan.resources[1].backward_workspace_bytes, torch.uint8)
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    _cabi.call(x.device, _cabi.lib.tnx_moe_swiglu_backward, ctypes.byref(plan.problems[1]), dy.data_ptr(), stride_dy,
+               x.data_ptr(), w12.data_ptr(), w3.data_ptr(), saved.data_ptr(), ptr(dx), ptr(dw12), ptr(dw3),
+               ptr(dweights), workspace.data_ptr(), workspace.numel(), _cabi.status_word(x.device).data_ptr())
+    return dx, dw12, dw3, dweights
 
 
 def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
@@ -240,6 +253,37 @@ def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.
             and torch.is_grad_enabled():
         return _MoeSwiglu.apply(x, w12, w3, weights, ids, plan)
     return _moe_forward(plan, x, w12, w3, ids, weights, 0)[0]
+
+
+# The two passes of moe_swiglu as the custom operators call them: with operands of any strides, what is
+# kept between the passes in a tensor of its own.
+
+def _moe_plan(x, w12, w3, ids, weights, activation):
+    x, w12, w3 = _pitched(x), _pitched(w12), _pitched(w3)
+    return x, w12, w3, _MoePlan(x, w12, w3, ids, weights, activation)
+
+
+def moe_forward_kept(x, w12, w3, ids, weights, activation):
+    _check_moe(x, w12, w3, ids, weights, activation)
+    x, w12, w3, plan = _moe_plan(x, w12, w3, ids, weights, activation)
+    return _moe_forward(plan, x, w12, w3, ids.contiguous(), weights.contiguous(), 1)
+
+
+def moe_gradients_kept(dy, x, w12, w3, ids, saved, activation, wants):
+    weights = torch.empty(ids.shape, device=ids.device, dtype=torch.float32)  # (for the checks: `saved` has them)
+    x, w12, w3, plan = _moe_plan(x, w12, w3, ids, weights, activation)
+    return _moe_backward(plan, dy, x, w12, w3, saved, wants)
+
+
+def moe_saved_bytes(x, w12, w3, ids, activation) -> int:
+    """Size of what a training forward call keeps, from shapes alone."""
+    (n, d, two_f), n_out = map(int, w12.shape), int(w3.shape[2])
+    problem = _cabi.MoeProblem(int(x.shape[0]), n, int(ids.shape[1]), d, two_f // 2, n_out, _cabi.DTYPES[x.dtype],
+                               _cabi.ACTIVATIONS[activation], int(ids.dtype == torch.int64), 1, d, d * two_f, two_f,
+                               two_f // 2 * n_out, n_out, n_out)
+    res = _cabi.MoeResources()
+    _cabi.raise_for(_cabi.lib.tnx_moe_query(ctypes.byref(problem), ctypes.byref(res)))
+    return res.saved_bytes
 
 
 def _check_moe(x, w12, w3, ids, weights, activation) -> int:

@@ -84,22 +84,25 @@ class _GatedResidualNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dn):
-        y, residual, post, pre, gate, stats = ctx.saved_tensors
-        plan, device = ctx.plan, y.device
-        dh, dn = _cabi.rows_view(dh), _cabi.rows_view(dn)
-        dy = torch.empty(plan.shape, device=device, dtype=y.dtype)
-        dres = torch.empty_like(dy)
-        dpost, dpre = torch.empty((2, plan.shape[1]), device=device, dtype=post.dtype).unbind()
-        dgate = torch.empty(gate.shape, device=device, dtype=gate.dtype) if gate is not None else None
-        workspace = torch.empty(plan.workspace_bytes, device=device, dtype=torch.uint8)
-        _cabi.call(device, _cabi.lib.tnx_gated_residual_norm_backward, ctypes.byref(plan.problem),
-                   dh.data_ptr(), dh.stride(0), dn.data_ptr(), dn.stride(0), y.data_ptr(),
-                   residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
-                   gate.data_ptr() if gate is not None else None, stats.data_ptr(), dy.data_ptr(),
-                   dres.data_ptr(), dpost.data_ptr(), dpre.data_ptr(),
-                   dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(), plan.workspace_bytes,
-                   _cabi.status_word(device).data_ptr())
-        return dy, dres, dpost, dpre, dgate, None
+        return *_backward(ctx.plan, dh, dn, *ctx.saved_tensors), None
+
+
+def _backward(plan, dh, dn, y, residual, post, pre, gate, stats):
+    device = y.device
+    dh, dn = _cabi.rows_view(dh), _cabi.rows_view(dn)
+    dy = torch.empty(plan.shape, device=device, dtype=y.dtype)
+    dres = torch.empty_like(dy)
+    dpost, dpre = torch.empty((2, plan.shape[1]), device=device, dtype=post.dtype).unbind()
+    dgate = torch.empty(gate.shape, device=device, dtype=gate.dtype) if gate is not None else None
+    workspace = torch.empty(plan.workspace_bytes, device=device, dtype=torch.uint8)
+    _cabi.call(device, _cabi.lib.tnx_gated_residual_norm_backward, ctypes.byref(plan.problem),
+               dh.data_ptr(), dh.stride(0), dn.data_ptr(), dn.stride(0), y.data_ptr(),
+               residual.data_ptr(), post.data_ptr(), pre.data_ptr(),
+               gate.data_ptr() if gate is not None else None, stats.data_ptr(), dy.data_ptr(),
+               dres.data_ptr(), dpost.data_ptr(), dpre.data_ptr(),
+               dgate.data_ptr() if dgate is not None else None, workspace.data_ptr(), plan.workspace_bytes,
+               _cabi.status_word(device).data_ptr())
+    return dy, dres, dpost, dpre, dgate
 
 
 def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor,
@@ -118,19 +121,47 @@ def gated_residual_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: to
     if plan is None:
         plan = _cabi.remember(_plans, key, _NormPlan(y, residual, post_weight, pre_weight, gate, residual_scale, eps))
     if not plan.ready:  # as rows, and once more
-        rows = plan.shape[0]
-        if plan.form == _cabi.GATE_CHANNEL:
-            gate = gate.contiguous()
-        elif gate is not None:
-            gate = _cabi.rows_view(gate.reshape(rows, gate.shape[-1]))
-        h, n = gated_residual_norm(_cabi.rows_view(y.reshape(plan.shape)), _cabi.rows_view(residual.reshape(plan.shape)),
-                                   post_weight.contiguous(), pre_weight.contiguous(), gate, residual_scale, eps)
+        h, n = gated_residual_norm(*_as_rows(plan, y, residual, post_weight, pre_weight, gate), residual_scale, eps)
         return h.view(y.shape), n.view(y.shape)
     if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or post_weight.requires_grad or
                                     pre_weight.requires_grad or (gate is not None and gate.requires_grad)):
         return _GatedResidualNorm.apply(y, residual, post_weight, pre_weight, gate, plan)
     h, n, _ = _forward(plan, y, residual, post_weight, pre_weight, gate, False)
     return h, n
+
+
+def _as_rows(plan, y, residual, post_weight, pre_weight, gate):
+    """The operands of a call whose plan is not ready, as the kernels take them."""
+    if plan.form == _cabi.GATE_CHANNEL:
+        gate = gate.contiguous()
+    elif gate is not None:
+        gate = _cabi.rows_view(gate.reshape(plan.shape[0], gate.shape[-1]))
+    return (_cabi.rows_view(y.reshape(plan.shape)), _cabi.rows_view(residual.reshape(plan.shape)),
+            post_weight.contiguous(), pre_weight.contiguous(), gate)
+
+
+# The two passes as the custom operators call them: with operands of any strides and leading dimensions,
+# the reciprocal norms kept between the passes in a tensor of their own.
+
+def _ready_plan(y, residual, post_weight, pre_weight, gate, residual_scale, eps):
+    operands = (y, residual, post_weight, pre_weight, gate)
+    plan = _NormPlan(*operands, residual_scale, eps)
+    if not plan.ready:
+        operands = _as_rows(plan, *operands)
+        plan = _NormPlan(*operands, residual_scale, eps)
+    return plan, operands
+
+
+def norm_forward_kept(y, residual, post_weight, pre_weight, gate, residual_scale, eps):
+    plan, operands = _ready_plan(y, residual, post_weight, pre_weight, gate, residual_scale, eps)
+    h, n, stats = _forward(plan, *operands, True)
+    return h.view(y.shape), n.view(y.shape), stats
+
+
+def norm_gradients_kept(dh, dn, y, residual, post_weight, pre_weight, gate, stats, residual_scale, eps):
+    plan, operands = _ready_plan(y, residual, post_weight, pre_weight, gate, residual_scale, eps)
+    dy, dres, dpost, dpre, dgate = _backward(plan, dh.reshape(plan.shape), dn.reshape(plan.shape), *operands, stats)
+    return dy.view(y.shape), dres.view(y.shape), dpost, dpre, dgate if gate is None else dgate.view(gate.shape)
 
 
 def _check(y, residual, post_weight, pre_weight, gate, eps) -> int:
