@@ -408,7 +408,7 @@ int tnx_conv2d_forward(const tnx_conv2d_problem* problem, const tnx_config* conf
  * always distinct and in range.
  */
 typedef struct tnx_route_problem {
-  int32_t tokens, experts; /* experts <= 512                                               */
+  int32_t tokens, experts; /* tokens <= 2^31 - 4, experts <= 512                           */
   int32_t top_k;           /* <= 32 and <= the experts of top_groups groups                */
   int32_t groups;          /* divides experts, <= 32; 1 = no groups                        */
   int32_t top_groups;      /* 1 .. groups                                                  */

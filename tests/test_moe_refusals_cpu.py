@@ -221,3 +221,9 @@ def test_custom_ops_carry_gradients_without_a_device():
         assert not ops.moe_swiglu(x, w12, w3, i, w, "silu").requires_grad
     with torch.inference_mode():
         assert ops.moe_swiglu(x, w12, w3, i, w, "silu").shape == (5, 32)
+
+
+@pytest.mark.parametrize("tokens", [2 ** 31 - 3, 2 ** 31 - 1])
+def test_route_refuses_more_tokens_than_it_can_number(tokens):
+    assert lib.tnx_route_experts(ctypes.byref(route(tokens=tokens)), PTR, None, PTR, PTR, None) == _cabi.ERR_INVALID
+    assert "tokens" in _cabi.last_error()

@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kWarps = 4;  // tokens of a block
 constexpr int kMaxExperts = 512;
+constexpr int kMaxTokens = 2147483647 - (kWarps - 1);
 constexpr int kMaxPicks = 32;  // lane i keeps pick i
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -537,9 +538,10 @@ int route_check(const tnx_route_problem* p) {
     set_error("unknown dtype %d", p->dtype);
     return TNX_ERR_INVALID;
   }
-  if (p->tokens < 0 || p->experts < 1 || p->experts > kMaxExperts) {
-    set_error("routing needs tokens >= 0 and 1 <= experts <= %d (got %d tokens, %d experts)", kMaxExperts, p->tokens,
-              p->experts);
+  // (the number of a block's last token is an int too)
+  if (p->tokens < 0 || p->tokens > kMaxTokens || p->experts < 1 || p->experts > kMaxExperts) {
+    set_error("routing needs 0 to %d tokens and 1 <= experts <= %d (got %d tokens, %d experts)", kMaxTokens, kMaxExperts,
+              p->tokens, p->experts);
     return TNX_ERR_INVALID;
   }
   if (p->groups < 1 || p->groups > 32 || p->experts % p->groups != 0 || p->top_groups < 1 ||
