@@ -112,16 +112,18 @@ __device__ __forceinline__ float2 sigmoid_and_rest(float l) {
   const float e = expf(-fabsf(l)), near = 1.f / (1.f + e), far = e * near;
   return l >= 0.f ? make_float2(near, far) : make_float2(far, near);
 }
-// A renormalised sigmoid's weight of the lane's pick, before the division by the warp's sum of them:
-// sigmoid(l) / exp(m), m the largest of the picks' min(l, 0), so that it does not matter whether fp32
-// holds the scores (below l = -103 it does not).  Scores that are 0 in 64 bits (1 / (1 + exp(-l)) with
-// an exponential that overflows: l < -709.78, a type's lowest value among them) stay 0.
+// A renormalised sigmoid's weight of the lane's pick, before the division by the warp's sum of them,
+// for picks whose scores themselves have a sum below kFewScores: sigmoid(l) / exp(m), m the largest of
+// the picks' min(l, 0), so that it does not matter whether fp32 holds the scores (below l = -103 it
+// does not).  Scores that are 0 in 64 bits (1 / (1 + exp(-l)) with an exponential that overflows:
+// l < -709.78, a type's lowest value among them) stay 0.  (Above the limit scores that fp32 does not
+// hold are weights below 2^-125.)
+constexpr float kFewScores = 1e-7f;
 __device__ __forceinline__ float sigmoid_share(float l, bool picked) {
   const bool zero = !picked || l < -709.78265f;
   const float a = fminf(l, 0.f);
-  const float m = warp_max(zero || l != l ? -CUDART_INF_F : a);
+  const float m = warp_max(zero ? -CUDART_INF_F : a);
   if (zero) return 0.f;
-  if (l != l) return l;
   // (the rounding of a - m would be an error of the weight's 80 units in the last place at a - m = -80)
   const float d = a - m, b = d - a, rest = (a - (d - b)) - (m + b);
   const float e = expf(d);
@@ -413,10 +415,12 @@ __global__ void __launch_bounds__(kWarps * 32, VPT <= 8 ? 8 : 4) route_kernel(co
       // a softmax over the picks alone: the same ratio, and no score underflows in it
       const float top = warp_max(picked ? my_logit : -CUDART_INF_F);
       w = picked ? expf(my_logit - (top == -CUDART_INF_F ? 0.f : top)) : 0.f;
-    } else {
-      w = sigmoid_share(my_logit, picked);
     }
-    const float sum = warp_sum(picked ? w : 0.f);
+    float sum = warp_sum(picked ? w : 0.f);
+    if (!softmax && sum < kFewScores) {
+      w = sigmoid_share(my_logit, picked);
+      sum = warp_sum(w);
+    }
     w = sum == 0.f ? 0.f : w / sum;
   }
   if (picked) {
@@ -483,22 +487,29 @@ __global__ void __launch_bounds__(kWarps * 32) route_backward_kernel(const Route
       out[j] = score * (d - base);
     }
   } else {
-    const float2 s = softmax ? make_float2(0.f, 1.f) : sigmoid_and_rest(logit);  // s, 1 - s
-    if (p.renormalize) {
-      float r;
-      if (softmax) {
-        const float top = warp_max(logit);
-        r = picked ? expf(logit - (top == -CUDART_INF_F ? 0.f : top)) : 0.f;
-      } else {
-        r = sigmoid_share(logit, picked);
+    float r, sum, rest = 1.f;  // rest: 1 - s
+    if (softmax) {
+      const float top = warp_max(logit);
+      r = picked ? expf(logit - (top == -CUDART_INF_F ? 0.f : top)) : 0.f;
+      sum = warp_sum(r);
+    } else {
+      const float2 s = sigmoid_and_rest(logit);
+      r = picked ? s.x : 0.f;
+      rest = s.y;
+      sum = 1.f;
+      if (p.renormalize) {
+        sum = warp_sum(r);
+        if (sum < kFewScores) {
+          r = sigmoid_share(logit, picked);
+          sum = warp_sum(r);
+        }
       }
-      const float sum = warp_sum(r);
+    }
+    if (p.renormalize) {
       r = sum == 0.f ? 0.f : r / sum;
       base = warp_sum(picked ? dw * r : 0.f);
-      g = r * (dw - base) * s.y;
-    } else {
-      g = dw * s.x * s.y;
     }
+    g = r * (dw - base) * rest;
     for (int i = 0; i < p.top_k; ++i) {
       const int pick = __shfl_sync(kAll, e, i);
       const float v = __shfl_sync(kAll, g, i);
