@@ -239,6 +239,11 @@ def moe_swiglu(x: torch.Tensor, w12: torch.Tensor, w3: torch.Tensor, ids: torch.
     and an expert may stand in several slots of a token.  ``activation``: "silu", "sigmoid" or
     "none" (``swiglu`` and ``glu`` take the same).
 
+    The hidden activation, times its weight, is rounded to the operands' type between the two products
+    (not for a single token without gradients).  A call's scratch is 4 bytes per (token, slot) pair and column of ``y``, times
+    up to eight where there are few tiles, and 2 per pair and column of ``x`` and of the hidden
+    activation; training keeps 10 per pair and hidden column.
+
     Gradients flow to ``x``, ``w12``, ``w3`` and ``weights``.  The routing stays on the device: no
     call waits for it.  Results do not depend on timing (every sum has a fixed order)."""
     _cabi.refuse_tangents(x, w12, w3, weights)
