@@ -238,3 +238,19 @@ def test_custom_ops_refuse_second_derivatives_and_tangents():
                 others = [a.detach() for a in args]
                 with pytest.raises(RuntimeError):
                     block_of_ops(others[:j] + [dual] + others[j + 1:], case["bias"].to(DEV))
+
+
+@pytest.mark.parametrize("traced", [False, True])
+def test_custom_ops_with_one_output_unused(traced):
+    case = make(20, 16, 64, 32, seed=4)
+    bias = case["bias"].to(DEV)
+    for used in (0, 1):
+        args = leaves(case)
+        want = torch.autograd.grad(block(args, bias)[used].float().sum(), args, allow_unused=True)
+        fn = lambda *a: block_of_ops(a, bias)[used]  # noqa: E731
+        if traced:
+            fn = torch.compile(fn, backend="aot_eager", fullgraph=True)
+        args = leaves(case)
+        got = torch.autograd.grad(fn(*args).float().sum(), args, allow_unused=True)
+        for a, b in zip(want, got):
+            assert torch.equal(a, b if b is not None else torch.zeros_like(a))
